@@ -82,6 +82,25 @@ _SIGNATURES = {
                                                  ctypes.c_float, _c_void_p, _i64, _i64,
                                                  _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                                  _i64, _c_void_p]),
+    # mtl_paged.h
+    "mtl_paged_attention_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32, _i64, _i32]),
+    "mtl_paged_attention": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32,
+                                   _i32, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p, _i64,
+                                   _c_void_p]),
+    "mtl_paged_write": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                               _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64,
+                               ctypes.c_float, _i32, _i32, _c_void_p, _c_void_p]),
+    "mtl_pages_workspace_bytes": (_i64, [_i64, _i64]),
+    "mtl_pages_extend": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
+                                _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "mtl_pages_fork": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64,
+                              _c_void_p]),
+    "mtl_pages_truncate": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
+                                  _i64, _c_void_p]),
+    "mtl_pages_compact": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
+                                 _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "mtl_pages_copy": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                              _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p]),
     # tuning knobs (not part of the headers)
     "mtl_w4_gemm_splits": (_i32, [_i64, _i64]),
     "mtl_w4_gemm_partials": (_i32, [_c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _c_void_p,
@@ -172,6 +191,26 @@ _SIGNATURES = {
     "mtl_w4_strip": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p]),
 }
 
+
+class PagePool(ctypes.Structure):
+    """``mtl_page_pool``: one layer's pages."""
+    _fields_ = [("k", _c_void_p), ("v", _c_void_p), ("pages", _i64), ("k_page", _i64),
+                ("k_head", _i64), ("k_token", _i64), ("v_page", _i64), ("v_head", _i64),
+                ("v_token", _i64), ("kv_heads", _i32), ("page_size", _i32), ("head_dim", _i32),
+                ("type", _i32), ("k_scale", _c_void_p), ("v_scale", _c_void_p)]
+
+
+class PageTable(ctypes.Structure):
+    """``mtl_page_table``: the pages of a batch of sequences."""
+    _fields_ = [("table", _c_void_p), ("ld", _i64), ("width", _i64), ("seqs", _i64)]
+
+
+class PageState(ctypes.Structure):
+    """``mtl_page_state``: what the page bookkeeping works on."""
+    _fields_ = [("table", _c_void_p), ("ld", _i64), ("width", _i64), ("seqs", _i64),
+                ("lens", _c_void_p), ("refs", _c_void_p), ("pages", _i64), ("page_size", _i32)]
+
+
 class StripGeometry(ctypes.Structure):
     """``mtl_strip_geometry``: the strip GEMV's launch shape (0 = automatic per field)."""
     _fields_ = [("strips_per_wg", ctypes.c_int32), ("blocks_per_wave", ctypes.c_int32),
@@ -198,6 +237,7 @@ LAYOUT_ROWS, LAYOUT_TILED, LAYOUT_STRIP, LAYOUT_STRIP_QSZ = 0, 1, 2, 3
 XPART_HALVES = 1 << 30                # MTL_XPART_HALVES, OR'ed into mtl_w4_gemm_residual's xsplits
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL = 0, 1, 2
 META_GPTQ, META_QSZ = 0, 1
+T_BF16, T_F16, T_E4M3 = 0, 1, 2
 
 _lib = None
 

@@ -1,7 +1,6 @@
 """Build recipe of ``libmtl_hip.so``: every ``csrc/*.hip`` compiled for gfx950.
 
-The library exposes only the plain C ABI declared in ``include/mtl_gptq.h`` and
-``include/mtl_decode.h`` (raw device pointers, sizes, a ``hipStream_t``), so it
+The library exposes only the plain C ABI declared in ``include/*.h`` (raw device pointers, sizes, a ``hipStream_t``), so it
 links against whichever HIP runtime the process already has loaded (torch's).
 """
 from __future__ import annotations
@@ -53,7 +52,7 @@ def _run(cmd: list[str]) -> str:
     return err
 
 
-TORCH_OPS_SRC = os.path.join(PKG_DIR, "torch_ops", "mtl_torch_ops.cpp")
+TORCH_OPS_SRCS = sorted(glob.glob(os.path.join(PKG_DIR, "torch_ops", "*.cpp")))
 TORCH_OPS_PATH = os.path.join(PKG_DIR, "libmtl_torch_ops.so")
 
 
@@ -69,7 +68,7 @@ def torch_ops_command(out: str = TORCH_OPS_PATH) -> list[str]:
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
             *[f"-I{p}" for p in incs], "-I/opt/rocm/include", f"-I{os.path.join(ROOT, 'include')}",
-            TORCH_OPS_SRC, f"-L{os.path.join(tdir, 'lib')}", f"-L{PKG_DIR}",
+            *TORCH_OPS_SRCS, f"-L{os.path.join(tdir, 'lib')}", f"-L{PKG_DIR}",
             "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{os.path.join(tdir, 'lib')}",
             "-lmtl_hip", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-o", out]
 
