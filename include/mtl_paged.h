@@ -62,7 +62,8 @@ typedef struct mtl_page_table {
  * fp32 softmax and sums.  Lengths past width * page_size count as that, negative ones as 0.
  *   q    [seqs, n_heads, head_dim] of q_type (bf16 or f16), rows ldq and heads ldh elements
  *        apart (multiples of 8, base 16-byte aligned)
- *   out  [seqs, n_heads, head_dim] of q_type, contiguous; a sequence without positions: 0
+ *   out  [seqs, n_heads, head_dim] of q_type, contiguous, 16-byte aligned; a sequence without
+ *        positions: 0
  *   lse  NULL, or fp32 [seqs, n_heads]: the natural logarithm of sum_j exp(s_j) (-inf for a
  *        sequence without positions)
  *   workspace  mtl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, any content,
