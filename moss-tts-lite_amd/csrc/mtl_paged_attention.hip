@@ -15,9 +15,12 @@
 //   maximum grew.  Weights enter the product as two rows-type numbers, the rounded weight and
 //   what the rounding left: the output is then off by its own rounding alone (with one, by
 //   1.4 times that).
-// * Sequences are cut into chunks of equal length, chosen on the device from the lengths so that
-//   all chunks together fill the chip; chunks of one sequence are joined by a second launch in
-//   chunk order.  Short tables (at most kDirectPositions) need neither.
+// * A launch of kWorkgroups workgroups, all on the chip at once, shares the blocks of 128
+//   positions of all sequences evenly: the blocks stand in one row, sequence after sequence, and
+//   each workgroup of a kv head finds its piece of that row on the device from the lengths.  A
+//   sequence that several workgroups have pieces of is joined by a second launch, piece after
+//   piece.  Short tables (at most kDirectPositions) need neither: a workgroup a sequence and
+//   kv head.
 #include "mtl_paged_pool.h"
 
 namespace mtl {
@@ -31,28 +34,54 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;               // positions a wave takes at a time
 constexpr int kSplitWaves = 4;
-constexpr int kBlock = kTile * kSplitWaves;   // chunks are multiples of this
-constexpr int kTargetChunks = 2048;     // chunks of all heads together, at most this many ...
-constexpr int kDirectPositions = 1024;
+constexpr int kBlock = kTile * kSplitWaves;
+constexpr int kWorkgroups = 512;        // 2 of 4 waves on each of 256 CUs
+constexpr int kDirectPositions = 512;
 constexpr int kDirectWaves = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// The workspace: [groups][heads][head_dim] sums and [groups][heads][2] (maximum, sum) in fp32,
-// then int2 [seqs] (first chunk, chunks), for `groups` workgroups of up to 16 query heads.
+// How the launch is shared: `pieces` workgroups for each unit (up to 16 query heads of a kv
+// head).  The workspace holds two rows of sums a workgroup, its first piece's and its last's
+// (fp32 [pieces * units][2][tile_heads][head_dim], then (maximum, sum) for each), and int4
+// [seqs] with what the second launch needs.
 struct Split {
-  int64_t groups;
-  int head_tiles, tile_heads;
+  int units, head_tiles, tile_heads, pieces;
+  int64_t rows;
 };
 
-__host__ __device__ inline Split split_of(int64_t seqs, int n_heads, int kv_heads) {
+__host__ __device__ inline Split split_of(int n_heads, int kv_heads) {
   Split s;
   const int g = n_heads / kv_heads;
   s.tile_heads = g < 16 ? g : 16;
   s.head_tiles = (g + 15) / 16;
-  const int64_t units = (int64_t)kv_heads * s.head_tiles;
-  s.groups = (kTargetChunks / units + seqs) * units;
+  s.units = kv_heads * s.head_tiles;
+  s.pieces = s.units < kWorkgroups ? kWorkgroups / s.units : 1;
+  s.rows = (int64_t)s.pieces * s.units * 2 * s.tile_heads;
   return s;
+}
+
+// K and V are read once: loads that leave no trace in the caches read 7.1 TB/s here, others 6.4.
+// With more than 16 query heads to a kv head its rows are read again, from the caches.
+template <bool ONCE, class T>
+__device__ __forceinline__ T load(const char* p) {
+  const T* q = reinterpret_cast<const T*>(p);
+  return ONCE ? __builtin_nontemporal_load(q) : *q;
+}
+
+// A lane's 32-bit offset, formed where it is used: the load then takes base and offset as they
+// are.  Without this the compiler keeps every offset as a 64-bit pair (24 registers).
+__device__ __forceinline__ uint32_t fresh(int offset) {
+  uint32_t o = (uint32_t)offset;
+  asm volatile("" : "+v"(o));
+  return o;
+}
+
+// table[i] for an i that is the same in all lanes, as a scalar load: a vector load would have
+// the wave wait for the K and V in flight before it.
+__device__ __forceinline__ int uniform_load(const int32_t* p, int64_t i) {
+  typedef const int32_t __attribute__((address_space(4)))* Constant;
+  return ((Constant)(uintptr_t)p)[i];
 }
 
 template <int QT>
@@ -96,7 +125,7 @@ __device__ __forceinline__ int clamp_len(int32_t len, int64_t cap) {
 }
 
 // One chunk of one sequence for up to 16 query heads of one kv head.
-template <int QT, int KT, int D, int WAVES>
+template <int QT, int KT, int D, int WAVES, bool ONCE>
 struct Attend {
   static constexpr int E = KT == MTL_T_E4M3 ? 1 : 2;    // bytes of a stored element
   static constexpr int KL = D * E / 64;                 // 16-byte loads of a lane's K row
@@ -108,7 +137,7 @@ struct Attend {
   uint32_t vf[8][VW];
   floatx4 acc[VD];
   float m, l, c;                                        // c: scale to base 2
-  int lane, r, g, k_lane, v_lane, k_row, v_row;
+  int r, g, k_lane, v_lane, v_row;
 
   // The pages of the tile's two halves of 16 positions; -1: none.
   struct Tile {
@@ -122,7 +151,7 @@ struct Attend {
     for (int h = 0; h < 2; ++h) {
       const int p = p0 + 16 * h;
       int id = -1;
-      if (p < end) id = row[p >> shift];
+      if (p < end) id = uniform_load(row, p >> shift);
       t.page[h] = (uint32_t)id < (uint32_t)n_pages ? id : -1;
     }
     return t;
@@ -137,9 +166,9 @@ struct Attend {
       const int id = t.page[h] < 0 ? 0 : t.page[h];
       const char* p = base + (id * pool.k_page + ((p0 + 16 * h) & (pool.page_size - 1)) *
                                                      pool.k_token) * E;
+      const uint32_t o = fresh(k_lane);
 #pragma unroll
-      for (int s = 0; s < KL; ++s)
-        kf[h][s] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(k_lane + 64 * s));
+      for (int s = 0; s < KL; ++s) kf[h][s] = load<ONCE, u32x4>(p + o + 64 * s);
     }
   }
 
@@ -152,40 +181,47 @@ struct Attend {
                                                      pool.v_token) * E;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const char* q = p + (uint32_t)(v_lane + j * v_row);
+        const char* q = p + fresh(v_lane + j * v_row);
         if (VW == 4) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(q);
+          const u32x4 x = load<ONCE, u32x4>(q);
           vf[4 * h + j][0] = x.x; vf[4 * h + j][1 % VW] = x.y;
           vf[4 * h + j][2 % VW] = x.z; vf[4 * h + j][3 % VW] = x.w;
         } else if (VW == 2) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(q);
+          const u32x2 x = load<ONCE, u32x2>(q);
           vf[4 * h + j][0] = x.x; vf[4 * h + j][1 % VW] = x.y;
         } else {
-          vf[4 * h + j][0] = *reinterpret_cast<const uint32_t*>(q);
+          vf[4 * h + j][0] = load<ONCE, uint32_t>(q);
         }
       }
     }
   }
 
   __device__ __forceinline__ void scores(float (&s)[8]) const {
+    floatx4 a[2] = {};                    // two chains of products, in turn
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      floatx4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < KL; ++i) {
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
+      for (int h = 0; h < 2; ++h) {
         const u32x4 x = kf[h][i];
-        if (E == 2) {
-          a = mfma<QT>(x, qf[i], a);
-        } else {
-          a = mfma<QT>(u32x4{widen<QT, false>(x.x), widen<QT, true>(x.x), widen<QT, false>(x.y),
-                             widen<QT, true>(x.y)}, qf[(2 * i) % QS], a);
-          a = mfma<QT>(u32x4{widen<QT, false>(x.z), widen<QT, true>(x.z), widen<QT, false>(x.w),
-                             widen<QT, true>(x.w)}, qf[(2 * i + 1) % QS], a);
+        if (E == 2)
+          a[h] = mfma<QT>(x, qf[i], a[h]);
+        else
+          a[h] = mfma<QT>(u32x4{widen<QT, false>(x.x), widen<QT, true>(x.x),
+                                widen<QT, false>(x.y), widen<QT, true>(x.y)},
+                          qf[(2 * i) % QS], a[h]);
+      }
+      if (E == 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 x = kf[h][i];
+          a[h] = mfma<QT>(u32x4{widen<QT, false>(x.z), widen<QT, true>(x.z),
+                                widen<QT, false>(x.w), widen<QT, true>(x.w)},
+                          qf[(2 * i + 1) % QS], a[h]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * h + i] = a[i] * c;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = a[j >> 2][j & 3] * c;
   }
 
   // Positions past the end and without a page: score -inf, value 0 (what is stored there may
@@ -230,21 +266,27 @@ struct Attend {
       lo[j] = b;
     }
 #pragma unroll
-    for (int d = 0; d < VD; ++d) {
-      u32x4 v;
+    for (int d0 = 0; d0 < VD; d0 += 2) {  // two accumulators in turn
+      u32x4 v[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a = vf[2 * j][d * E / 4], b = vf[2 * j + 1][d * E / 4];
-        if (E == 2) {
-          v[j] = __builtin_amdgcn_perm(b, a, (d & 1) ? 0x07060302u : 0x05040100u);
-        } else {
-          // bytes (a0 b0 a1 b1) or (a2 b2 a3 b3): two dims' pairs of positions
-          const uint32_t x = __builtin_amdgcn_perm(b, a, (d & 2) ? 0x07030602u : 0x05010400u);
-          v[j] = (d & 1) ? widen<QT, true>(x) : widen<QT, false>(x);
+      for (int e = 0; e < 2; ++e) {
+        const int d = d0 + e;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a = vf[2 * j][d * E / 4], b = vf[2 * j + 1][d * E / 4];
+          if (E == 2) {
+            v[e][j] = __builtin_amdgcn_perm(b, a, e ? 0x07060302u : 0x05040100u);
+          } else {
+            // bytes (a0 b0 a1 b1) or (a2 b2 a3 b3): two dims' pairs of positions
+            const uint32_t x = __builtin_amdgcn_perm(b, a, (d & 2) ? 0x07030602u : 0x05010400u);
+            v[e][j] = e ? widen<QT, true>(x) : widen<QT, false>(x);
+          }
         }
       }
-      acc[d] = mfma<QT>(v, hi, acc[d]);
-      acc[d] = mfma<QT>(v, lo, acc[d]);
+      acc[d0] = mfma<QT>(v[0], hi, acc[d0]);
+      acc[d0 + 1] = mfma<QT>(v[1], hi, acc[d0 + 1]);
+      acc[d0] = mfma<QT>(v[0], lo, acc[d0]);
+      acc[d0 + 1] = mfma<QT>(v[1], lo, acc[d0 + 1]);
     }
   }
 
@@ -272,225 +314,286 @@ struct Attend {
     load_v(pool, vb, t, p0);
     int p1 = p0 + WAVES * kTile;
     Tile next = pages(row, shift, p1, end, pool.pages);
-    while (true) {
-      float s[8];
+    float s[8];
+    // The next tile's K is loaded once this one's scores are formed, its V once this one's values
+    // are summed.  The last tile stands apart: a load under a condition would have the compiler
+    // wait for all loads wherever it joins.
+    while (p1 < end) {
       scores(s);
-      const bool more = p1 < end;
-      if (more) load_k(pool, kb, next, p1);
-      if (p0 + kTile > end || t.page[0] < 0 || t.page[1] < 0) mask(s, t, p0, end);
+      load_k(pool, kb, next, p1);
+      if (t.page[0] < 0 || t.page[1] < 0) mask(s, t, p0, end);
       weights(s);
       values(s);
-      if (!more) break;
       load_v(pool, vb, next, p1);
       t = next;
       p0 = p1;
       p1 += WAVES * kTile;
       next = pages(row, shift, p1, end, pool.pages);
     }
+    scores(s);
+    if (p0 + kTile > end || t.page[0] < 0 || t.page[1] < 0) mask(s, t, p0, end);
+    weights(s);
+    values(s);
   }
 };
 
-// Chunk of a workgroup: the sequence, its positions and how many chunks it has.
-struct Chunk {
-  int seq, begin, end, count;
+// The blocks of all sequences in one row, cut into `pieces` parts that differ by one block at
+// most.
+struct Cuts {
+  int each, extra;
+  __device__ __forceinline__ Cuts(int total, int pieces) : each(total / pieces),
+                                                           extra(total % pieces) {}
+  __device__ __forceinline__ int start(int piece) const {
+    return piece * each + min(piece, extra);
+  }
+  __device__ __forceinline__ int piece_of(int block) const {
+    const int longer = extra * (each + 1);
+    return block < longer ? block / (each + 1) : extra + (block - longer) / each;
+  }
 };
 
-// Where group `slot` of the launch belongs.  Every wave finds it by itself: a lane counts the
-// blocks of a run of sequences, the sum over the wave gives the chunks' length, a scan over the
-// lanes' chunks the place.  Returns false past the last chunk.
-__device__ __forceinline__ bool find_chunk(const int32_t* __restrict__ lens, int64_t seqs,
-                                           int64_t cap, int units, int slot, Chunk& c) {
-  const int lane = threadIdx.x & 63;
-  const int per = (int)((seqs + 63) / 64);
-  const int64_t s0 = (int64_t)lane * per;
-  int blocks = 0;
-  for (int i = 0; i < per; ++i)
-    if (s0 + i < seqs) blocks += (clamp_len(lens[s0 + i], cap) + kBlock - 1) / kBlock;
-  int total = blocks;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  const int64_t work = (int64_t)total * units;
-  int len = (int)((work + kTargetChunks - 1) / kTargetChunks);     // blocks of a chunk
-  len = len < 1 ? 1 : len;
-  int chunks = 0;
-  for (int i = 0; i < per; ++i)
-    if (s0 + i < seqs) {
-      const int n = ((clamp_len(lens[s0 + i], cap) + kBlock - 1) / kBlock + len - 1) / len;
-      chunks += n < 1 ? 1 : n;
-    }
-  int upto = chunks;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(upto, o);
-    if (lane >= o) upto += y;
-  }
-  const uint64_t past = __ballot(slot < upto);
-  if (past == 0) return false;
-  const int at = __builtin_ctzll(past);
-  int first = __builtin_amdgcn_readlane(upto - chunks, at);
-  for (int64_t s = (int64_t)at * per;; ++s) {
-    const int n_pos = clamp_len(lens[s], cap);
-    int n = ((n_pos + kBlock - 1) / kBlock + len - 1) / len;
-    n = n < 1 ? 1 : n;
-    if (slot < first + n) {
-      const int64_t begin = (int64_t)(slot - first) * len * kBlock;
-      const int64_t end = begin + (int64_t)len * kBlock;
-      c.seq = (int)s;
-      c.begin = (int)begin;
-      c.end = end < n_pos ? (int)end : n_pos;
-      c.count = n;
-      return true;
-    }
-    first += n;
-  }
+__device__ __forceinline__ int blocks_of(int len) { return (len + kBlock - 1) / kBlock; }
+
+// Inclusive sum over the lanes of a wave (all active).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
 }
 
-// DIRECT: workgroup (unit, sequence) takes the whole sequence.
-template <int QT, int KT, int D, int WAVES, bool DIRECT>
-__global__ void __launch_bounds__(WAVES * 64) paged_attention_kernel(
-    const uint16_t* __restrict__ q, int64_t ldq, int64_t ldh, PagePool pool,
-    const int32_t* __restrict__ table, int64_t ldt, int64_t cap, int64_t seqs,
-    const int32_t* __restrict__ lens, int n_heads, int head_tiles, int tile_heads, float scale,
-    uint16_t* __restrict__ out, float* __restrict__ lse, float* __restrict__ part,
-    float* __restrict__ part_ml, int2* __restrict__ plan) {
-  extern __shared__ float lds[];
-  constexpr int LD = D + 4;
-  const int units = pool.kv_heads * head_tiles;
-  Chunk ch;
-  int unit;
-  if (DIRECT) {
-    unit = blockIdx.x % units;
-    ch.seq = blockIdx.x / units;
-    ch.begin = 0;
-    ch.end = clamp_len(lens[ch.seq], cap);
-    ch.count = 1;
-  } else {
-    unit = blockIdx.x % units;
-    const int slot = blockIdx.x / units;
-    if (!find_chunk(lens, seqs, cap, units, slot, ch)) return;
-    if (unit == 0 && ch.begin == 0 && threadIdx.x == 0) plan[ch.seq] = make_int2(slot, ch.count);
+// Every wave finds its place by itself: a lane counts the blocks of a run of `per` sequences.
+struct Scan {
+  int per, len, upto, total;
+  __device__ __forceinline__ Scan(const int32_t* __restrict__ lens, int seqs, int64_t cap) {
+    const int lane = threadIdx.x & 63;
+    per = (seqs + 63) / 64;
+    const int64_t s0 = (int64_t)lane * per;
+    int blocks = 0;
+    for (int i = 0; i < per; ++i) {
+      len = s0 + i < seqs ? clamp_len(lens[s0 + i], cap) : 0;
+      blocks += blocks_of(len);
+    }
+    upto = wave_scan(blocks);
+    total = __builtin_amdgcn_readlane(upto, 63);
   }
-  ch.seq = __builtin_amdgcn_readfirstlane(ch.seq);
-  ch.begin = __builtin_amdgcn_readfirstlane(ch.begin);
-  ch.end = __builtin_amdgcn_readfirstlane(ch.end);
-  ch.count = __builtin_amdgcn_readfirstlane(ch.count);
-  const int kvh = unit / head_tiles, group = n_heads / pool.kv_heads;
-  const int h0 = kvh * group + (unit % head_tiles) * 16;
+};
+
+// The output of one query head of one sequence from its sum o (4 dims), base-2 maximum and
+// weights' sum.
+template <int QT, int D>
+__device__ __forceinline__ void write_out(uint16_t* __restrict__ out, float* __restrict__ lse,
+                                          int64_t head, int d, floatx4 o, float top, float sum,
+                                          float vs) {
+  const float f = sum == 0.f ? 0.f : vs / sum;
+  *reinterpret_cast<u32x2*>(out + head * D + d) =
+      u32x2{pack_out<QT>(o[0] * f, o[1] * f), pack_out<QT>(o[2] * f, o[3] * f)};
+  if (lse && d == 0)
+    lse[head] = sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+struct Rows {
+  const uint16_t* q;
+  int64_t ldq, ldh;
+  const int32_t* table;
+  int64_t ldt, cap;
+  const int32_t* lens;
+  int seqs, n_heads, head_tiles, tile_heads, pieces;
+  float scale;
+  uint16_t* out;
+  float* lse;
+  float* part;
+  float* part_ml;
+  int4* plan;
+};
+
+// Positions [begin, end) of a sequence for one unit; the waves' results are joined through LDS
+// into out (row < 0) or into a row of the workspace.
+template <int QT, int KT, int D, int WAVES, bool ONCE>
+__device__ __forceinline__ void attend_piece(const Rows& a, const PagePool& pool, int unit, int seq,
+                                             int begin, int end, int64_t row, float* lds) {
+  constexpr int LD = D + 4;
+  const int kvh = unit / a.head_tiles, group = a.n_heads / pool.kv_heads;
+  const int h0 = kvh * group + (unit % a.head_tiles) * 16;
   const int heads = min(16, (kvh + 1) * group - h0);
   const int wave = wave_id();
 
-  Attend<QT, KT, D, WAVES> a;
-  a.lane = threadIdx.x & 63;
-  a.r = a.lane & 15;
-  a.g = a.lane >> 4;
-  a.m = -__builtin_inff();
-  a.l = 0.f;
-  a.c = scale * (pool.k_scale ? pool.k_scale[kvh] : 1.f) * kLog2e;
+  Attend<QT, KT, D, WAVES, ONCE> w;
+  // what depends on the thread is formed anew for each piece, before and after the loop over
+  // its tiles: kept over the loop it costs 30 registers
+  int thread = (int)fresh(threadIdx.x);
+  w.r = thread & 15;
+  w.g = (thread & 63) >> 4;
+  w.m = -__builtin_inff();
+  w.l = 0.f;
+  w.c = a.scale * (pool.k_scale ? pool.k_scale[kvh] : 1.f) * kLog2e;
 #pragma unroll
-  for (int d = 0; d < a.VD; ++d) a.acc[d] = floatx4{0.f, 0.f, 0.f, 0.f};
-  a.load_q(q + ch.seq * ldq + h0 * ldh, ldh, heads);
-  a.run(pool, table + ch.seq * ldt, kvh, ch.begin, ch.end, wave);
+  for (int d = 0; d < w.VD; ++d) w.acc[d] = floatx4{0.f, 0.f, 0.f, 0.f};
+  w.load_q(a.q + seq * a.ldq + h0 * a.ldh, a.ldh, heads);
+  w.run(pool, a.table + seq * a.ldt, kvh, begin, end, wave);
 
-  // join the waves
-  float* ml = lds + WAVES * tile_heads * LD;
-  a.l = xor32_add(xor16_add(a.l));
-  if (a.r < heads) {
-    float* o = lds + (wave * tile_heads + a.r) * LD + a.VD * 4 * a.g;
+  float* ml = lds + WAVES * a.tile_heads * LD;
+  w.l = xor32_add(xor16_add(w.l));
+  thread = (int)fresh(threadIdx.x);
+  const int r = thread & 15, g = (thread & 63) >> 4;
+  if (r < heads) {
+    float* o = lds + (wave * a.tile_heads + r) * LD + w.VD * 4 * g;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int d = 0; d < a.VD; d += 4)
-        *reinterpret_cast<floatx4*>(o + i * a.VD + d) =
-            floatx4{a.acc[d][i], a.acc[d + 1][i], a.acc[d + 2][i], a.acc[d + 3][i]};
-    if (a.g == 0) {
-      ml[2 * (wave * 16 + a.r)] = a.m;
-      ml[2 * (wave * 16 + a.r) + 1] = a.l;
+      for (int d = 0; d < w.VD; d += 4)
+        *reinterpret_cast<floatx4*>(o + i * w.VD + d) =
+            floatx4{w.acc[d][i], w.acc[d + 1][i], w.acc[d + 2][i], w.acc[d + 3][i]};
+    if (g == 0) {
+      ml[2 * (wave * 16 + r)] = w.m;
+      ml[2 * (wave * 16 + r) + 1] = w.l;
     }
   }
   __syncthreads();
-  const float vs = pool.v_scale ? pool.v_scale[kvh] : 1.f;
-  for (int i = threadIdx.x; i < heads * (D / 4); i += WAVES * 64) {
+  for (int i = thread; i < heads * (D / 4); i += WAVES * 64) {
     const int h = i / (D / 4), d = 4 * (i % (D / 4));
     float top = -__builtin_inff();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ml[2 * (w * 16 + h)]);
+    for (int x = 0; x < WAVES; ++x) top = fmaxf(top, ml[2 * (x * 16 + h)]);
     const float mu = top == -__builtin_inff() ? 0.f : top;
     float sum = 0.f;
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float e = __builtin_amdgcn_exp2f(ml[2 * (w * 16 + h)] - mu);
-      sum = fmaf(ml[2 * (w * 16 + h) + 1], e, sum);
-      o += e * *reinterpret_cast<const floatx4*>(lds + (w * tile_heads + h) * LD + d);
+    for (int x = 0; x < WAVES; ++x) {
+      const float e = __builtin_amdgcn_exp2f(ml[2 * (x * 16 + h)] - mu);
+      sum = fmaf(ml[2 * (x * 16 + h) + 1], e, sum);
+      o += e * *reinterpret_cast<const floatx4*>(lds + (x * a.tile_heads + h) * LD + d);
     }
-    if (ch.count == 1) {
-      const float f = sum == 0.f ? 0.f : vs / sum;
-      *reinterpret_cast<u32x2*>(out + ((int64_t)ch.seq * n_heads + h0 + h) * D + d) =
-          u32x2{pack_out<QT>(o[0] * f, o[1] * f), pack_out<QT>(o[2] * f, o[3] * f)};
-      if (lse && d == 0)
-        lse[(int64_t)ch.seq * n_heads + h0 + h] =
-            sum == 0.f ? -__builtin_inff() : (mu + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (row < 0) {
+      write_out<QT, D>(a.out, a.lse, (int64_t)seq * a.n_heads + h0 + h, d, o, mu, sum,
+                       pool.v_scale ? pool.v_scale[kvh] : 1.f);
     } else {
-      const int64_t at = (int64_t)blockIdx.x * tile_heads + h;
-      *reinterpret_cast<floatx4*>(part + at * D + d) = o;
+      *reinterpret_cast<floatx4*>(a.part + (row + h) * D + d) = o;
       if (d == 0) {
-        part_ml[2 * at] = top;
-        part_ml[2 * at + 1] = sum;
+        a.part_ml[2 * (row + h)] = top;
+        a.part_ml[2 * (row + h) + 1] = sum;
       }
     }
   }
 }
 
-// Joins the chunks of one query head of one sequence, in chunk order.
+// Workgroup (unit, sequence) takes the whole sequence.
+template <int QT, int KT, int D, bool ONCE>
+__global__ void __launch_bounds__(kDirectWaves * 64) paged_attention_direct_kernel(Rows a,
+                                                                                   PagePool pool) {
+  extern __shared__ float lds[];
+  const int units = pool.kv_heads * a.head_tiles;
+  const int seq = blockIdx.x / units;
+  attend_piece<QT, KT, D, kDirectWaves, ONCE>(a, pool, blockIdx.x % units, seq, 0,
+                                              clamp_len(uniform_load(a.lens, seq), a.cap), -1, lds);
+}
+
+// Workgroup (unit, piece) takes its piece of the row of blocks; the one past them all writes
+// down for each sequence which pieces it has (first piece, pieces, the first one's row).
+template <int QT, int KT, int D, bool ONCE>
+__global__ void __launch_bounds__(kSplitWaves * 64, 2) paged_attention_kernel(Rows a,
+                                                                              PagePool pool) {
+  extern __shared__ float lds[];
+  const int units = pool.kv_heads * a.head_tiles;
+  const int unit = blockIdx.x % units, piece = blockIdx.x / units;
+  const Scan scan(a.lens, a.seqs, a.cap);
+  const Cuts cuts(scan.total, a.pieces);
+  const int lane = threadIdx.x & 63;
+  if (piece == a.pieces) {
+    if (threadIdx.x >= 64) return;
+    int base = __builtin_amdgcn_update_dpp(0, scan.upto, 0x138, 0xf, 0xf, false);   // wave_shr:1
+    for (int i = 0; i < scan.per; ++i) {
+      const int64_t s = (int64_t)lane * scan.per + i;
+      if (s >= a.seqs) break;
+      const int n = blocks_of(clamp_len(a.lens[s], a.cap));
+      int4 p = make_int4(0, 0, 0, 0);
+      if (n > 0) {
+        p.x = cuts.piece_of(base);
+        p.y = cuts.piece_of(base + n - 1) - p.x + 1;
+        p.z = cuts.start(p.x) < base;
+      }
+      a.plan[s] = p;
+      base += n;
+    }
+    return;
+  }
+  int at = cuts.start(piece);
+  const int stop = cuts.start(piece + 1);
+  if (at == stop) return;
+  const int from = __builtin_ctzll(__ballot(at < scan.upto));
+  int base = from ? __builtin_amdgcn_readlane(scan.upto, from - 1) : 0;
+  int seq = from * scan.per;
+  int len = scan.per == 1 ? __builtin_amdgcn_readlane(scan.len, from) : clamp_len(uniform_load(a.lens, seq), a.cap);
+  while (true) {
+    const int n = blocks_of(len);
+    if (at < base + n) {
+      const int first = at - base, last = min(stop - base, n);
+      const int64_t row = first == 0 && last == n ? -1
+          : ((int64_t)blockIdx.x * 2 + (at > cuts.start(piece))) * a.tile_heads;
+      attend_piece<QT, KT, D, kSplitWaves, ONCE>(a, pool, unit, seq, first * kBlock,
+                                                 min(last * kBlock, len), row, lds);
+      at = base + last;
+      if (at == stop) return;
+      __syncthreads();                 // the next piece uses the same LDS
+    }
+    base += n;
+    if (++seq >= a.seqs) return;       // lengths that changed under the launch
+    len = clamp_len(uniform_load(a.lens, seq), a.cap);
+  }
+}
+
+// Joins the pieces of one query head of one sequence, in their order: each set of lanes takes
+// every SETS-th piece with a running maximum of its own, the sets are joined through LDS.
 template <int QT, int D>
-__global__ void __launch_bounds__(256) paged_attention_join_kernel(
-    const float* __restrict__ part, const float* __restrict__ part_ml,
-    const int2* __restrict__ plan, int kv_heads, int head_tiles, int tile_heads, int n_heads,
-    const float* __restrict__ v_scale, uint16_t* __restrict__ out, float* __restrict__ lse) {
+__global__ void __launch_bounds__(256) paged_attention_join_kernel(Rows a, int kv_heads,
+                                                                   const float* __restrict__ v_scale) {
   constexpr int LANES = D / 4, SETS = 256 / LANES;
   __shared__ floatx4 sums[SETS][LANES];
-  __shared__ float tops[4], totals[SETS];
+  __shared__ float tops[SETS], totals[SETS];
   const int64_t seq = blockIdx.y;
-  const int h = blockIdx.x, group = n_heads / kv_heads, kvh = h / group;
-  const int2 p = plan[seq];
+  const int h = blockIdx.x, group = a.n_heads / kv_heads, kvh = h / group;
+  const int4 p = a.plan[seq];
   if (p.y == 1) return;
-  const int units = kv_heads * head_tiles, unit = kvh * head_tiles + h % group / 16;
-  const int64_t first = ((int64_t)p.x * units + unit) * tile_heads + h % group % 16;
-  const int64_t step = (int64_t)units * tile_heads;        // from one chunk's row to the next's
-  float top = -__builtin_inff();
-  for (int i = threadIdx.x; i < p.y; i += 256) top = fmaxf(top, part_ml[2 * (first + i * step)]);
-  top = wave_max_valu(top);
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  const float mu = top == -__builtin_inff() ? 0.f : top;
+  const int units = kv_heads * a.head_tiles, unit = kvh * a.head_tiles + h % group / 16;
   const int set = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  float total = 0.f;
+  float top = -__builtin_inff(), total = 0.f;
 #pragma unroll 4
   for (int i = set; i < p.y; i += SETS) {
-    const int64_t at = first + i * step;
-    const float e = __builtin_amdgcn_exp2f(part_ml[2 * at] - mu);
-    total = fmaf(part_ml[2 * at + 1], e, total);
-    o += e * *reinterpret_cast<const floatx4*>(part + at * D + 4 * lane);
+    const int64_t at = (((int64_t)(p.x + i) * units + unit) * 2 + (i == 0 ? p.z : 0)) *
+                           a.tile_heads + h % group % 16;
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+    const floatx4 x = *reinterpret_cast<const floatx4*>(a.part + at * D + 4 * lane);
+    const float t = fmaxf(top, ml.x), mu = t == -__builtin_inff() ? 0.f : t;
+    const float e0 = __builtin_amdgcn_exp2f(top - mu), e1 = __builtin_amdgcn_exp2f(ml.x - mu);
+    total = total * e0 + ml.y * e1;
+    o = o * e0 + x * e1;
+    top = t;
   }
   sums[set][lane] = o;
-  if (lane == 0) totals[set] = total;
+  if (lane == 0) {
+    tops[set] = top;
+    totals[set] = total;
+  }
   __syncthreads();
   if (threadIdx.x >= LANES) return;
+  top = tops[0];
+#pragma unroll
+  for (int s = 1; s < SETS; ++s) top = fmaxf(top, tops[s]);
+  const float mu = top == -__builtin_inff() ? 0.f : top;
   total = 0.f;
   o = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int s = 0; s < SETS; ++s) {
-    total += totals[s];
-    o += sums[s][lane];
+    const float e = __builtin_amdgcn_exp2f(tops[s] - mu);
+    total = fmaf(totals[s], e, total);
+    o += e * sums[s][lane];
   }
-  const float f = total == 0.f ? 0.f : (v_scale ? v_scale[kvh] : 1.f) / total;
-  *reinterpret_cast<u32x2*>(out + (seq * n_heads + h) * D + 4 * lane) =
-      u32x2{pack_out<QT>(o[0] * f, o[1] * f), pack_out<QT>(o[2] * f, o[3] * f)};
-  if (lse && lane == 0)
-    lse[seq * n_heads + h] = total == 0.f ? -__builtin_inff()
-                                          : (mu + __builtin_amdgcn_logf(total)) * kLn2;
+  write_out<QT, D>(a.out, a.lse, seq * a.n_heads + h, 4 * lane, o, mu, total,
+                   v_scale ? v_scale[kvh] : 1.f);
 }
 
 }  // namespace mtl
@@ -501,11 +604,29 @@ extern "C" int64_t mtl_paged_attention_workspace_bytes(int64_t seqs, int32_t n_h
                                                        int32_t kv_heads, int32_t head_dim,
                                                        int64_t width, int32_t page_size) {
   if (seqs < 1 || kv_heads < 1 || n_heads < kv_heads || n_heads % kv_heads || head_dim < 1 ||
-      page_size < 1 || width < 0 || width * page_size <= kDirectPositions)
+      page_size < 1 || width < 0 || width <= kDirectPositions / page_size)
     return 0;
-  const Split s = split_of(seqs, n_heads, kv_heads);
-  return s.groups * s.tile_heads * (head_dim + 2) * 4 + 8 * seqs;
+  return split_of(n_heads, kv_heads).rows * (head_dim + 2) * 4 + 16 * seqs;
 }
+
+namespace mtl {
+
+template <int QT, int KT, int D, bool ONCE>
+static void launch_attention(const Rows& a, const PagePool& p, bool direct, const Split& s,
+                             hipStream_t stream) {
+  const size_t wave = (size_t)(s.tile_heads * (D + 4) + 32) * 4;
+  if (direct) {
+    paged_attention_direct_kernel<QT, KT, D, ONCE>
+        <<<(unsigned)(a.seqs * s.units), kDirectWaves * 64, kDirectWaves * wave, stream>>>(a, p);
+    return;
+  }
+  paged_attention_kernel<QT, KT, D, ONCE>
+      <<<(unsigned)(s.pieces * s.units + 1), kSplitWaves * 64, kSplitWaves * wave, stream>>>(a, p);
+  paged_attention_join_kernel<QT, D><<<dim3(a.n_heads, a.seqs), 256, 0, stream>>>(a, p.kv_heads,
+                                                                                  p.v_scale);
+}
+
+}  // namespace mtl
 
 extern "C" int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh,
                                    const mtl_page_pool* pool, const mtl_page_table* table,
@@ -515,58 +636,38 @@ extern "C" int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh,
   PagePool p;
   const int st = check_pool(pool, table, q_type, p);
   if (st != MTL_OK) return st;
-  if (n_heads < 1 || n_heads % pool->kv_heads) return MTL_ERR_SHAPE;
+  if (n_heads < 1 || n_heads % pool->kv_heads || n_heads > 65535) return MTL_ERR_SHAPE;
   if (table->seqs == 0) return MTL_OK;
   if (!q || !lens || !out) return MTL_ERR_INVALID_ARG;
   if (ldq % 8 || ldh % 8 || !aligned16(q) || !aligned16(out)) return MTL_ERR_ALIGN;
-  // rows of a page within 31 bits of a lane's offset; blocks of all sequences within 31 bits
+  // a lane's offset within a page, and the row of all sequences' blocks, within 31 bits
   const int64_t most = INT32_MAX / 64;
   if (p.k_token > most || p.v_token > most || table->seqs > 65535) return MTL_ERR_SHAPE;
-  int64_t cap = table->width > INT32_MAX / p.page_size ? INT32_MAX / p.page_size * p.page_size
-                                                       : table->width * p.page_size;
+  const int64_t wide = INT32_MAX / p.page_size;
+  const int64_t cap = (table->width < wide ? table->width : wide) * p.page_size;
   if (table->seqs * ((cap + kBlock - 1) / kBlock) > INT32_MAX) return MTL_ERR_SHAPE;
-  const Split s = split_of(table->seqs, n_heads, pool->kv_heads);
-  const int units = pool->kv_heads * s.head_tiles, d = pool->head_dim;
+  const Split s = split_of(n_heads, pool->kv_heads);
+  const int d = pool->head_dim;
   const int64_t need = mtl_paged_attention_workspace_bytes(table->seqs, n_heads, pool->kv_heads, d,
                                                            table->width, p.page_size);
   const bool direct = need == 0;
-  const int64_t groups = direct ? table->seqs * units : s.groups;
-  if (groups > INT32_MAX) return MTL_ERR_SHAPE;
+  if (table->seqs * s.units > INT32_MAX) return MTL_ERR_SHAPE;
   if (!direct && (!workspace || ws_bytes < need)) return MTL_ERR_WORKSPACE;
   if (!direct && !aligned16(workspace)) return MTL_ERR_ALIGN;
-  float* part = static_cast<float*>(workspace);
-  float* part_ml = direct ? nullptr : part + s.groups * s.tile_heads * d;
-  int2* plan = direct ? nullptr
-                      : reinterpret_cast<int2*>(part_ml + s.groups * s.tile_heads * 2);
-  const int waves = direct ? kDirectWaves : kSplitWaves;
-  const size_t shared = (size_t)waves * (s.tile_heads * (d + 4) + 32) * 4;
-  hipStream_t hs = (hipStream_t)stream;
-#define MTL_RUN(T, KT, D)                                                                       \
-  do {                                                                                          \
-    if (direct)                                                                                 \
-      paged_attention_kernel<T, KT, D, kDirectWaves, true>                                      \
-          <<<(unsigned)groups, kDirectWaves * 64, shared, hs>>>(                                \
-              (const uint16_t*)q, ldq, ldh, p, table->table, table->ld, cap, table->seqs, lens, \
-              n_heads, s.head_tiles, s.tile_heads, scale, (uint16_t*)out, lse, part, part_ml,   \
-              plan);                                                                            \
-    else                                                                                        \
-      paged_attention_kernel<T, KT, D, kSplitWaves, false>                                      \
-          <<<(unsigned)groups, kSplitWaves * 64, shared, hs>>>(                                 \
-              (const uint16_t*)q, ldq, ldh, p, table->table, table->ld, cap, table->seqs, lens, \
-              n_heads, s.head_tiles, s.tile_heads, scale, (uint16_t*)out, lse, part, part_ml,   \
-              plan);                                                                            \
+  char* ws = static_cast<char*>(workspace);
+  const Rows a{static_cast<const uint16_t*>(q), ldq, ldh, table->table, table->ld, cap, lens,
+               (int)table->seqs, n_heads, s.head_tiles, s.tile_heads, s.pieces, scale,
+               static_cast<uint16_t*>(out), lse, reinterpret_cast<float*>(ws + 16 * table->seqs),
+               reinterpret_cast<float*>(ws + 16 * table->seqs + s.rows * d * 4),
+               reinterpret_cast<int4*>(ws)};
+#define MTL_RUN(T, KT, D)                                                        \
+  do {                                                                           \
+    if (s.head_tiles == 1)                                                       \
+      launch_attention<T, KT, D, true>(a, p, direct, s, (hipStream_t)stream);    \
+    else                                                                         \
+      launch_attention<T, KT, D, false>(a, p, direct, s, (hipStream_t)stream);   \
   } while (0)
   MTL_PAGED_CASES(MTL_RUN, q_type, pool->type, d);
 #undef MTL_RUN
-  if (!direct) {
-    const dim3 grid(n_heads, (unsigned)table->seqs);
-#define MTL_JOIN(T, D)                                                                       \
-  paged_attention_join_kernel<T, D><<<grid, 256, 0, hs>>>(part, part_ml, plan, p.kv_heads,   \
-                                                          s.head_tiles, s.tile_heads, n_heads, \
-                                                          p.v_scale, (uint16_t*)out, lse)
-    if (q_type == MTL_T_BF16) { if (d == 128) MTL_JOIN(MTL_T_BF16, 128); else MTL_JOIN(MTL_T_BF16, 64); }
-    else { if (d == 128) MTL_JOIN(MTL_T_F16, 128); else MTL_JOIN(MTL_T_F16, 64); }
-#undef MTL_JOIN
-  }
   return launch_status();
 }
