@@ -29,8 +29,8 @@ extern "C" {
 #define MTL_T_F16 1
 #define MTL_T_E4M3 2
 
-/* One layer's pages.  Strides in elements; the head_dim elements of a row are adjacent;
- * bases and strides are multiples of 16 bytes. */
+/* One layer's pages.  Strides in elements; the head_dim elements of a row are adjacent, and
+ * k_token, v_token >= head_dim; bases and strides are multiples of 16 bytes. */
 typedef struct mtl_page_pool {
   void* k;
   void* v;
@@ -59,7 +59,8 @@ typedef struct mtl_page_table {
  * step, moss_tts_lite/fast.py:149-162, over pages): for sequence b and query head h, with
  * kv head h / (n_heads / kv_heads),
  *   s_j = scale * k_scale * (q . k_j),  j in [0, lens[b]);  out = v_scale * sum softmax(s)_j v_j
- * fp32 softmax and sums.  Lengths past width * page_size count as that, negative ones as 0.
+ * fp32 softmax and sums.  Lengths past width * page_size (at most 2^30) count as that, negative
+ * ones as 0.
  *   q    [seqs, n_heads, head_dim] of q_type (bf16 or f16), rows ldq and heads ldh elements
  *        apart (multiples of 8, base 16-byte aligned)
  *   out  [seqs, n_heads, head_dim] of q_type, contiguous, 16-byte aligned; a sequence without
@@ -88,6 +89,7 @@ int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh, const mtl_page_
  *   q_norm, k_norm  [head_dim] of type; both NULL: no norm
  *   cos_tab, sin_tab  [rope_rows, head_dim], fp32 (rope_f32 = 1) or of type; both NULL: no RoPE
  *   q_out      [rows, n_heads, head_dim] of type, contiguous
+ * q_out, norms and tables are 16-byte aligned.
  * The arithmetic is fp32 throughout with one rounding where q, k and v are stored (the dense
  * entries round after every step as the reference does).  E4M3 pages store x / scale,
  * limited to +-448, rounded to nearest even.  Rows whose page is a hole, whose position lies

@@ -38,19 +38,22 @@ constexpr int kBlock = kTile * kSplitWaves;
 constexpr int kWorkgroups = 512;        // 2 of 4 waves on each of 256 CUs
 constexpr int kDirectPositions = 512;
 constexpr int kDirectWaves = 8;
+constexpr int64_t kMaxPositions = 1 << 30;      // of one sequence: they fit an int with room
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // How the launch is shared: `pieces` workgroups for each unit (up to 16 query heads of a kv
 // head).  The workspace holds two rows of sums a workgroup, its first piece's and its last's
 // (fp32 [pieces * units][2][tile_heads][head_dim], then (maximum, sum) for each), and int4
-// [seqs] with what the second launch needs.
+// [min(seqs, pieces)] with what the second launch joins.
 struct Split {
   int units, head_tiles, tile_heads, pieces;
   int64_t rows;
+  // sequences that lie in several pieces, at most
+  int64_t joined(int64_t seqs) const { return seqs < pieces ? seqs : pieces; }
 };
 
-__host__ __device__ inline Split split_of(int n_heads, int kv_heads) {
+inline Split split_of(int n_heads, int kv_heads) {
   Split s;
   const int g = n_heads / kv_heads;
   s.tile_heads = g < 16 ? g : 16;
@@ -61,20 +64,43 @@ __host__ __device__ inline Split split_of(int n_heads, int kv_heads) {
   return s;
 }
 
+// A lane's 16, 8 or 4 bytes of 16 rows that begin at a base, through a buffer descriptor: the
+// descriptor's length lets rows that are not there be read as 0, whatever lies behind them, so
+// every load of a tile can be issued without a condition (under a condition the compiler waits
+// for all loads in flight where its paths join).
 // K and V are read once: loads that leave no trace in the caches read 7.1 TB/s here, others 6.4.
 // With more than 16 query heads to a kv head its rows are read again, from the caches.
-template <bool ONCE, class T>
-__device__ __forceinline__ T load(const char* p) {
-  const T* q = reinterpret_cast<const T*>(p);
-  return ONCE ? __builtin_nontemporal_load(q) : *q;
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+
+__device__ __forceinline__ Rsrc rows_at(const char* base, int bytes) {
+  // the same in all lanes, which the compiler does not see everywhere
+  const uint64_t b = reinterpret_cast<uintptr_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0,
+      __builtin_amdgcn_readfirstlane(bytes), 0x00027000);
 }
 
-// A lane's 32-bit offset, formed where it is used: the load then takes base and offset as they
-// are.  Without this the compiler keeps every offset as a 64-bit pair (24 registers).
-__device__ __forceinline__ uint32_t fresh(int offset) {
-  uint32_t o = (uint32_t)offset;
-  asm volatile("" : "+v"(o));
-  return o;
+template <bool ONCE>
+__device__ __forceinline__ void load_row(Rsrc rows, int offset, uint32_t (&x)[4]) {
+  const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, ONCE ? 2 : 0);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+template <bool ONCE>
+__device__ __forceinline__ void load_row(Rsrc rows, int offset, uint32_t (&x)[2]) {
+  const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, ONCE ? 2 : 0);
+  x[0] = v.x; x[1] = v.y;
+}
+template <bool ONCE>
+__device__ __forceinline__ void load_row(Rsrc rows, int offset, uint32_t (&x)[1]) {
+  x[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, offset, 0, ONCE ? 2 : 0);
+}
+
+// x as a value that the compiler forms anew from here on, and does not keep over a loop before.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // table[i] for an i that is the same in all lanes, as a scalar load: a vector load would have
@@ -133,66 +159,65 @@ struct Attend {
   static constexpr int VD = D / 16;                     // dims of a lane's V pieces
   static constexpr int VW = VD * E / 4;                 // ... in dwords
   u32x4 qf[QS];
-  u32x4 kf[2][KL];
+  uint32_t kf[2][KL][4];
   uint32_t vf[8][VW];
   floatx4 acc[VD];
   float m, l, c;                                        // c: scale to base 2
   int r, g, k_lane, v_lane, v_row;
 
-  // The pages of the tile's two halves of 16 positions; -1: none.
+  // A tile's two halves of 16 positions: each one's page and how many of its rows count (0: none).
   struct Tile {
-    int page[2];
+    int page[2], rows[2];
+  };
+  Tile t;                                               // of the tile in kf and vf
+
+  // One kv head's ends of the pages.
+  struct Ends {
+    const char* k;
+    const char* v;
+    int shift;
   };
 
-  __device__ __forceinline__ Tile pages(const int32_t* __restrict__ row, int shift, int p0, int end,
-                                        int n_pages) const {
-    Tile t;
+  // The page ids of the tile at p0, where the table has them (`limit`).
+  __device__ __forceinline__ void ids(const int32_t* __restrict__ row, int shift, int p0, int limit,
+                                      Tile& t) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int p = p0 + 16 * h;
-      int id = -1;
-      if (p < end) id = uniform_load(row, p >> shift);
-      t.page[h] = (uint32_t)id < (uint32_t)n_pages ? id : -1;
-    }
-    return t;
-  }
-
-  // A half without a page reads page 0 (any rows do: they are masked).  All 16 rows of a half
-  // lie in its page, those past the sequence's end too.
-  __device__ __forceinline__ void load_k(const PagePool& pool, const char* base, const Tile& t,
-                                         int p0) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int id = t.page[h] < 0 ? 0 : t.page[h];
-      const char* p = base + (id * pool.k_page + ((p0 + 16 * h) & (pool.page_size - 1)) *
-                                                     pool.k_token) * E;
-      const uint32_t o = fresh(k_lane);
-#pragma unroll
-      for (int s = 0; s < KL; ++s) kf[h][s] = load<ONCE, u32x4>(p + o + 64 * s);
+      t.page[h] = p < limit ? uniform_load(row, p >> shift) : -1;
     }
   }
 
-  __device__ __forceinline__ void load_v(const PagePool& pool, const char* base, const Tile& t,
+  __device__ __forceinline__ void count(int p0, int end, int n_pages, Tile& t) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool there = (uint32_t)t.page[h] < (uint32_t)n_pages;
+      t.rows[h] = there ? min(max(end - (p0 + 16 * h), 0), 16) : 0;
+      t.page[h] = there ? t.page[h] : 0;
+    }
+  }
+
+  __device__ __forceinline__ void load_k(const PagePool& pool, const Ends& e, const Tile& t,
                                          int p0) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int id = t.page[h] < 0 ? 0 : t.page[h];
-      const char* p = base + (id * pool.v_page + ((p0 + 16 * h) & (pool.page_size - 1)) *
-                                                     pool.v_token) * E;
+      const Rsrc rows = rows_at(e.k + (t.page[h] * pool.k_page +
+                                       ((p0 + 16 * h) & (pool.page_size - 1)) * pool.k_token) * E,
+                                t.rows[h] * (int)pool.k_token * E);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const char* q = p + fresh(v_lane + j * v_row);
-        if (VW == 4) {
-          const u32x4 x = load<ONCE, u32x4>(q);
-          vf[4 * h + j][0] = x.x; vf[4 * h + j][1 % VW] = x.y;
-          vf[4 * h + j][2 % VW] = x.z; vf[4 * h + j][3 % VW] = x.w;
-        } else if (VW == 2) {
-          const u32x2 x = load<ONCE, u32x2>(q);
-          vf[4 * h + j][0] = x.x; vf[4 * h + j][1 % VW] = x.y;
-        } else {
-          vf[4 * h + j][0] = load<ONCE, uint32_t>(q);
-        }
-      }
+      for (int s = 0; s < KL; ++s) load_row<ONCE>(rows, k_lane + 64 * s, kf[h][s]);
+    }
+  }
+
+  __device__ __forceinline__ void load_v(const PagePool& pool, const Ends& e, const Tile& t,
+                                         int p0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Rsrc rows = rows_at(e.v + (t.page[h] * pool.v_page +
+                                       ((p0 + 16 * h) & (pool.page_size - 1)) * pool.v_token) * E,
+                                t.rows[h] * (int)pool.v_token * E);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load_row<ONCE>(rows, v_lane + j * v_row, vf[4 * h + j]);
     }
   }
 
@@ -202,20 +227,20 @@ struct Attend {
     for (int i = 0; i < KL; ++i) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const u32x4 x = kf[h][i];
+        const uint32_t(&x)[4] = kf[h][i];
         if (E == 2)
-          a[h] = mfma<QT>(x, qf[i], a[h]);
+          a[h] = mfma<QT>(u32x4{x[0], x[1], x[2], x[3]}, qf[i], a[h]);
         else
-          a[h] = mfma<QT>(u32x4{widen<QT, false>(x.x), widen<QT, true>(x.x),
-                                widen<QT, false>(x.y), widen<QT, true>(x.y)},
+          a[h] = mfma<QT>(u32x4{widen<QT, false>(x[0]), widen<QT, true>(x[0]),
+                                widen<QT, false>(x[1]), widen<QT, true>(x[1])},
                           qf[(2 * i) % QS], a[h]);
       }
       if (E == 1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const u32x4 x = kf[h][i];
-          a[h] = mfma<QT>(u32x4{widen<QT, false>(x.z), widen<QT, true>(x.z),
-                                widen<QT, false>(x.w), widen<QT, true>(x.w)},
+          const uint32_t(&x)[4] = kf[h][i];
+          a[h] = mfma<QT>(u32x4{widen<QT, false>(x[2]), widen<QT, true>(x[2]),
+                                widen<QT, false>(x[3]), widen<QT, true>(x[3])},
                           qf[(2 * i + 1) % QS], a[h]);
         }
       }
@@ -224,17 +249,11 @@ struct Attend {
     for (int j = 0; j < 8; ++j) s[j] = a[j >> 2][j & 3] * c;
   }
 
-  // Positions past the end and without a page: score -inf, value 0 (what is stored there may
-  // be anything).
-  __device__ __forceinline__ void mask(float (&s)[8], const Tile& t, int p0, int end) {
+  // Rows that do not count: score -inf (their K and V are 0).
+  __device__ __forceinline__ void mask(float (&s)[8]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int h = j >> 2;
-      const bool in = t.page[h] >= 0 && p0 + 16 * h + 4 * g + (j & 3) < end;
-      s[j] = in ? s[j] : -__builtin_inff();
-#pragma unroll
-      for (int w = 0; w < VW; ++w) vf[j][w] = in ? vf[j][w] : 0u;
-    }
+    for (int j = 0; j < 8; ++j)
+      s[j] = 4 * g + (j & 3) < t.rows[j >> 2] ? s[j] : -__builtin_inff();
   }
 
   // Running softmax; s becomes the weights.
@@ -290,50 +309,37 @@ struct Attend {
     }
   }
 
-  __device__ __forceinline__ void load_q(const uint16_t* __restrict__ q, int64_t ldh, int heads) {
+  __device__ __forceinline__ void load_q(const uint16_t* __restrict__ q, int64_t ldh, int heads,
+                                         u32x4 (&f)[QS]) const {
 #pragma unroll
     for (int s = 0; s < QS; ++s) {
       const int d = E == 2 ? 32 * s + 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-      qf[s] = r < heads ? *reinterpret_cast<const u32x4*>(q + r * ldh + d) : u32x4{0, 0, 0, 0};
+      f[s] = r < heads ? *reinterpret_cast<const u32x4*>(q + r * ldh + d) : u32x4{0, 0, 0, 0};
     }
   }
 
-  // Positions [begin, end) of one sequence, this wave's tiles of them.
-  __device__ __forceinline__ void run(const PagePool& pool, const int32_t* __restrict__ row,
-                                      int kvh, int begin, int end, int wave) {
-    const int shift = __builtin_ctz(pool.page_size);
-    const char* kb = static_cast<const char*>(pool.k) + kvh * pool.k_head * E;
-    const char* vb = static_cast<const char*>(pool.v) + kvh * pool.v_head * E;
-    k_lane = r * (int)pool.k_token * E + 16 * g;
-    v_row = (int)pool.v_token * E;
-    v_lane = 4 * g * v_row + r * VD * E;
-    int p0 = begin + wave * kTile;
-    if (p0 >= end) return;
-    Tile t = pages(row, shift, p0, end, pool.pages);
-    load_k(pool, kb, t, p0);
-    load_v(pool, vb, t, p0);
-    int p1 = p0 + WAVES * kTile;
-    Tile next = pages(row, shift, p1, end, pool.pages);
-    float s[8];
-    // The next tile's K is loaded once this one's scores are formed, its V once this one's values
-    // are summed.  The last tile stands apart: a load under a condition would have the compiler
-    // wait for all loads wherever it joins.
-    while (p1 < end) {
+  // This wave's tiles of positions [begin, end); the page ids of a tile are read while the one
+  // before is worked on, up to position `limit` >= end.
+  __device__ __forceinline__ void run(const PagePool& pool, const Ends& e,
+                                      const int32_t* __restrict__ row, int begin, int end,
+                                      int limit) {
+    constexpr int kStep = WAVES * kTile;
+    int p0 = begin + wave_id() * kTile;
+    Tile next;
+    ids(row, e.shift, p0, limit, next);
+    while (p0 < end) {
+      t = next;
+      count(p0, end, pool.pages, t);
+      load_k(pool, e, t, p0);
+      load_v(pool, e, t, p0);
+      ids(row, e.shift, p0 + kStep, limit, next);
+      float s[8];
       scores(s);
-      load_k(pool, kb, next, p1);
-      if (t.page[0] < 0 || t.page[1] < 0) mask(s, t, p0, end);
+      if (t.rows[0] + t.rows[1] < kTile) mask(s);
       weights(s);
       values(s);
-      load_v(pool, vb, next, p1);
-      t = next;
-      p0 = p1;
-      p1 += WAVES * kTile;
-      next = pages(row, shift, p1, end, pool.pages);
+      p0 += kStep;
     }
-    scores(s);
-    if (p0 + kTile > end || t.page[0] < 0 || t.page[1] < 0) mask(s, t, p0, end);
-    weights(s);
-    values(s);
   }
 };
 
@@ -353,6 +359,12 @@ struct Cuts {
 };
 
 __device__ __forceinline__ int blocks_of(int len) { return (len + kBlock - 1) / kBlock; }
+
+// The end of `blocks` blocks of a sequence of len positions.
+__device__ __forceinline__ int blocks_end(int blocks, int len) {
+  const int64_t end = (int64_t)blocks * kBlock;
+  return end < len ? (int)end : len;
+}
 
 // Inclusive sum over the lanes of a wave (all active).
 __device__ __forceinline__ int wave_scan(int v) {
@@ -410,89 +422,167 @@ struct Rows {
   int4* plan;
 };
 
-// Positions [begin, end) of a sequence for one unit; the waves' results are joined through LDS
-// into out (row < 0) or into a row of the workspace.
+// What a workgroup of one unit works with.
 template <int QT, int KT, int D, int WAVES, bool ONCE>
-__device__ __forceinline__ void attend_piece(const Rows& a, const PagePool& pool, int unit, int seq,
-                                             int begin, int end, int64_t row, float* lds) {
-  constexpr int LD = D + 4;
-  const int kvh = unit / a.head_tiles, group = a.n_heads / pool.kv_heads;
-  const int h0 = kvh * group + (unit % a.head_tiles) * 16;
-  const int heads = min(16, (kvh + 1) * group - h0);
-  const int wave = wave_id();
+struct Unit {
+  using Wave = Attend<QT, KT, D, WAVES, ONCE>;
+  static constexpr int LD = D + 4;
+  const Rows& a;
+  const PagePool& pool;
+  float* lds;
+  int kvh, h0, heads;
+  typename Wave::Ends ends;
+  Wave w;
 
-  Attend<QT, KT, D, WAVES, ONCE> w;
-  // what depends on the thread is formed anew for each piece, before and after the loop over
-  // its tiles: kept over the loop it costs 30 registers
-  int thread = (int)fresh(threadIdx.x);
-  w.r = thread & 15;
-  w.g = (thread & 63) >> 4;
-  w.m = -__builtin_inff();
-  w.l = 0.f;
-  w.c = a.scale * (pool.k_scale ? pool.k_scale[kvh] : 1.f) * kLog2e;
-#pragma unroll
-  for (int d = 0; d < w.VD; ++d) w.acc[d] = floatx4{0.f, 0.f, 0.f, 0.f};
-  w.load_q(a.q + seq * a.ldq + h0 * a.ldh, a.ldh, heads);
-  w.run(pool, a.table + seq * a.ldt, kvh, begin, end, wave);
-
-  float* ml = lds + WAVES * a.tile_heads * LD;
-  w.l = xor32_add(xor16_add(w.l));
-  thread = (int)fresh(threadIdx.x);
-  const int r = thread & 15, g = (thread & 63) >> 4;
-  if (r < heads) {
-    float* o = lds + (wave * a.tile_heads + r) * LD + w.VD * 4 * g;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int d = 0; d < w.VD; d += 4)
-        *reinterpret_cast<floatx4*>(o + i * w.VD + d) =
-            floatx4{w.acc[d][i], w.acc[d + 1][i], w.acc[d + 2][i], w.acc[d + 3][i]};
-    if (g == 0) {
-      ml[2 * (wave * 16 + r)] = w.m;
-      ml[2 * (wave * 16 + r) + 1] = w.l;
-    }
+  __device__ __forceinline__ Unit(const Rows& a, const PagePool& pool, int unit, float* lds)
+      : a(a), pool(pool), lds(lds) {
+    kvh = unit / a.head_tiles;
+    const int group = a.n_heads / pool.kv_heads;
+    h0 = kvh * group + (unit % a.head_tiles) * 16;
+    heads = min(16, (kvh + 1) * group - h0);
+    ends.shift = __builtin_ctz(pool.page_size);
+    ends.k = static_cast<const char*>(pool.k) + kvh * pool.k_head * w.E;
+    ends.v = static_cast<const char*>(pool.v) + kvh * pool.v_head * w.E;
+    w.c = a.scale * (pool.k_scale ? pool.k_scale[kvh] : 1.f) * kLog2e;
   }
-  __syncthreads();
-  for (int i = thread; i < heads * (D / 4); i += WAVES * 64) {
-    const int h = i / (D / 4), d = 4 * (i % (D / 4));
-    float top = -__builtin_inff();
+
+  // What depends on the lane is formed anew for each piece: kept from one to the next, with what
+  // the compiler derives from it, it costs 30 registers.
+  __device__ __forceinline__ void lane() {
+    const int thread = fresh(threadIdx.x);
+    w.r = thread & 15;
+    w.g = (thread & 63) >> 4;
+    w.k_lane = w.r * (int)pool.k_token * w.E + 16 * w.g;
+    w.v_row = (int)pool.v_token * w.E;
+    w.v_lane = 4 * w.g * w.v_row + w.r * w.VD * w.E;
+  }
+
+  __device__ __forceinline__ const int32_t* row(int seq) const { return a.table + seq * a.ldt; }
+
+  __device__ __forceinline__ void query(int seq, u32x4 (&f)[Wave::QS]) const {
+    w.load_q(a.q + seq * a.ldq + h0 * a.ldh, a.ldh, heads, f);
+  }
+
+  __device__ __forceinline__ void clear() {
+    w.m = -__builtin_inff();
+    w.l = 0.f;
 #pragma unroll
-    for (int x = 0; x < WAVES; ++x) top = fmaxf(top, ml[2 * (x * 16 + h)]);
-    const float mu = top == -__builtin_inff() ? 0.f : top;
-    float sum = 0.f;
-    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < w.VD; ++d) w.acc[d] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Joins the waves through LDS, into out (dst < 0) or into rows of the workspace from dst on.
+  __device__ __forceinline__ void join(int seq, int64_t dst) {
+    float* ml = lds + WAVES * a.tile_heads * LD;
+    const int thread = fresh(threadIdx.x), wave = wave_id();
+    const int r = thread & 15, g = (thread & 63) >> 4;
+    w.l = xor32_add(xor16_add(w.l));
+    if (r < heads) {
+      float* o = lds + (wave * a.tile_heads + r) * LD + w.VD * 4 * g;
 #pragma unroll
-    for (int x = 0; x < WAVES; ++x) {
-      const float e = __builtin_amdgcn_exp2f(ml[2 * (x * 16 + h)] - mu);
-      sum = fmaf(ml[2 * (x * 16 + h) + 1], e, sum);
-      o += e * *reinterpret_cast<const floatx4*>(lds + (x * a.tile_heads + h) * LD + d);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < w.VD; d += 4)
+          *reinterpret_cast<floatx4*>(o + i * w.VD + d) =
+              floatx4{w.acc[d][i], w.acc[d + 1][i], w.acc[d + 2][i], w.acc[d + 3][i]};
+      if (g == 0) {
+        ml[2 * (wave * 16 + r)] = w.m;
+        ml[2 * (wave * 16 + r) + 1] = w.l;
+      }
     }
-    if (row < 0) {
-      write_out<QT, D>(a.out, a.lse, (int64_t)seq * a.n_heads + h0 + h, d, o, mu, sum,
-                       pool.v_scale ? pool.v_scale[kvh] : 1.f);
-    } else {
-      *reinterpret_cast<floatx4*>(a.part + (row + h) * D + d) = o;
-      if (d == 0) {
-        a.part_ml[2 * (row + h)] = top;
-        a.part_ml[2 * (row + h) + 1] = sum;
+    __syncthreads();
+    for (int i = thread; i < heads * (D / 4); i += WAVES * 64) {
+      const int h = i / (D / 4), d = 4 * (i % (D / 4));
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int x = 0; x < WAVES; ++x) top = fmaxf(top, ml[2 * (x * 16 + h)]);
+      const float mu = top == -__builtin_inff() ? 0.f : top;
+      float sum = 0.f;
+      floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < WAVES; ++x) {
+        const float e = __builtin_amdgcn_exp2f(ml[2 * (x * 16 + h)] - mu);
+        sum = fmaf(ml[2 * (x * 16 + h) + 1], e, sum);
+        o += e * *reinterpret_cast<const floatx4*>(lds + (x * a.tile_heads + h) * LD + d);
+      }
+      if (dst < 0) {
+        write_out<QT, D>(a.out, a.lse, (int64_t)seq * a.n_heads + h0 + h, d, o, mu, sum,
+                         pool.v_scale ? pool.v_scale[kvh] : 1.f);
+      } else {
+        *reinterpret_cast<floatx4*>(a.part + (dst + h) * D + d) = o;
+        if (d == 0) {
+          a.part_ml[2 * (dst + h)] = top;
+          a.part_ml[2 * (dst + h) + 1] = sum;
+        }
       }
     }
   }
-}
+};
 
-// Workgroup (unit, sequence) takes the whole sequence.
+// Workgroup (unit, sequence) takes the whole sequence; page ids and length are read at once.
 template <int QT, int KT, int D, bool ONCE>
 __global__ void __launch_bounds__(kDirectWaves * 64) paged_attention_direct_kernel(Rows a,
                                                                                    PagePool pool) {
   extern __shared__ float lds[];
   const int units = pool.kv_heads * a.head_tiles;
   const int seq = blockIdx.x / units;
-  attend_piece<QT, KT, D, kDirectWaves, ONCE>(a, pool, blockIdx.x % units, seq, 0,
-                                              clamp_len(uniform_load(a.lens, seq), a.cap), -1, lds);
+  Unit<QT, KT, D, kDirectWaves, ONCE> u(a, pool, blockIdx.x % units, lds);
+  u.lane();
+  u.query(seq, u.w.qf);
+  u.clear();
+  u.w.run(pool, u.ends, u.row(seq), 0, clamp_len(uniform_load(a.lens, seq), a.cap), (int)a.cap);
+  u.join(seq, -1);
 }
 
-// Workgroup (unit, piece) takes its piece of the row of blocks; the one past them all writes
-// down for each sequence which pieces it has (first piece, pieces, the first one's row).
+// What the second launch joins: sequences with several pieces, (sequence, first piece, pieces,
+// the first piece's row), at most one for each cut; (., ., 0, .) behind them.
+__device__ __forceinline__ void write_plan(const Rows& a, const Scan& scan, const Cuts& cuts) {
+  const int lane = threadIdx.x & 63;
+  const int most = min(a.seqs, a.pieces);
+  const int before = __builtin_amdgcn_update_dpp(0, scan.upto, 0x138, 0xf, 0xf, false);  // lane - 1
+  for (int pass = 0, slot = 0, listed = 0; pass < 2; ++pass) {
+    int base = before, mine = 0;
+    for (int i = 0; i < scan.per; ++i) {
+      const int64_t s = (int64_t)lane * scan.per + i;
+      const int n = s < a.seqs ? blocks_of(clamp_len(a.lens[s], a.cap)) : 0;
+      if (n > 1) {
+        const int p = cuts.piece_of(base), count = cuts.piece_of(base + n - 1) - p + 1;
+        if (count > 1) {
+          if (pass == 1) a.plan[slot + mine] = make_int4((int)s, p, count, cuts.start(p) < base);
+          ++mine;
+        }
+      }
+      base += n;
+    }
+    if (pass == 0) {
+      const int upto = wave_scan(mine);
+      slot = upto - mine;
+      listed = __builtin_amdgcn_readlane(upto, 63);
+    } else {
+      for (int k = listed + lane; k < most; k += 64) a.plan[k] = make_int4(0, 0, 0, 0);
+    }
+  }
+}
+
+// Sequences without positions: 0 and -inf, shared among the workgroup's waves.
+template <int D>
+__device__ __forceinline__ void write_empty(const Rows& a, const Scan& scan, int h0, int heads) {
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  for (int i = 0; i < scan.per; ++i) {
+    const int64_t s = (int64_t)lane * scan.per + i;
+    uint64_t empty = __ballot(s < a.seqs && clamp_len(s < a.seqs ? a.lens[s] : 1, a.cap) == 0);
+    for (int k = 0; empty; ++k, empty &= empty - 1) {
+      if (k % kSplitWaves != wave) continue;
+      const int64_t head = ((int64_t)__builtin_ctzll(empty) * scan.per + i) * a.n_heads + h0;
+      for (int j = lane; j < heads * (D / 8); j += 64)
+        *reinterpret_cast<u32x4*>(a.out + head * D + 8 * j) = u32x4{0, 0, 0, 0};
+      if (a.lse && lane < heads) a.lse[head + lane] = -__builtin_inff();
+    }
+  }
+}
+
+// Workgroup (unit, piece) takes its piece of the row of blocks, sequence after sequence; what it
+// reads first of the next one is on its way before it joins its waves' results of this one.  The
+// workgroups past the pieces write down what needs joining, and the empty sequences' outputs.
 template <int QT, int KT, int D, bool ONCE>
 __global__ void __launch_bounds__(kSplitWaves * 64, 2) paged_attention_kernel(Rows a,
                                                                               PagePool pool) {
@@ -501,43 +591,32 @@ __global__ void __launch_bounds__(kSplitWaves * 64, 2) paged_attention_kernel(Ro
   const int unit = blockIdx.x % units, piece = blockIdx.x / units;
   const Scan scan(a.lens, a.seqs, a.cap);
   const Cuts cuts(scan.total, a.pieces);
-  const int lane = threadIdx.x & 63;
+  Unit<QT, KT, D, kSplitWaves, ONCE> u(a, pool, unit, lds);
   if (piece == a.pieces) {
-    if (threadIdx.x >= 64) return;
-    int base = __builtin_amdgcn_update_dpp(0, scan.upto, 0x138, 0xf, 0xf, false);   // wave_shr:1
-    for (int i = 0; i < scan.per; ++i) {
-      const int64_t s = (int64_t)lane * scan.per + i;
-      if (s >= a.seqs) break;
-      const int n = blocks_of(clamp_len(a.lens[s], a.cap));
-      int4 p = make_int4(0, 0, 0, 0);
-      if (n > 0) {
-        p.x = cuts.piece_of(base);
-        p.y = cuts.piece_of(base + n - 1) - p.x + 1;
-        p.z = cuts.start(p.x) < base;
-      }
-      a.plan[s] = p;
-      base += n;
-    }
+    if (unit == 0 && a.pieces > 1 && wave_id() == 0) write_plan(a, scan, cuts);
+    write_empty<D>(a, scan, u.h0, u.heads);
     return;
   }
-  int at = cuts.start(piece);
-  const int stop = cuts.start(piece + 1);
-  if (at == stop) return;
-  const int from = __builtin_ctzll(__ballot(at < scan.upto));
+  const int start = cuts.start(piece), stop = cuts.start(piece + 1);
+  if (start == stop) return;
+  const int from = __builtin_ctzll(__ballot(start < scan.upto));
   int base = from ? __builtin_amdgcn_readlane(scan.upto, from - 1) : 0;
   int seq = from * scan.per;
-  int len = scan.per == 1 ? __builtin_amdgcn_readlane(scan.len, from) : clamp_len(uniform_load(a.lens, seq), a.cap);
+  int at = start, len = scan.per == 1 ? __builtin_amdgcn_readlane(scan.len, from)
+                          : clamp_len(uniform_load(a.lens, seq), a.cap);
   while (true) {
     const int n = blocks_of(len);
     if (at < base + n) {
-      const int first = at - base, last = min(stop - base, n);
-      const int64_t row = first == 0 && last == n ? -1
-          : ((int64_t)blockIdx.x * 2 + (at > cuts.start(piece))) * a.tile_heads;
-      attend_piece<QT, KT, D, kSplitWaves, ONCE>(a, pool, unit, seq, first * kBlock,
-                                                 min(last * kBlock, len), row, lds);
-      at = base + last;
+      const int first = at - base, end = blocks_end(stop - base, len);
+      u.lane();
+      u.query(seq, u.w.qf);
+      u.clear();
+      u.w.run(pool, u.ends, u.row(seq), first * kBlock, end, end);
+      u.join(seq, first == 0 && end == len
+                      ? -1 : ((int64_t)blockIdx.x * 2 + (at > start)) * a.tile_heads);
+      at = min(base + n, stop);
       if (at == stop) return;
-      __syncthreads();                 // the next piece uses the same LDS
+      __syncthreads();                 // the next sequence uses the same LDS
     }
     base += n;
     if (++seq >= a.seqs) return;       // lengths that changed under the launch
@@ -553,17 +632,16 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(Rows a, int k
   constexpr int LANES = D / 4, SETS = 256 / LANES;
   __shared__ floatx4 sums[SETS][LANES];
   __shared__ float tops[SETS], totals[SETS];
-  const int64_t seq = blockIdx.y;
   const int h = blockIdx.x, group = a.n_heads / kv_heads, kvh = h / group;
-  const int4 p = a.plan[seq];
-  if (p.y == 1) return;
+  const int4 p = a.plan[blockIdx.y];
+  if (p.z == 0) return;
   const int units = kv_heads * a.head_tiles, unit = kvh * a.head_tiles + h % group / 16;
   const int set = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
   float top = -__builtin_inff(), total = 0.f;
 #pragma unroll 4
-  for (int i = set; i < p.y; i += SETS) {
-    const int64_t at = (((int64_t)(p.x + i) * units + unit) * 2 + (i == 0 ? p.z : 0)) *
+  for (int i = set; i < p.z; i += SETS) {
+    const int64_t at = (((int64_t)(p.y + i) * units + unit) * 2 + (i == 0 ? p.w : 0)) *
                            a.tile_heads + h % group % 16;
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
     const floatx4 x = *reinterpret_cast<const floatx4*>(a.part + at * D + 4 * lane);
@@ -592,7 +670,7 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(Rows a, int k
     total = fmaf(totals[s], e, total);
     o += e * sums[s][lane];
   }
-  write_out<QT, D>(a.out, a.lse, seq * a.n_heads + h, 4 * lane, o, mu, total,
+  write_out<QT, D>(a.out, a.lse, (int64_t)p.x * a.n_heads + h, 4 * lane, o, mu, total,
                    v_scale ? v_scale[kvh] : 1.f);
 }
 
@@ -606,7 +684,8 @@ extern "C" int64_t mtl_paged_attention_workspace_bytes(int64_t seqs, int32_t n_h
   if (seqs < 1 || kv_heads < 1 || n_heads < kv_heads || n_heads % kv_heads || head_dim < 1 ||
       page_size < 1 || width < 0 || width <= kDirectPositions / page_size)
     return 0;
-  return split_of(n_heads, kv_heads).rows * (head_dim + 2) * 4 + 16 * seqs;
+  const Split s = split_of(n_heads, kv_heads);
+  return s.rows * (head_dim + 2) * 4 + 16 * s.joined(seqs);
 }
 
 namespace mtl {
@@ -621,9 +700,10 @@ static void launch_attention(const Rows& a, const PagePool& p, bool direct, cons
     return;
   }
   paged_attention_kernel<QT, KT, D, ONCE>
-      <<<(unsigned)(s.pieces * s.units + 1), kSplitWaves * 64, kSplitWaves * wave, stream>>>(a, p);
-  paged_attention_join_kernel<QT, D><<<dim3(a.n_heads, a.seqs), 256, 0, stream>>>(a, p.kv_heads,
-                                                                                  p.v_scale);
+      <<<(unsigned)((s.pieces + 1) * s.units), kSplitWaves * 64, kSplitWaves * wave, stream>>>(a, p);
+  if (s.pieces == 1) return;           // no sequence is cut
+  paged_attention_join_kernel<QT, D>
+      <<<dim3(a.n_heads, (unsigned)s.joined(a.seqs)), 256, 0, stream>>>(a, p.kv_heads, p.v_scale);
 }
 
 }  // namespace mtl
@@ -643,8 +723,8 @@ extern "C" int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh,
   // a lane's offset within a page, and the row of all sequences' blocks, within 31 bits
   const int64_t most = INT32_MAX / 64;
   if (p.k_token > most || p.v_token > most || table->seqs > 65535) return MTL_ERR_SHAPE;
-  const int64_t wide = INT32_MAX / p.page_size;
-  const int64_t cap = (table->width < wide ? table->width : wide) * p.page_size;
+  if (table->width > kMaxPositions / p.page_size) return MTL_ERR_SHAPE;
+  const int64_t cap = table->width * p.page_size;
   if (table->seqs * ((cap + kBlock - 1) / kBlock) > INT32_MAX) return MTL_ERR_SHAPE;
   const Split s = split_of(n_heads, pool->kv_heads);
   const int d = pool->head_dim;
@@ -655,10 +735,11 @@ extern "C" int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh,
   if (!direct && (!workspace || ws_bytes < need)) return MTL_ERR_WORKSPACE;
   if (!direct && !aligned16(workspace)) return MTL_ERR_ALIGN;
   char* ws = static_cast<char*>(workspace);
+  const int64_t lists = 16 * s.joined(table->seqs);
   const Rows a{static_cast<const uint16_t*>(q), ldq, ldh, table->table, table->ld, cap, lens,
                (int)table->seqs, n_heads, s.head_tiles, s.tile_heads, s.pieces, scale,
-               static_cast<uint16_t*>(out), lse, reinterpret_cast<float*>(ws + 16 * table->seqs),
-               reinterpret_cast<float*>(ws + 16 * table->seqs + s.rows * d * 4),
+               static_cast<uint16_t*>(out), lse, reinterpret_cast<float*>(ws + lists),
+               reinterpret_cast<float*>(ws + lists + s.rows * d * 4),
                reinterpret_cast<int4*>(ws)};
 #define MTL_RUN(T, KT, D)                                                        \
   do {                                                                           \

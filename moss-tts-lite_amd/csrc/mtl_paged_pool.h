@@ -17,17 +17,6 @@ struct PagePool {
   int pages, kv_heads, page_size;
 };
 
-template <int TYPE>
-__device__ __forceinline__ float load_elem(const void* p, int64_t i) {
-  if (TYPE == MTL_T_E4M3) {
-    const uint32_t b = static_cast<const uint8_t*>(p)[i];
-    const bf16x2_t v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
-    return (float)v.x;
-  }
-  const uint32_t b = static_cast<const uint16_t*>(p)[i];
-  return TYPE == MTL_T_BF16 ? bf16_to_f32(b) : f16_to_f32(b);
-}
-
 // float32 -> one stored element, to nearest even; e4m3 limited to +-448 (a NaN stays one).
 template <int TYPE>
 __device__ __forceinline__ uint32_t to_elem(float x) {
@@ -37,14 +26,6 @@ __device__ __forceinline__ uint32_t to_elem(float x) {
   }
   return TYPE == MTL_T_BF16 ? f32_to_bf16(x)
                             : (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)x);
-}
-
-template <int TYPE>
-__device__ __forceinline__ void store_elem(void* p, int64_t i, float x) {
-  if (TYPE == MTL_T_E4M3)
-    static_cast<uint8_t*>(p)[i] = (uint8_t)to_elem<TYPE>(x);
-  else
-    static_cast<uint16_t*>(p)[i] = (uint16_t)to_elem<TYPE>(x);
 }
 
 inline bool page_size_ok(int32_t ps) {
@@ -63,6 +44,8 @@ inline int check_pool(const mtl_page_pool* p, const mtl_page_table* t, int32_t t
   if ((p->head_dim != 64 && p->head_dim != 128) || !page_size_ok(p->page_size))
     return MTL_ERR_SHAPE;
   const int64_t piece = p->type == MTL_T_E4M3 ? 16 : 8;   // elements in 16 bytes
+  // rows of a head must not overlap: a token's stride holds a row
+  if (p->k_token < p->head_dim || p->v_token < p->head_dim) return MTL_ERR_SHAPE;
   const int64_t st[6] = {p->k_page, p->k_head, p->k_token, p->v_page, p->v_head, p->v_token};
   for (int64_t s : st)
     if (s < 0 || s % piece) return MTL_ERR_ALIGN;

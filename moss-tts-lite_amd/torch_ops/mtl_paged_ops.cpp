@@ -85,6 +85,7 @@ mtl_page_pool pool_of(const at::Tensor& k, const at::Tensor& v, const OptTensor&
                 " must have the rows' type or be float8_e4m3fn, got ", t.scalar_type());
     TORCH_CHECK(t.size(0) >= 1 && t.size(1) >= 1, name, " must hold at least one page and head");
     const int64_t piece = e4m3 ? 16 : 8;
+    TORCH_CHECK(t.stride(3) != 1 || t.stride(2) >= t.size(3), name, "'s rows must not overlap");
     TORCH_CHECK(t.stride(3) == 1 && step(t, 0) % piece == 0 && step(t, 1) % piece == 0 &&
                     t.stride(2) % piece == 0 && (t.is_meta() || aligned16(t.data_ptr())),
                 name, " must have unit last stride, other strides of multiples of 16 bytes and a "
