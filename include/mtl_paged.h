@@ -109,10 +109,13 @@ int mtl_paged_write(const void* qkv, int64_t ldq, int64_t rows, const mtl_page_p
  *   0  done
  *   1  not enough free pages (extend)
  *   2  a sequence outside [0, seqs), the same one twice, or a length out of range
- * n <= MTL_PAGES_MAX_CALL sequences a call, seqs <= MTL_PAGES_MAX_SEQS.
+ * n <= MTL_PAGES_MAX_CALL sequences a call, seqs <= MTL_PAGES_MAX_SEQS, width <=
+ * MTL_PAGES_MAX_WIDTH, page_size as in mtl_page_pool.  workspace: mtl_pages_workspace_bytes(n,
+ * pages) bytes (n = 0 for compaction), 16-byte aligned, any content, one launch at a time.
  */
 #define MTL_PAGES_MAX_CALL 1024
 #define MTL_PAGES_MAX_SEQS 32768
+#define MTL_PAGES_MAX_WIDTH (1 << 20)
 
 typedef struct mtl_page_state {
   int32_t* table;                     /* [seqs][ld], width entries used */
@@ -120,7 +123,7 @@ typedef struct mtl_page_state {
   int32_t* lens;                      /* [seqs]; not read by mtl_pages_compact */
   int32_t* refs;                      /* [pages] */
   int64_t pages;
-  int32_t page_size;                  /* a power of two */
+  int32_t page_size;
 } mtl_page_state;
 
 int64_t mtl_pages_workspace_bytes(int64_t n, int64_t pages);
@@ -128,12 +131,12 @@ int64_t mtl_pages_workspace_bytes(int64_t n, int64_t pages);
 /*
  * Room for counts[i] more tokens of sequence seqs[i], in call order: a partly filled last
  * page that others hold too is replaced by a copy, then each further page is taken; every
- * page taken is the lowest free one.  Adds counts to lens.  copy_src[i] / copy_dst[i]: the
- * page whose contents the caller has to copy for entry i (mtl_pages_copy), -1 where none.
+ * page taken is the lowest free one.  Adds counts to lens.  copies[0] pairs copy_src[i],
+ * copy_dst[i] (up to n) say which pages' contents the caller has to copy (mtl_pages_copy).
  */
 int mtl_pages_extend(const mtl_page_state* st, const int32_t* seqs, const int32_t* counts,
-                     int64_t n, int32_t* copy_src, int32_t* copy_dst, int32_t* status,
-                     void* workspace, int64_t ws_bytes, void* stream);
+                     int64_t n, int32_t* copy_src, int32_t* copy_dst, int32_t* copies,
+                     int32_t* status, void* workspace, int64_t ws_bytes, void* stream);
 
 /*
  * Sequence children[i] becomes parents[i]: the same pages (their counts rise) and length.

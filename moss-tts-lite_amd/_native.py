@@ -92,7 +92,7 @@ _SIGNATURES = {
                                ctypes.c_float, _i32, _i32, _c_void_p, _c_void_p]),
     "mtl_pages_workspace_bytes": (_i64, [_i64, _i64]),
     "mtl_pages_extend": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
-                                _c_void_p, _c_void_p, _i64, _c_void_p]),
+                                _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "mtl_pages_fork": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64,
                               _c_void_p]),
     "mtl_pages_truncate": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,

@@ -366,17 +366,6 @@ __device__ __forceinline__ int blocks_end(int blocks, int len) {
   return end < len ? (int)end : len;
 }
 
-// Inclusive sum over the lanes of a wave (all active).
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15, 31
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
-}
-
 // Every wave finds its place by itself: a lane counts the blocks of a run of `per` sequences.
 struct Scan {
   int per, len, upto, total;
@@ -580,8 +569,7 @@ __device__ __forceinline__ void write_empty(const Rows& a, const Scan& scan, int
   }
 }
 
-// Workgroup (unit, piece) takes its piece of the row of blocks, sequence after sequence; what it
-// reads first of the next one is on its way before it joins its waves' results of this one.  The
+// Workgroup (unit, piece) takes its piece of the row of blocks, sequence after sequence.  The
 // workgroups past the pieces write down what needs joining, and the empty sequences' outputs.
 template <int QT, int KT, int D, bool ONCE>
 __global__ void __launch_bounds__(kSplitWaves * 64, 2) paged_attention_kernel(Rows a,

@@ -28,6 +28,17 @@ __device__ __forceinline__ uint32_t to_elem(float x) {
                             : (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)x);
 }
 
+// Inclusive sum over the lanes of a wave (all active).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 inline bool page_size_ok(int32_t ps) {
   return ps == 16 || ps == 32 || ps == 64 || ps == 128 || ps == 256;
 }

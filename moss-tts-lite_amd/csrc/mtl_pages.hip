@@ -5,8 +5,7 @@
 // lowest free pages are global), then, where work grows with the sequences' lengths, a second
 // launch carries it out.  Every result is a function of the arguments alone: pages are taken in
 // ascending order by ranks from prefix sums, and the atomics only add integers.
-#include "mtl_common.h"
-#include "mtl_paged.h"
+#include "mtl_paged_pool.h"
 
 namespace mtl {
 
@@ -14,26 +13,24 @@ constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxCall = MTL_PAGES_MAX_CALL;
 constexpr int kMaxSeqs = MTL_PAGES_MAX_SEQS;
+constexpr int kStrip = 16 * kThreads;    // pages the workgroup looks at in one turn
+// Table entries up to which the deciding workgroup does the work itself: 16 a thread.  64 rows
+// of 32 pages forked: 3.4 us, 1.8 + 2.4 us in two launches.
+constexpr int64_t kOneLaunch = 16 * kThreads;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Exclusive prefix sum over the workgroup's threads; total receives the sum.  All threads.
-template <class I>
-__device__ __forceinline__ I block_scan(I v, I* waves, I& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  I x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const I y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+__device__ __forceinline__ int block_scan(int v, int* waves, int& total) {
+  const int wave = threadIdx.x >> 6;
+  const int x = wave_scan(v);
   __syncthreads();                       // the sums of an earlier call have been read
-  if (lane == 63) waves[wave] = x;
+  if ((threadIdx.x & 63) == 63) waves[wave] = x;
   __syncthreads();
-  I before = 0, sum = 0;
+  int before = 0, sum = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const I s = waves[w];
+    const int s = waves[w];
     before += w < wave ? s : 0;
     sum += s;
   }
@@ -47,21 +44,79 @@ __device__ __forceinline__ bool mark(uint32_t* bits, int s) {
   return atomicOr(&bits[s >> 5], b) & b;
 }
 
+__device__ __forceinline__ void clear_marks(uint32_t* bits, int64_t seqs) {
+  for (int i = threadIdx.x; i < (seqs + 31) / 32; i += kThreads) bits[i] = 0;
+}
+
 __device__ __forceinline__ int pages_of(int64_t len, int page_size) {
   return (int)((len + page_size - 1) / page_size);
 }
 
+// Which of pages p0 .. p0 + 15 are held (bit i: page p0 + i; pages past the pool count as held).
+__device__ __forceinline__ uint32_t held_mask(const int32_t* refs, int64_t p0, int64_t pages) {
+  uint32_t m = 0;
+  if (p0 + 16 <= pages && (reinterpret_cast<uintptr_t>(refs) & 15u) == 0) {
+    int4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const int4*>(refs + p0 + 4 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m |= ((v[i].x > 0) | (v[i].y > 0) << 1 | (v[i].z > 0) << 2 | (v[i].w > 0) << 3) << 4 * i;
+    return m;
+  }
+  for (int i = 0; i < 16; ++i)
+    if (p0 + i >= pages || refs[p0 + i] > 0) m |= 1u << i;
+  return m;
+}
+
+// What an entry of a call to fork or truncate moves: held pages from the first on.
+struct Span {
+  int row, from, first, held;            // row: the table row written; from: the one read
+};
+
+// Forks (FORK) or truncates: the spans' pages one a thread, four in turn so that their loads are
+// in flight together.
+template <bool FORK>
+__device__ __forceinline__ void move_pages(const mtl_page_state& st, const Span* spans, int n,
+                                           int widest) {
+  const int all = n * widest;              // at most kOneLaunch
+  for (int e0 = threadIdx.x; e0 < all; e0 += 4 * kThreads) {
+    int page[4], at[4], row[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = e0 + k * kThreads;
+      at[k] = -1;
+      if (e < all) {
+        const Span& s = spans[e / widest];
+        const int j = s.first + e % widest;
+        if (j < s.held) {
+          at[k] = j;
+          row[k] = s.row;
+          page[k] = st.table[s.from * st.ld + j];
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (at[k] < 0) continue;
+      st.table[row[k] * st.ld + at[k]] = FORK ? page[k] : -1;
+      if (page[k] >= 0 && page[k] < st.pages) atomicAdd(&st.refs[page[k]], FORK ? 1 : -1);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
     mtl_page_state st, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int n,
-    int32_t* __restrict__ copy_src, int32_t* __restrict__ copy_dst, int32_t* __restrict__ status,
-    int32_t* __restrict__ list) {
+    int32_t* __restrict__ copy_src, int32_t* __restrict__ copy_dst, int32_t* __restrict__ copies,
+    int32_t* __restrict__ status, int32_t* __restrict__ list) {
   __shared__ uint32_t seen[kMaxSeqs / 32];
   __shared__ int last[kMaxCall], off[kMaxCall], first[kMaxCall], seq[kMaxCall];
-  __shared__ int64_t waves64[kWaves];
   __shared__ int waves[kWaves];
   __shared__ int bad, shared_pages;
   const int t = threadIdx.x;
-  for (int i = t; i < kMaxSeqs / 32; i += kThreads) seen[i] = 0;
+  // the first strip of the search, needed whatever the call holds
+  const uint32_t strip0 = 16 * t < st.pages ? held_mask(st.refs, 16 * t, st.pages) : 0xffffu;
+  clear_marks(seen, st.seqs);
   if (t == 0) bad = shared_pages = 0;
   __syncthreads();
   const int64_t cap = st.width * st.page_size;
@@ -74,7 +129,7 @@ __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
     wrong = s < 0 || s >= st.seqs || c < 0;
     if (!wrong) {
       len = st.lens[s];
-      wrong = mark(seen, s) || len < 0 || len + c > cap || len + c > INT32_MAX;
+      wrong = mark(seen, s) || len < 0 || len + c > cap;
     }
     if (!wrong) {
       held = pages_of(len, st.page_size);
@@ -96,37 +151,43 @@ __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
     for (int i = 0; i < t; ++i) earlier += last[i] == page;
     copy = page_refs - earlier > 1;
   }
-  int64_t need = 0, total;
-  if (t < n && !wrong) need = pages_of(len + c, st.page_size) - held + (copy ? 1 : 0);
-  const int64_t at = block_scan<int64_t>(need, waves64, total);
-  int64_t found = 0;
-  if (!bad && total <= st.pages) {
-    for (int64_t p0 = 0; p0 < st.pages && found < total; p0 += kThreads) {
-      const int64_t p = p0 + t;
-      const int free_page = p < st.pages && st.refs[p] == 0;
+  int need = 0, total, all_copies;
+  if (t < n && !wrong) need = pages_of(len + c, st.page_size) - held + copy;
+  const int at = block_scan(need, waves, total);
+  const int place = block_scan(copy, waves, all_copies);
+  int found = 0;
+  if (!bad) {
+    for (int64_t p0 = 0; p0 < st.pages && found < total; p0 += kStrip) {
+      const int64_t p = p0 + 16 * t;
+      uint32_t free_pages = p0 == 0 ? strip0 : p < st.pages ? held_mask(st.refs, p, st.pages) : ~0u;
+      free_pages = ~free_pages & 0xffffu;
       int here;
-      const int64_t rank = found + block_scan<int>(free_page, waves, here);
-      if (free_page && rank < total) list[rank] = (int)p;
+      int rank = found + block_scan(__popc(free_pages), waves, here);
+      for (; free_pages && rank < total; free_pages &= free_pages - 1)
+        list[rank++] = (int)p + __ffs(free_pages) - 1;
       found += here;
     }
   }
   const bool ok = !bad && total <= found;
-  if (t == 0) status[0] = bad ? 2 : ok ? 0 : 1;
+  if (t == 0) {
+    status[0] = bad ? 2 : ok ? 0 : 1;
+    copies[0] = ok ? all_copies : 0;
+  }
   if (t < n) {
-    off[t] = (int)at;
+    off[t] = at;
     first[t] = copy ? (int)(len / st.page_size) : held;    // a copied page is the one before
     seq[t] = s;
   }
   __syncthreads();                                         // the list and the entries' places
+  if (!ok) return;
   if (t < n) {
-    copy_src[t] = ok && copy ? page : -1;
-    copy_dst[t] = ok && copy ? list[at] : -1;
-    if (ok) {
-      st.lens[s] = (int)(len + c);
-      if (copy) atomicSub(&st.refs[page], 1);
+    st.lens[s] = (int)(len + c);
+    if (copy) {
+      copy_src[place] = page;
+      copy_dst[place] = list[at];
+      atomicSub(&st.refs[page], 1);
     }
   }
-  if (!ok) return;
   for (int r = t; r < total; r += kThreads) {
     int lo = 0, hi = n - 1;                                // the last entry with off <= r
     while (lo < hi) {
@@ -139,108 +200,122 @@ __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
   }
 }
 
-__global__ void __launch_bounds__(kThreads) pages_fork_check_kernel(
-    mtl_page_state st, const int32_t* __restrict__ parents, const int32_t* __restrict__ children,
-    int n, int32_t* __restrict__ status, int32_t* __restrict__ held) {
+// Checks a call to fork or truncate and moves its pages, or leaves that to the next launch
+// (spans).  a, b: parents and children, or sequences and new lengths.
+template <bool FORK, bool ALL>
+__global__ void __launch_bounds__(kThreads) pages_move_kernel(
+    mtl_page_state st, const int32_t* __restrict__ a, const int32_t* __restrict__ b, int n,
+    int32_t* __restrict__ status, Span* __restrict__ spans_out) {
   __shared__ uint32_t seen[kMaxSeqs / 32];
-  __shared__ int bad;
+  __shared__ Span spans[kMaxCall];
+  __shared__ int bad, widest;
   const int t = threadIdx.x;
-  for (int i = t; i < kMaxSeqs / 32; i += kThreads) seen[i] = 0;
-  if (t == 0) bad = 0;
+  clear_marks(seen, st.seqs);
+  if (t == 0) bad = widest = 0;
   __syncthreads();
-  int p = 0, c = 0;
+  const int64_t cap = st.width * st.page_size;
+  int x = 0, y = 0;
   int64_t len = 0;
   bool wrong = false;
   if (t < n) {
-    p = parents[t];
-    c = children[t];
-    wrong = p < 0 || p >= st.seqs || c < 0 || c >= st.seqs;
+    x = a[t];
+    y = b[t];
+    wrong = x < 0 || x >= st.seqs || y < 0 || (FORK && y >= st.seqs);
     if (!wrong) {
-      len = st.lens[p];
-      wrong = mark(seen, c) || st.lens[c] != 0 || len < 0 || len > st.width * st.page_size;
+      len = st.lens[x];
+      wrong = mark(seen, FORK ? y : x) || len < 0 || len > cap ||
+              (FORK ? st.lens[y] != 0 : y > len);
     }
   }
-  __syncthreads();
-  if (t < n && !wrong) wrong = seen[p >> 5] >> (p & 31) & 1;
+  if (FORK) {                                              // no parent is a child
+    __syncthreads();
+    if (t < n && !wrong) wrong = seen[x >> 5] >> (x & 31) & 1;
+  }
   if (wrong) bad = 1;
   __syncthreads();
-  if (t == 0) status[0] = bad ? 2 : 0;
+  const bool ok = !bad;
+  if (t == 0) status[0] = ok ? 0 : 2;
   if (t < n) {
-    held[t] = bad ? 0 : pages_of(len, st.page_size);
-    if (!bad) st.lens[c] = (int)len;
-  }
-}
-
-__global__ void __launch_bounds__(256) pages_fork_kernel(
-    mtl_page_state st, const int32_t* __restrict__ parents, const int32_t* __restrict__ children,
-    const int32_t* __restrict__ held) {
-  const int i = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= held[i]) return;
-  const int p = st.table[parents[i] * st.ld + j];
-  st.table[children[i] * st.ld + j] = p;
-  if (p >= 0 && p < st.pages) atomicAdd(&st.refs[p], 1);
-}
-
-__global__ void __launch_bounds__(kThreads) pages_truncate_check_kernel(
-    mtl_page_state st, const int32_t* __restrict__ seqs, const int32_t* __restrict__ new_lens,
-    int n, int32_t* __restrict__ status, int32_t* __restrict__ held) {
-  __shared__ uint32_t seen[kMaxSeqs / 32];
-  __shared__ int bad;
-  const int t = threadIdx.x;
-  for (int i = t; i < kMaxSeqs / 32; i += kThreads) seen[i] = 0;
-  if (t == 0) bad = 0;
-  __syncthreads();
-  int s = 0, keep = 0;
-  int64_t len = 0;
-  bool wrong = false;
-  if (t < n) {
-    s = seqs[t];
-    keep = new_lens[t];
-    wrong = s < 0 || s >= st.seqs || keep < 0;
-    if (!wrong) {
-      len = st.lens[s];
-      wrong = mark(seen, s) || keep > len || len > st.width * st.page_size;
+    Span s{FORK ? y : x, x, FORK ? 0 : pages_of(y, st.page_size), 0};
+    if (ok) {
+      s.held = pages_of(len, st.page_size);
+      st.lens[s.row] = FORK ? (int)len : y;
     }
-    if (wrong) bad = 1;
+    if (ALL) {
+      spans[t] = s;
+      if (s.held > s.first) atomicMax(&widest, s.held - s.first);
+    } else {
+      spans_out[t] = s;
+    }
   }
-  __syncthreads();
-  if (t == 0) status[0] = bad ? 2 : 0;
-  if (t < n) {
-    held[t] = bad ? 0 : pages_of(len, st.page_size);
-    if (!bad) st.lens[s] = keep;
+  if (ALL) {
+    __syncthreads();
+    if (widest > 0) move_pages<FORK>(st, spans, n, widest);
   }
 }
 
-__global__ void __launch_bounds__(256) pages_truncate_kernel(
-    mtl_page_state st, const int32_t* __restrict__ seqs, const int32_t* __restrict__ new_lens,
-    const int32_t* __restrict__ held) {
-  const int i = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= held[i] || j < pages_of(new_lens[i], st.page_size)) return;
-  int32_t* e = st.table + seqs[i] * st.ld + j;
-  const int p = *e;
-  *e = -1;
-  if (p >= 0 && p < st.pages) atomicSub(&st.refs[p], 1);
+template <bool FORK>
+__global__ void __launch_bounds__(256) pages_move_wide_kernel(mtl_page_state st,
+                                                              const Span* __restrict__ spans) {
+  const Span s = spans[blockIdx.y];
+  const int j = s.first + blockIdx.x * 256 + threadIdx.x;
+  if (j >= s.held) return;
+  const int p = st.table[s.from * st.ld + j];
+  st.table[s.row * st.ld + j] = FORK ? p : -1;
+  if (p >= 0 && p < st.pages) atomicAdd(&st.refs[p], FORK ? 1 : -1);
 }
 
+__device__ __forceinline__ int moved(int p, int live, int64_t pages, const int32_t* goes) {
+  return p >= live && p < pages ? goes[p] : p;
+}
+
+// Plans the moves; with ALL it rewrites the table too.
+template <bool ALL>
 __global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(
     const int32_t* refs, int64_t pages, int32_t* refs_out, int32_t* __restrict__ live_out,
     int32_t* __restrict__ moves_out, int32_t* __restrict__ src, int32_t* __restrict__ dst,
-    int32_t* __restrict__ goes) {
+    int32_t* __restrict__ goes, const int32_t* table, int64_t ld, int64_t width, int64_t seqs,
+    int32_t* table_out, int64_t ld_out) {
   __shared__ int waves[kWaves];
   const int t = threadIdx.x;
+  const int all = (int)(seqs * width), w = (int)width;   // with ALL at most kOneLaunch
+  int page[4];                               // the table's first entries
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int e = t + k * kThreads;
+    page[k] = ALL && e < all ? table[e / w * ld + e % w] : 0;
+  }
   int held = 0, live;
-  for (int64_t p = t; p < pages; p += kThreads) held += refs[p] > 0;
-  block_scan<int>(held, waves, live);
+  uint32_t strip0 = 0;
+  for (int64_t p = 16 * t; p < pages; p += kStrip) {
+    const uint32_t in = pages - p < 16 ? (1u << (pages - p)) - 1 : 0xffffu;
+    const uint32_t used = held_mask(refs, p, pages) & in;
+    if (p < kStrip) strip0 = used;
+    held += __popc(used);
+  }
+  block_scan(held, waves, live);
   int movers = 0, holes = 0;
-  for (int64_t p0 = 0; p0 < pages; p0 += kThreads) {
-    const int64_t p = p0 + t;
-    const bool in = p < pages, used = in && refs[p] > 0;
-    const int mover = used && p >= live, hole = in && !used && p < live;
-    int sum;                                   // both counts stay below 2^16 in a strip
-    const int ranks = block_scan<int>(mover | hole << 16, waves, sum);
-    if (mover) src[movers + (ranks & 0xffff)] = (int)p;
-    if (hole) dst[holes + (ranks >> 16)] = (int)p;
-    if (in && p >= live && !mover) goes[p] = (int)p;
+  for (int64_t p0 = 0; p0 < pages; p0 += kStrip) {
+    const int64_t p = p0 + 16 * t;
+    uint32_t mover = 0, hole = 0, rest = 0;
+    if (p < pages) {
+      const uint32_t in = pages - p < 16 ? (1u << (pages - p)) - 1 : 0xffffu;
+      const uint32_t used = p0 == 0 ? strip0 : held_mask(refs, p, pages) & in;
+      const uint32_t low = live <= p ? 0u : live - p < 16 ? (1u << (live - p)) - 1 : 0xffffu;
+      mover = used & ~low;
+      hole = ~used & low & in;
+      rest = ~used & ~low & in;
+    }
+    int sum;                                   // at most 2^14 of each in a strip
+    const int ranks = block_scan(__popc(mover) | __popc(hole) << 16, waves, sum);
+    int k = movers + (ranks & 0xffff);
+    for (; mover; mover &= mover - 1) src[k++] = (int)p + __ffs(mover) - 1;
+    k = holes + (ranks >> 16);
+    for (; hole; hole &= hole - 1) dst[k++] = (int)p + __ffs(hole) - 1;
+    for (; rest; rest &= rest - 1) {
+      const int q = (int)p + __ffs(rest) - 1;
+      goes[q] = q;
+    }
     movers += sum & 0xffff;
     holes += sum >> 16;
   }
@@ -259,6 +334,21 @@ __global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(
     live_out[0] = live;
     moves_out[0] = movers;
   }
+  if (!ALL) return;
+  for (int e0 = t; e0 < all; e0 += 4 * kThreads) {
+#pragma unroll
+    for (int k = 0; k < 4 && e0 >= kThreads; ++k) {
+      const int e = e0 + k * kThreads;
+      page[k] = e < all ? table[e / w * ld + e % w] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) page[k] = moved(page[k], live, pages, goes);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = e0 + k * kThreads;
+      if (e < all) table_out[e / w * ld_out + e % w] = page[k];
+    }
+  }
 }
 
 __global__ void __launch_bounds__(256) pages_compact_table_kernel(
@@ -266,38 +356,75 @@ __global__ void __launch_bounds__(256) pages_compact_table_kernel(
     int64_t pages, const int32_t* __restrict__ live, const int32_t* __restrict__ goes) {
   const int64_t j = blockIdx.x * (int64_t)256 + threadIdx.x, s = blockIdx.y;
   if (j >= width) return;
-  const int p = table[s * ld + j];
-  table_out[s * ld_out + j] = p >= live[0] && p < pages ? goes[p] : p;
+  table_out[s * ld_out + j] = moved(table[s * ld + j], live[0], pages, goes);
 }
 
+// A workgroup takes pieces of kPiece bytes of (pair, layer, K or V), as many pairs as there are,
+// all of a pair's before the next one's.  Bound by memory.  Loads may stay in the caches (forks
+// of one sequence copy the same page), stores leave no trace there: 16 pages four times each in
+// 36 layers (302 MB) 32 us, with loads that leave none either 49, layer by layer 40.  A pool's
+// 2.1 GB take 427 us that way, 411 with both.
+constexpr int kPiece = 16384;
+constexpr int kCopyGroups = 4096;
+
 __global__ void __launch_bounds__(256) pages_copy_kernel(
-    char* __restrict__ k, char* __restrict__ v, int64_t k_layer, int64_t v_layer, int64_t k_page,
+    char* k, char* v, int64_t layers, int64_t k_layer, int64_t v_layer, int64_t k_page,
     int64_t v_page, int64_t page_bytes, int64_t pages, const int32_t* __restrict__ src,
-    const int32_t* __restrict__ dst, const int32_t* __restrict__ count) {
-  const int i = blockIdx.x;
-  if (count && i >= count[0]) return;
-  const int64_t a = src[i], b = dst[i], l = blockIdx.y;
-  if (a < 0 || a >= pages || b < 0 || b >= pages) return;
-  const char* from = blockIdx.z ? v + l * v_layer + a * v_page : k + l * k_layer + a * k_page;
-  char* to = blockIdx.z ? v + l * v_layer + b * v_page : k + l * k_layer + b * k_page;
-  for (int64_t o = 16 * threadIdx.x; o < page_bytes; o += 16 * 256)
-    *reinterpret_cast<u32x4*>(to + o) = *reinterpret_cast<const u32x4*>(from + o);
+    const int32_t* __restrict__ dst, int64_t n, const int32_t* __restrict__ count) {
+  const int64_t pairs = count && count[0] < n ? count[0] : n;
+  const int64_t pieces = (page_bytes + kPiece - 1) / kPiece;
+  const int64_t all = pairs * layers * 2 * pieces;
+  for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const int64_t piece = i % pieces, j = i / pieces % (2 * layers), l = j / 2,
+                  pair = i / pieces / (2 * layers);
+    const int64_t a = src[pair], b = dst[pair];
+    if (a < 0 || a >= pages || b < 0 || b >= pages) continue;
+    const char* from = j & 1 ? v + l * v_layer + a * v_page : k + l * k_layer + a * k_page;
+    char* to = j & 1 ? v + l * v_layer + b * v_page : k + l * k_layer + b * k_page;
+    const int64_t o = piece * kPiece + 16 * threadIdx.x;
+    u32x4 x[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      if (o + 4096 * m < page_bytes)
+        x[m] = *reinterpret_cast<const u32x4*>(from + o + 4096 * m);
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      if (o + 4096 * m < page_bytes)
+        __builtin_nontemporal_store(x[m], reinterpret_cast<u32x4*>(to + o + 4096 * m));
+  }
 }
 
 // Arguments every bookkeeping entry shares.
 static int check_state(const mtl_page_state* st, int64_t n, const void* status, const void* ws,
                        int64_t ws_bytes, bool lens = true) {
   if (!st || n < 0 || st->seqs < 0 || st->width < 0 || st->ld < st->width || st->pages < 0 ||
-      st->pages > INT32_MAX || !status)
+      st->pages > INT32_MAX - kStrip || !status)
     return MTL_ERR_INVALID_ARG;
-  if (n > kMaxCall || st->seqs > kMaxSeqs) return MTL_ERR_SHAPE;
-  if (st->page_size < 1 || (st->page_size & (st->page_size - 1))) return MTL_ERR_SHAPE;
-  if (st->width > INT32_MAX / st->page_size) return MTL_ERR_SHAPE;
+  if (n > kMaxCall || st->seqs > kMaxSeqs || st->width > MTL_PAGES_MAX_WIDTH)
+    return MTL_ERR_SHAPE;
+  if (!page_size_ok(st->page_size)) return MTL_ERR_SHAPE;
   if ((st->seqs > 0 && ((lens && !st->lens) || (st->width > 0 && !st->table))) ||
       (st->pages > 0 && !st->refs))
     return MTL_ERR_INVALID_ARG;
   if (!ws || ws_bytes < mtl_pages_workspace_bytes(n, st->pages)) return MTL_ERR_WORKSPACE;
-  return MTL_OK;
+  return aligned16(ws) ? MTL_OK : MTL_ERR_ALIGN;
+}
+
+template <bool FORK>
+static int move_call(const mtl_page_state* st, const int32_t* a, const int32_t* b, int64_t n,
+                     int32_t* status, void* workspace, int64_t ws_bytes, hipStream_t stream) {
+  const int e = check_state(st, n, status, workspace, ws_bytes);
+  if (e != MTL_OK) return e;
+  if (n > 0 && (!a || !b)) return MTL_ERR_INVALID_ARG;
+  Span* spans = static_cast<Span*>(workspace);
+  if (n * st->width <= kOneLaunch) {
+    pages_move_kernel<FORK, true><<<1, kThreads, 0, stream>>>(*st, a, b, (int)n, status, spans);
+  } else {
+    pages_move_kernel<FORK, false><<<1, kThreads, 0, stream>>>(*st, a, b, (int)n, status, spans);
+    const dim3 grid((unsigned)((st->width + 255) / 256), (unsigned)n);
+    pages_move_wide_kernel<FORK><<<grid, 256, 0, stream>>>(*st, spans);
+  }
+  return launch_status();
 }
 
 }  // namespace mtl
@@ -306,51 +433,34 @@ using namespace mtl;
 
 extern "C" int64_t mtl_pages_workspace_bytes(int64_t n, int64_t pages) {
   if (n < 0 || pages < 0) return 0;
-  return 4 * (n + pages + 16);
+  return 16 * (n + 1) + 4 * pages;
 }
 
 extern "C" int mtl_pages_extend(const mtl_page_state* st, const int32_t* seqs,
                                 const int32_t* counts, int64_t n, int32_t* copy_src,
-                                int32_t* copy_dst, int32_t* status, void* workspace,
-                                int64_t ws_bytes, void* stream) {
+                                int32_t* copy_dst, int32_t* copies, int32_t* status,
+                                void* workspace, int64_t ws_bytes, void* stream) {
   const int e = check_state(st, n, status, workspace, ws_bytes);
   if (e != MTL_OK) return e;
-  if (n > 0 && (!seqs || !counts || !copy_src || !copy_dst)) return MTL_ERR_INVALID_ARG;
+  if (!copies || (n > 0 && (!seqs || !counts || !copy_src || !copy_dst)))
+    return MTL_ERR_INVALID_ARG;
   pages_extend_kernel<<<1, kThreads, 0, (hipStream_t)stream>>>(
-      *st, seqs, counts, (int)n, copy_src, copy_dst, status, static_cast<int32_t*>(workspace));
+      *st, seqs, counts, (int)n, copy_src, copy_dst, copies, status,
+      static_cast<int32_t*>(workspace));
   return launch_status();
 }
 
 extern "C" int mtl_pages_fork(const mtl_page_state* st, const int32_t* parents,
                               const int32_t* children, int64_t n, int32_t* status,
                               void* workspace, int64_t ws_bytes, void* stream) {
-  const int e = check_state(st, n, status, workspace, ws_bytes);
-  if (e != MTL_OK) return e;
-  if (n > 0 && (!parents || !children)) return MTL_ERR_INVALID_ARG;
-  int32_t* held = static_cast<int32_t*>(workspace);
-  pages_fork_check_kernel<<<1, kThreads, 0, (hipStream_t)stream>>>(*st, parents, children, (int)n,
-                                                                   status, held);
-  if (n > 0 && st->width > 0) {
-    const dim3 grid((unsigned)((st->width + 255) / 256), (unsigned)n);
-    pages_fork_kernel<<<grid, 256, 0, (hipStream_t)stream>>>(*st, parents, children, held);
-  }
-  return launch_status();
+  return move_call<true>(st, parents, children, n, status, workspace, ws_bytes,
+                         (hipStream_t)stream);
 }
 
 extern "C" int mtl_pages_truncate(const mtl_page_state* st, const int32_t* seqs,
                                   const int32_t* new_lens, int64_t n, int32_t* status,
                                   void* workspace, int64_t ws_bytes, void* stream) {
-  const int e = check_state(st, n, status, workspace, ws_bytes);
-  if (e != MTL_OK) return e;
-  if (n > 0 && (!seqs || !new_lens)) return MTL_ERR_INVALID_ARG;
-  int32_t* held = static_cast<int32_t*>(workspace);
-  pages_truncate_check_kernel<<<1, kThreads, 0, (hipStream_t)stream>>>(*st, seqs, new_lens, (int)n,
-                                                                       status, held);
-  if (n > 0 && st->width > 0) {
-    const dim3 grid((unsigned)((st->width + 255) / 256), (unsigned)n);
-    pages_truncate_kernel<<<grid, 256, 0, (hipStream_t)stream>>>(*st, seqs, new_lens, held);
-  }
-  return launch_status();
+  return move_call<false>(st, seqs, new_lens, n, status, workspace, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int mtl_pages_compact(const mtl_page_state* st, int32_t* table_out, int64_t ld_out,
@@ -364,12 +474,18 @@ extern "C" int mtl_pages_compact(const mtl_page_state* st, int32_t* table_out, i
       (st->seqs > 0 && st->width > 0 && !table_out))
     return MTL_ERR_INVALID_ARG;
   int32_t* goes = static_cast<int32_t*>(workspace);
-  pages_compact_plan_kernel<<<1, kThreads, 0, (hipStream_t)stream>>>(
-      st->refs, st->pages, refs_out, live, moves, move_src, move_dst, goes);
-  if (st->seqs > 0 && st->width > 0) {
+  hipStream_t hs = (hipStream_t)stream;
+  if (st->seqs * st->width <= kOneLaunch) {
+    pages_compact_plan_kernel<true><<<1, kThreads, 0, hs>>>(
+        st->refs, st->pages, refs_out, live, moves, move_src, move_dst, goes, st->table, st->ld,
+        st->width, st->seqs, table_out, ld_out);
+  } else {
+    pages_compact_plan_kernel<false><<<1, kThreads, 0, hs>>>(
+        st->refs, st->pages, refs_out, live, moves, move_src, move_dst, goes, st->table, st->ld,
+        st->width, st->seqs, table_out, ld_out);
     const dim3 grid((unsigned)((st->width + 255) / 256), (unsigned)st->seqs);
-    pages_compact_table_kernel<<<grid, 256, 0, (hipStream_t)stream>>>(
-        st->table, st->ld, st->width, table_out, ld_out, st->pages, live, goes);
+    pages_compact_table_kernel<<<grid, 256, 0, hs>>>(st->table, st->ld, st->width, table_out,
+                                                     ld_out, st->pages, live, goes);
   }
   return launch_status();
 }
@@ -387,9 +503,10 @@ extern "C" int mtl_pages_copy(void* k, void* v, int64_t layers, int64_t k_layer,
       v_page % 16 || page_bytes % 16)
     return MTL_ERR_ALIGN;
   if (layers > 65535 || n > INT32_MAX) return MTL_ERR_SHAPE;
-  const dim3 grid((unsigned)n, (unsigned)layers, 2);
-  pages_copy_kernel<<<grid, 256, 0, (hipStream_t)stream>>>(
-      static_cast<char*>(k), static_cast<char*>(v), k_layer, v_layer, k_page, v_page, page_bytes,
-      pages, src, dst, count);
+  const int64_t most = n * layers * 2 * ((page_bytes + kPiece - 1) / kPiece);
+  pages_copy_kernel<<<(unsigned)(most < kCopyGroups ? most : kCopyGroups), 256, 0,
+                      (hipStream_t)stream>>>(
+      static_cast<char*>(k), static_cast<char*>(v), layers, k_layer, v_layer, k_page, v_page,
+      page_bytes, pages, src, dst, n, count);
   return launch_status();
 }

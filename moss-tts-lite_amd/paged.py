@@ -59,9 +59,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``out`` like q, and with ``return_lse`` also the fp32 ``[seqs, heads]`` logarithm of the
     softmax sums, with which the result joins that of other keys.  A sequence without positions
     gives 0 and -inf.  Lengths past the table's width count as that width."""
-    out, lse = ops.overload("paged_attention")(q, k_pages, v_pages, table, lens, scale, k_scale,
-                                               v_scale, return_lse)
-    return (out, lse) if return_lse else out
+    op = ops.overload("paged_attention_lse" if return_lse else "paged_attention")
+    return op(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale)
 
 
 def paged_write(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,

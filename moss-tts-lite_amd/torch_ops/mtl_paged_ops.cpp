@@ -1,5 +1,5 @@
 // torch dispatcher operators of the paged key-value cache over the C ABI in mtl_paged.h:
-// mtl::paged_attention, mtl::paged_write, mtl::pages_extend, mtl::pages_fork,
+// mtl::paged_attention(_lse), mtl::paged_write, mtl::pages_extend, mtl::pages_fork,
 // mtl::pages_truncate, mtl::pages_compact and mtl::pages_copy.
 //
 // Host code only, as mtl_torch_ops.cpp: each operator checks its tensors, takes outputs and
@@ -8,6 +8,7 @@
 // graphs captured from them share nothing.  Meta kernels make the same checks and give the
 // output shapes to tracing.
 #include <ATen/ATen.h>
+#include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -132,11 +133,20 @@ hipStream_t stream_of(const at::Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
-std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k_pages,
-                                                   const at::Tensor& v_pages,
-                                                   const at::Tensor& table, const at::Tensor& lens,
-                                                   double scale, const OptTensor& k_scale,
-                                                   const OptTensor& v_scale, bool return_lse) {
+// Memory of a call's own from torch's caching allocator, without a tensor around it.
+struct Workspace {
+  c10::DataPtr data;
+  int64_t bytes;
+  Workspace(const at::Tensor& like, int64_t n)
+      : data(n > 0 ? c10::GetAllocator(like.device().type())->allocate(n) : c10::DataPtr()),
+        bytes(n) {}
+  void* get() const { return data.get(); }
+};
+
+// out, and where lse is not null the log-sum-exp
+at::Tensor attend(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                  const at::Tensor& table, const at::Tensor& lens, double scale,
+                  const OptTensor& k_scale, const OptTensor& v_scale, at::Tensor* lse) {
   TORCH_CHECK(q.dim() == 3, "q must be [sequences, heads, head_dim], got ", q.sizes());
   const int32_t type = row_type(q, "q");
   const mtl_page_pool pool = pool_of(k_pages, v_pages, k_scale, v_scale, type);
@@ -151,8 +161,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at
   TORCH_CHECK(tab.seqs == b && lens.size(0) == b, "q, table and lens must have the same number of "
               "sequences, got ", b, ", ", tab.seqs, " and ", lens.size(0));
   at::Tensor out = at::empty({b, h, q.size(2)}, q.options());
-  at::Tensor lse = at::empty({return_lse ? b : 0, h}, q.options().dtype(at::kFloat));
-  if (q.is_meta() || b == 0) return {out, lse};
+  if (lse) *lse = at::empty({b, h}, q.options().dtype(at::kFloat));
+  if (q.is_meta() || b == 0) return out;
   const c10::DeviceGuard guard(q.device());
   // the kernel reads q in 16-byte pieces: any other view is copied
   at::Tensor q2 = q;
@@ -160,15 +170,30 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at
     q2 = q.contiguous();
     if (!aligned16(q2.data_ptr())) q2 = q2.clone();
   }
-  const int64_t ws = mtl_paged_attention_workspace_bytes(b, (int32_t)h, pool.kv_heads,
-                                                         pool.head_dim, tab.width, pool.page_size);
-  at::Tensor wsb;
-  if (ws > 0) wsb = at::empty({ws}, q.options().dtype(at::kByte));
+  const Workspace ws(q, mtl_paged_attention_workspace_bytes(
+                            b, (int32_t)h, pool.kv_heads, pool.head_dim, tab.width,
+                            pool.page_size));
   check_status(mtl_paged_attention(q2.data_ptr(), step(q2, 0), step(q2, 1), &pool, &tab,
                                    ptr<int32_t>(lens), (int32_t)h, type, (float)scale,
-                                   out.data_ptr(), return_lse ? ptr<float>(lse) : nullptr,
-                                   ws > 0 ? wsb.data_ptr() : nullptr, ws, stream_of(q)),
+                                   out.data_ptr(), lse ? ptr<float>(*lse) : nullptr, ws.get(),
+                                   ws.bytes, stream_of(q)),
                "mtl_paged_attention");
+  return out;
+}
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages,
+                           const at::Tensor& v_pages, const at::Tensor& table,
+                           const at::Tensor& lens, double scale, const OptTensor& k_scale,
+                           const OptTensor& v_scale) {
+  return attend(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale, nullptr);
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention_lse(
+    const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+    const at::Tensor& table, const at::Tensor& lens, double scale, const OptTensor& k_scale,
+    const OptTensor& v_scale) {
+  at::Tensor lse;
+  at::Tensor out = attend(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale, &lse);
   return {out, lse};
 }
 
@@ -286,10 +311,6 @@ int64_t check_call(const at::Tensor& a, const at::Tensor& b, const at::Tensor& t
   return a.size(0);
 }
 
-at::Tensor workspace_of(const at::Tensor& like, int64_t n, int64_t pages) {
-  return at::empty({mtl_pages_workspace_bytes(n, pages)}, like.options().dtype(at::kByte));
-}
-
 // How whole pages lie in a pool [layers,] pages, kv_heads, page_size, head_dim.
 struct PageBlocks {
   int64_t layers, layer_bytes, page_stride, page_bytes, pages;
@@ -349,15 +370,15 @@ at::Tensor pages_extend(at::Tensor& table, at::Tensor& lens, at::Tensor& refs,
   at::Tensor status = at::empty({1}, table.options());
   if (table.is_meta()) return status;
   const c10::DeviceGuard guard(table.device());
-  const at::Tensor pair = at::empty({2, std::max<int64_t>(n, 1)}, table.options());
-  const at::Tensor ws = workspace_of(table, n, st.pages);
-  int32_t* src = ptr<int32_t>(pair);
-  int32_t* dst = src + std::max<int64_t>(n, 1);
+  const int64_t bytes = (mtl_pages_workspace_bytes(n, st.pages) + 15) / 16 * 16;
+  const Workspace ws(table, bytes + 4 * (2 * n + 1));
+  int32_t* copies = reinterpret_cast<int32_t*>(static_cast<char*>(ws.get()) + bytes);
+  int32_t* src = copies + 1;
+  int32_t* dst = src + n;
   check_status(mtl_pages_extend(&st, ptr<int32_t>(seqs), ptr<int32_t>(counts), n, src, dst,
-                                ptr<int32_t>(status), ws.data_ptr(), ws.numel(),
-                                stream_of(table)),
+                                copies, ptr<int32_t>(status), ws.get(), bytes, stream_of(table)),
                "mtl_pages_extend");
-  copy_blocks(k_pages, v_pages, kb, vb, src, dst, n, nullptr);
+  copy_blocks(k_pages, v_pages, kb, vb, src, dst, n, copies);
   return status;
 }
 
@@ -368,9 +389,9 @@ at::Tensor pages_fork(at::Tensor& table, at::Tensor& lens, at::Tensor& refs,
   at::Tensor status = at::empty({1}, table.options());
   if (table.is_meta()) return status;
   const c10::DeviceGuard guard(table.device());
-  const at::Tensor ws = workspace_of(table, n, st.pages);
+  const Workspace ws(table, mtl_pages_workspace_bytes(n, st.pages));
   check_status(mtl_pages_fork(&st, ptr<int32_t>(parents), ptr<int32_t>(children), n,
-                              ptr<int32_t>(status), ws.data_ptr(), ws.numel(), stream_of(table)),
+                              ptr<int32_t>(status), ws.get(), ws.bytes, stream_of(table)),
                "mtl_pages_fork");
   return status;
 }
@@ -382,10 +403,9 @@ at::Tensor pages_truncate(at::Tensor& table, at::Tensor& lens, at::Tensor& refs,
   at::Tensor status = at::empty({1}, table.options());
   if (table.is_meta()) return status;
   const c10::DeviceGuard guard(table.device());
-  const at::Tensor ws = workspace_of(table, n, st.pages);
+  const Workspace ws(table, mtl_pages_workspace_bytes(n, st.pages));
   check_status(mtl_pages_truncate(&st, ptr<int32_t>(seqs), ptr<int32_t>(new_lens), n,
-                                  ptr<int32_t>(status), ws.data_ptr(), ws.numel(),
-                                  stream_of(table)),
+                                  ptr<int32_t>(status), ws.get(), ws.bytes, stream_of(table)),
                "mtl_pages_truncate");
   return status;
 }
@@ -405,13 +425,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> pages_compact(const at::Tensor& t
   if (table.is_meta()) return {new_table, new_refs, live};
   const c10::DeviceGuard guard(table.device());
   const int64_t half = st.pages / 2;
-  const at::Tensor lists = at::empty({2 * half + 1}, table.options());
-  const at::Tensor ws = workspace_of(table, 0, st.pages);
-  int32_t* src = ptr<int32_t>(lists);
-  int32_t* moves = src + 2 * half;
+  const int64_t bytes = (mtl_pages_workspace_bytes(0, st.pages) + 15) / 16 * 16;
+  const Workspace ws(table, bytes + 4 * (2 * half + 1));
+  int32_t* moves = reinterpret_cast<int32_t*>(static_cast<char*>(ws.get()) + bytes);
+  int32_t* src = moves + 1;
   check_status(mtl_pages_compact(&st, ptr<int32_t>(new_table), table.size(1),
                                  ptr<int32_t>(new_refs), ptr<int32_t>(live), moves, src,
-                                 src + half, ws.data_ptr(), ws.numel(), stream_of(table)),
+                                 src + half, ws.get(), bytes, stream_of(table)),
                "mtl_pages_compact");
   copy_blocks(k_pages, v_pages, kb, vb, src, src + half, half, moves);
   return {new_table, new_refs, live};
@@ -435,7 +455,9 @@ void pages_copy(at::Tensor& k_pages, at::Tensor& v_pages, const at::Tensor& src,
 
 TORCH_LIBRARY_FRAGMENT(mtl, m) {
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor lens, "
-        "float scale, Tensor? k_scale=None, Tensor? v_scale=None, bool return_lse=False) "
+        "float scale, Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor");
+  m.def("paged_attention_lse(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, "
+        "Tensor lens, float scale, Tensor? k_scale=None, Tensor? v_scale=None) "
         "-> (Tensor, Tensor)");
   m.def("paged_write(Tensor qkv, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, "
         "Tensor positions, Tensor? seqs=None, Tensor? q_norm=None, Tensor? k_norm=None, "
@@ -454,6 +476,7 @@ TORCH_LIBRARY_FRAGMENT(mtl, m) {
 
 #define MTL_PAGED_IMPLS(m)                   \
   m.impl("paged_attention", &paged_attention); \
+  m.impl("paged_attention_lse", &paged_attention_lse); \
   m.impl("paged_write", &paged_write);         \
   m.impl("pages_extend", &pages_extend);       \
   m.impl("pages_fork", &pages_fork);           \

@@ -84,6 +84,15 @@ def test_attention_many_sequences(dev):
     check_attention(attend_case(1500, 2, 1, 64, 16, "bf16", "bf16", lens, dev))
 
 
+@pytest.mark.parametrize("B", [65, 130, 700])
+def test_attention_many_sequences_split(dev, B):
+    # more sequences than a wave has lanes, shared among the workgroups: short, empty and long ones
+    rng = random.Random(B)
+    lens = [rng.choice((0, 1, 31, 33, rng.randint(1, 40), rng.randint(1, 700))) for _ in range(B)]
+    lens[B // 2] = 1100
+    check_attention(attend_case(B, 4, 2, 64, 16, "bf16", "bf16", lens, dev, B))
+
+
 def test_attention_peaked_scores(dev):
     # one position holds nearly all the weight, far below or above the others
     check_attention(attend_case(3, 8, 2, 128, 16, "bf16", "bf16", [400, 33, 1000], dev, 1,

@@ -107,12 +107,12 @@ def state(**kw):
     (dict(refs=None), 1, N.MTL_ERR_INVALID_ARG), (dict(ld=2), 1, N.MTL_ERR_INVALID_ARG),
     (dict(pages=-1), 1, N.MTL_ERR_INVALID_ARG), (dict(page_size=48), 1, N.MTL_ERR_SHAPE),
     (dict(page_size=0), 1, N.MTL_ERR_SHAPE), (dict(seqs=32769), 1, N.MTL_ERR_SHAPE),
-    (dict(width=1 << 28, ld=1 << 28), 1, N.MTL_ERR_SHAPE), (dict(), 1025, N.MTL_ERR_SHAPE),
+    (dict(width=(1 << 20) + 1, ld=1 << 21), 1, N.MTL_ERR_SHAPE), (dict(), 1025, N.MTL_ERR_SHAPE),
     (dict(), -1, N.MTL_ERR_INVALID_ARG)])
 def test_bookkeeping_refusals(lib, kw, n, expect):
     st = ctypes.byref(state(**kw))
     ws = (FAKE, 1 << 30, None)
-    assert lib.mtl_pages_extend(st, FAKE, FAKE, n, FAKE, FAKE, FAKE, *ws) == expect
+    assert lib.mtl_pages_extend(st, FAKE, FAKE, n, FAKE, FAKE, FAKE, FAKE, *ws) == expect
     assert lib.mtl_pages_fork(st, FAKE, FAKE, n, FAKE, *ws) == expect
     assert lib.mtl_pages_truncate(st, FAKE, FAKE, n, FAKE, *ws) == expect
 
@@ -120,12 +120,15 @@ def test_bookkeeping_refusals(lib, kw, n, expect):
 def test_bookkeeping_workspace_and_pointers(lib):
     st = ctypes.byref(state())
     need = lib.mtl_pages_workspace_bytes(2, 8)
-    assert lib.mtl_pages_extend(st, FAKE, FAKE, 2, FAKE, FAKE, FAKE, FAKE, need - 1,
+    assert lib.mtl_pages_extend(st, FAKE, FAKE, 2, FAKE, FAKE, FAKE, FAKE, FAKE, need - 1,
                                 None) == N.MTL_ERR_WORKSPACE
-    assert lib.mtl_pages_extend(st, FAKE, FAKE, 2, None, FAKE, FAKE, FAKE, need,
-                                None) == N.MTL_ERR_INVALID_ARG
-    assert lib.mtl_pages_extend(st, FAKE, FAKE, 2, FAKE, FAKE, None, FAKE, need,
-                                None) == N.MTL_ERR_INVALID_ARG
+    assert lib.mtl_pages_extend(st, FAKE, FAKE, 2, FAKE, FAKE, FAKE, FAKE, FAKE + 4, need,
+                                None) == N.MTL_ERR_ALIGN
+    for i in range(5):                    # counts, sources, destinations, their number, status
+        p = [FAKE] * 5
+        p[i] = None
+        assert lib.mtl_pages_extend(st, FAKE, p[0], 2, *p[1:], FAKE, need,
+                                    None) == N.MTL_ERR_INVALID_ARG
     assert lib.mtl_pages_fork(st, None, FAKE, 2, FAKE, FAKE, need, None) == N.MTL_ERR_INVALID_ARG
     assert lib.mtl_pages_compact(st, FAKE, 3, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, need,
                                  None) == N.MTL_ERR_INVALID_ARG
