@@ -69,7 +69,8 @@ typedef struct mtl_page_table {
  *        sequence without positions)
  *   workspace  mtl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, any content,
  *        one launch at a time
- * The pages have q_type's type or E4M3.  n_heads % kv_heads == 0.
+ * The pages have q_type's type or E4M3.  n_heads % kv_heads == 0, n_heads and seqs at most
+ * 65535.  The same call gives the same bits; the order of a sequence's sums goes by all lengths.
  */
 int64_t mtl_paged_attention_workspace_bytes(int64_t seqs, int32_t n_heads, int32_t kv_heads,
                                             int32_t head_dim, int64_t width, int32_t page_size);

@@ -8,6 +8,7 @@ Modules
 ``_native``  ctypes binding of ``libmtl_hip.so`` (C ABI in ``include/``)
 ``ops``      torch-facing int4 GEMM / pack / dequant ops
 ``gptq``     the GPTQ linear module and the reference's format helpers
+``paged``    paged key-value cache of several sequences: attention, writes, page bookkeeping
 ``build``    the hipcc recipe of ``libmtl_hip.so``
 """
 __version__ = "0.1.0"

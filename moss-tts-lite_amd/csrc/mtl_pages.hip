@@ -14,9 +14,12 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxCall = MTL_PAGES_MAX_CALL;
 constexpr int kMaxSeqs = MTL_PAGES_MAX_SEQS;
 constexpr int kStrip = 16 * kThreads;    // pages the workgroup looks at in one turn
-// Table entries up to which the deciding workgroup does the work itself: 16 a thread.  64 rows
-// of 32 pages forked: 3.4 us, 1.8 + 2.4 us in two launches.
-constexpr int64_t kOneLaunch = 16 * kThreads;
+// Table entries up to which the deciding workgroup does the work itself, and a second launch
+// costs more than it saves.  Forking and freeing 16 sequences of 30 pages 6.3 us in one launch
+// each, 8.1 in two; 64 of 16 pages 10.4 and 8.0.  Planning a compaction with 3000 entries 5.8 and
+// 7.2, with 10000 10.8 and 9.0.
+constexpr int64_t kMoveHere = kThreads;
+constexpr int64_t kTableHere = 4 * kThreads;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -52,21 +55,35 @@ __device__ __forceinline__ int pages_of(int64_t len, int page_size) {
   return (int)((len + page_size - 1) / page_size);
 }
 
-// Which of pages p0 .. p0 + 15 are held (bit i: page p0 + i; pages past the pool count as held).
-__device__ __forceinline__ uint32_t held_mask(const int32_t* refs, int64_t p0, int64_t pages) {
-  uint32_t m = 0;
-  if (p0 + 16 <= pages && (reinterpret_cast<uintptr_t>(refs) & 15u) == 0) {
-    int4 v[4];
+// The counts of pages p0 .. p0 + 15, on their way; pages past the pool count as held.
+struct Counts {
+  int4 v[4];
+  __device__ __forceinline__ void load(const int32_t* refs, int64_t p0, int64_t pages) {
+    if (p0 + 16 <= pages && (reinterpret_cast<uintptr_t>(refs) & 15u) == 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const int4*>(refs + p0 + 4 * i);
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const int4*>(refs + p0 + 4 * i);
+    } else {
+      auto at = [&](int64_t p) { return p < pages ? refs[p] : 1; };
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = make_int4(at(p0 + 4 * i), at(p0 + 4 * i + 1), at(p0 + 4 * i + 2),
+                         at(p0 + 4 * i + 3));
+    }
+  }
+  // bit i: page p0 + i is held
+  __device__ __forceinline__ uint32_t held() const {
+    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       m |= ((v[i].x > 0) | (v[i].y > 0) << 1 | (v[i].z > 0) << 2 | (v[i].w > 0) << 3) << 4 * i;
     return m;
   }
-  for (int i = 0; i < 16; ++i)
-    if (p0 + i >= pages || refs[p0 + i] > 0) m |= 1u << i;
-  return m;
+};
+
+__device__ __forceinline__ uint32_t held_mask(const int32_t* refs, int64_t p0, int64_t pages) {
+  Counts c;
+  c.load(refs, p0, pages);
+  return c.held();
 }
 
 // What an entry of a call to fork or truncate moves: held pages from the first on.
@@ -74,35 +91,13 @@ struct Span {
   int row, from, first, held;            // row: the table row written; from: the one read
 };
 
-// Forks (FORK) or truncates: the spans' pages one a thread, four in turn so that their loads are
-// in flight together.
+// Forks (FORK) or truncates one page.
 template <bool FORK>
-__device__ __forceinline__ void move_pages(const mtl_page_state& st, const Span* spans, int n,
-                                           int widest) {
-  const int all = n * widest;              // at most kOneLaunch
-  for (int e0 = threadIdx.x; e0 < all; e0 += 4 * kThreads) {
-    int page[4], at[4], row[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = e0 + k * kThreads;
-      at[k] = -1;
-      if (e < all) {
-        const Span& s = spans[e / widest];
-        const int j = s.first + e % widest;
-        if (j < s.held) {
-          at[k] = j;
-          row[k] = s.row;
-          page[k] = st.table[s.from * st.ld + j];
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (at[k] < 0) continue;
-      st.table[row[k] * st.ld + at[k]] = FORK ? page[k] : -1;
-      if (page[k] >= 0 && page[k] < st.pages) atomicAdd(&st.refs[page[k]], FORK ? 1 : -1);
-    }
-  }
+__device__ __forceinline__ void move_page(const mtl_page_state& st, const Span& s, int j) {
+  if (j >= s.held) return;
+  const int p = st.table[s.from * st.ld + j];
+  st.table[s.row * st.ld + j] = FORK ? p : -1;
+  if (p >= 0 && p < st.pages) atomicAdd(&st.refs[p], FORK ? 1 : -1);
 }
 
 __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
@@ -114,8 +109,8 @@ __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
   __shared__ int waves[kWaves];
   __shared__ int bad, shared_pages;
   const int t = threadIdx.x;
-  // the first strip of the search, needed whatever the call holds
-  const uint32_t strip0 = 16 * t < st.pages ? held_mask(st.refs, 16 * t, st.pages) : 0xffffu;
+  Counts strip;                          // of the search for free pages, always one ahead
+  strip.load(st.refs, 16 * t, st.pages);
   clear_marks(seen, st.seqs);
   if (t == 0) bad = shared_pages = 0;
   __syncthreads();
@@ -159,8 +154,8 @@ __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
   if (!bad) {
     for (int64_t p0 = 0; p0 < st.pages && found < total; p0 += kStrip) {
       const int64_t p = p0 + 16 * t;
-      uint32_t free_pages = p0 == 0 ? strip0 : p < st.pages ? held_mask(st.refs, p, st.pages) : ~0u;
-      free_pages = ~free_pages & 0xffffu;
+      uint32_t free_pages = ~strip.held() & 0xffffu;
+      if (p0 + kStrip < st.pages) strip.load(st.refs, p + kStrip, st.pages);
       int here;
       int rank = found + block_scan(__popc(free_pages), waves, here);
       for (; free_pages && rank < total; free_pages &= free_pages - 1)
@@ -250,7 +245,10 @@ __global__ void __launch_bounds__(kThreads) pages_move_kernel(
   }
   if (ALL) {
     __syncthreads();
-    if (widest > 0) move_pages<FORK>(st, spans, n, widest);
+    for (int e = t; e < n * widest; e += kThreads) {       // at most kMoveHere
+      const Span& s = spans[e / widest];
+      move_page<FORK>(st, s, s.first + e % widest);
+    }
   }
 }
 
@@ -258,11 +256,7 @@ template <bool FORK>
 __global__ void __launch_bounds__(256) pages_move_wide_kernel(mtl_page_state st,
                                                               const Span* __restrict__ spans) {
   const Span s = spans[blockIdx.y];
-  const int j = s.first + blockIdx.x * 256 + threadIdx.x;
-  if (j >= s.held) return;
-  const int p = st.table[s.from * st.ld + j];
-  st.table[s.row * st.ld + j] = FORK ? p : -1;
-  if (p >= 0 && p < st.pages) atomicAdd(&st.refs[p], FORK ? 1 : -1);
+  move_page<FORK>(st, s, s.first + blockIdx.x * 256 + threadIdx.x);
 }
 
 __device__ __forceinline__ int moved(int p, int live, int64_t pages, const int32_t* goes) {
@@ -278,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(
     int32_t* table_out, int64_t ld_out) {
   __shared__ int waves[kWaves];
   const int t = threadIdx.x;
-  const int all = (int)(seqs * width), w = (int)width;   // with ALL at most kOneLaunch
+  const int all = (int)(seqs * width), w = (int)width;   // with ALL at most kTableHere
   int page[4];                               // the table's first entries
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -417,7 +411,7 @@ static int move_call(const mtl_page_state* st, const int32_t* a, const int32_t* 
   if (e != MTL_OK) return e;
   if (n > 0 && (!a || !b)) return MTL_ERR_INVALID_ARG;
   Span* spans = static_cast<Span*>(workspace);
-  if (n * st->width <= kOneLaunch) {
+  if (n * st->width <= kMoveHere) {
     pages_move_kernel<FORK, true><<<1, kThreads, 0, stream>>>(*st, a, b, (int)n, status, spans);
   } else {
     pages_move_kernel<FORK, false><<<1, kThreads, 0, stream>>>(*st, a, b, (int)n, status, spans);
@@ -475,7 +469,7 @@ extern "C" int mtl_pages_compact(const mtl_page_state* st, int32_t* table_out, i
     return MTL_ERR_INVALID_ARG;
   int32_t* goes = static_cast<int32_t*>(workspace);
   hipStream_t hs = (hipStream_t)stream;
-  if (st->seqs * st->width <= kOneLaunch) {
+  if (st->seqs * st->width <= kTableHere) {
     pages_compact_plan_kernel<true><<<1, kThreads, 0, hs>>>(
         st->refs, st->pages, refs_out, live, moves, move_src, move_dst, goes, st->table, st->ld,
         st->width, st->seqs, table_out, ld_out);

@@ -58,7 +58,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q [seqs, heads, head_dim]`` bf16 or fp16, any strides; softmax and sums in fp32.  Returns
     ``out`` like q, and with ``return_lse`` also the fp32 ``[seqs, heads]`` logarithm of the
     softmax sums, with which the result joins that of other keys.  A sequence without positions
-    gives 0 and -inf.  Lengths past the table's width count as that width."""
+    gives 0 and -inf.  Lengths past the table's width count as that width.  The same call gives
+    the same bits; the order of a sequence's sums goes by all lengths of the call."""
     op = ops.overload("paged_attention_lse" if return_lse else "paged_attention")
     return op(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale)
 

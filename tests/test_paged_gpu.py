@@ -739,6 +739,44 @@ def test_run_together(dev, kv, captured):
     run_stack(dev, kv, captured)
 
 
+def test_operators_keep_their_schemas(dev):
+    # only what a schema marks is written, and the meta kernels give the real shapes
+    from moss_tts_lite_amd import ops
+
+    def check(name, *args):
+        torch.library.opcheck(ops.overload(name), args, test_utils=("test_schema",
+                                                                    "test_faketensor"))
+
+    a = attend_case(3, 8, 2, 64, 16, "bf16", "bf16", [20, 0, 700], dev, 20)
+    for x in ("k_pages", "v_pages"):
+        a[x] = a[x].nan_to_num()                     # compared as values
+    args = [a[x] for x in ("q", "k_pages", "v_pages", "table", "lens", "scale")]
+    check("paged_attention", *args)
+    check("paged_attention_lse", *args)
+    qkv = torch.randn(3, 12 * 64, device=dev).bfloat16()
+    check("paged_write", qkv, a["k_pages"], a["v_pages"], a["table"],
+          torch.tensor([1, -1, 30], device=dev))
+    b = Both(dev, 5, 20, 4)
+    b.extend([0, 1], [20, 33])
+    check("pages_extend", *b.state(), ints([0, 2], dev), ints([3, 20], dev), b.k, b.v)
+    check("pages_fork", *b.state(), ints([0, 0], dev), ints([3, 4], dev), 16)
+    check("pages_truncate", *b.state(), ints([0, 1], dev), ints([0, 5], dev), 16)
+    check("pages_compact", b.table, b.refs, b.k, b.v)
+    check("pages_copy", b.k, b.v, ints([0], dev), ints([9], dev))
+
+
+def test_large_calls_of_two_launches(dev):
+    # more table entries than one workgroup moves or rewrites itself
+    b = Both(dev, 120, 700, 40)
+    assert b.extend(list(range(40)), [16 * (i % 17) + i for i in range(40)]) == 0
+    assert b.fork([i % 40 for i in range(60)], list(range(50, 110))) == 0
+    assert b.extend(list(range(50, 110)), [3] * 60) == 0
+    assert b.truncate(list(range(100)), [0 if i % 3 else min(b.plain.lens[i], 20)
+                                         for i in range(100)]) == 0
+    b.compact()
+    assert b.fork([60, 60], [60, 111]) == 2
+
+
 def test_calls_on_another_stream(dev):
     a = attend_case(4, 8, 2, 128, 16, "bf16", "bf16", [2100, 3, 700, 64], dev, 13)
     want = paged.paged_attention(**a)
