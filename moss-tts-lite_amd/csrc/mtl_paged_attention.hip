@@ -103,10 +103,11 @@ __device__ __forceinline__ int fresh(int x) {
   return x;
 }
 
-// table[i] for an i that is the same in all lanes, as a scalar load: a vector load would have
-// the wave wait for the K and V in flight before it.
-__device__ __forceinline__ int uniform_load(const int32_t* p, int64_t i) {
-  typedef const int32_t __attribute__((address_space(4)))* Constant;
+// p[i] for an i that is the same in all lanes, as a scalar load: a vector load would have the
+// wave wait for the K and V in flight before it.
+template <class T>
+__device__ __forceinline__ T uniform_load(const T* p, int64_t i) {
+  typedef const T __attribute__((address_space(4)))* Constant;
   return ((Constant)(uintptr_t)p)[i];
 }
 
@@ -420,6 +421,7 @@ struct Unit {
   const PagePool& pool;
   float* lds;
   int kvh, h0, heads;
+  float v_scale;
   typename Wave::Ends ends;
   Wave w;
 
@@ -432,7 +434,8 @@ struct Unit {
     ends.shift = __builtin_ctz(pool.page_size);
     ends.k = static_cast<const char*>(pool.k) + kvh * pool.k_head * w.E;
     ends.v = static_cast<const char*>(pool.v) + kvh * pool.v_head * w.E;
-    w.c = a.scale * (pool.k_scale ? pool.k_scale[kvh] : 1.f) * kLog2e;
+    w.c = a.scale * (pool.k_scale ? uniform_load(pool.k_scale, kvh) : 1.f) * kLog2e;
+    v_scale = pool.v_scale ? uniform_load(pool.v_scale, kvh) : 1.f;
   }
 
   // What depends on the lane is formed anew for each piece: kept from one to the next, with what
@@ -494,8 +497,7 @@ struct Unit {
         o += e * *reinterpret_cast<const floatx4*>(lds + (x * a.tile_heads + h) * LD + d);
       }
       if (dst < 0) {
-        write_out<QT, D>(a.out, a.lse, (int64_t)seq * a.n_heads + h0 + h, d, o, mu, sum,
-                         pool.v_scale ? pool.v_scale[kvh] : 1.f);
+        write_out<QT, D>(a.out, a.lse, (int64_t)seq * a.n_heads + h0 + h, d, o, mu, sum, v_scale);
       } else {
         *reinterpret_cast<floatx4*>(a.part + (dst + h) * D + d) = o;
         if (d == 0) {
