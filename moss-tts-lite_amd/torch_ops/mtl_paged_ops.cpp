@@ -8,6 +8,7 @@
 // graphs captured from them share nothing.  Meta kernels make the same checks and give the
 // output shapes to tracing.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -206,6 +207,8 @@ at::Tensor paged_write(const at::Tensor& qkv, const at::Tensor& k_pages, const a
               qkv.sizes());
   const int32_t type = row_type(qkv, "qkv");
   const mtl_page_pool pool = pool_of(k_pages, v_pages, k_scale, v_scale, type);
+  at::assert_no_internal_overlap(k_pages);
+  at::assert_no_internal_overlap(v_pages);
   const mtl_page_table tab = table_of(table);
   const int64_t rows = qkv.size(0), d = pool.head_dim;
   const int64_t heads = qkv.size(1) / d - 2 * (int64_t)pool.kv_heads;
@@ -322,6 +325,7 @@ PageBlocks blocks_of(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf ||
                   t.scalar_type() == at::kFloat8_e4m3fn,
               name, " must be bfloat16, float16 or float8_e4m3fn, got ", t.scalar_type());
+  at::assert_no_internal_overlap(t);
   const int64_t e = t.element_size(), p = t.dim() - 4;
   // kv_heads, page_size and head_dim have to fill one block, in any order
   std::array<std::pair<int64_t, int64_t>, 3> dims;

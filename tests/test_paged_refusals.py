@@ -86,6 +86,16 @@ def test_attention_refusals(lib):
                          nbytes=ws) == N.MTL_ERR_WORKSPACE
 
 
+def test_launch_limits(lib):
+    # more threads than a launch can have: refused, not left to the launch
+    p = dict(kv_heads=256, k_page=256 * 16 * 128, v_page=256 * 16 * 128)
+    assert attention(lib, pool(**p), table(width=1, ld=1, seqs=65535), heads=256,
+                     ldq=256 * 128) == N.MTL_ERR_SHAPE
+    assert write(lib, pool(), table(), rows=1 << 24) == N.MTL_ERR_SHAPE
+    assert attention(lib, pool(), table(seqs=65536)) == N.MTL_ERR_SHAPE
+    assert attention(lib, pool(), table(width=(1 << 26) + 1, ld=1 << 27)) == N.MTL_ERR_SHAPE
+
+
 def test_write_refusals(lib):
     assert write(lib, pool(), table(), norms=(FAKE, None)) == N.MTL_ERR_INVALID_ARG
     assert write(lib, pool(), table(), rope=(None, FAKE)) == N.MTL_ERR_INVALID_ARG
@@ -231,6 +241,21 @@ def test_write_operator_refusals(kw, what):
     with pytest.raises(RuntimeError, match=what):
         paged.paged_write(**write_args(**kw))
     assert paged.paged_write(**write_args()).shape == (5, 32, 128)
+
+
+def test_pages_that_overlap_are_not_written():
+    one = meta(1, 8, 16, 128).expand(9, 8, 16, 128)
+    with pytest.raises(RuntimeError, match="single memory location"):
+        paged.paged_write(**write_args(k_pages=one))
+    with pytest.raises(RuntimeError, match="single memory location"):
+        paged.paged_write(**write_args(v_pages=meta(9, 1, 16, 128).expand(9, 8, 16, 128)))
+    layers = meta(1, 9, 8, 16, 128).expand(2, 9, 8, 16, 128)
+    for k, v in ((layers, meta(2, 9, 8, 16, 128)), (meta(2, 9, 8, 16, 128), layers)):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            paged.pages_copy(k, v, i32(2), i32(2))
+        with pytest.raises(RuntimeError, match="single memory location"):
+            paged.pages_compact(i32(6, 4), i32(9), k, v)
+    assert paged.paged_attention(**attend_args(k_pages=one, v_pages=one)).shape == (2, 32, 128)
 
 
 def book(**kw):
