@@ -70,7 +70,10 @@ typedef struct mtl_page_table {
  *   workspace  mtl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, any content,
  *        one launch at a time
  * The pages have q_type's type or E4M3.  n_heads % kv_heads == 0, n_heads and seqs at most
- * 65535.  The same call gives the same bits; the order of a sequence's sums goes by all lengths.
+ * 65535, and with width * page_size <= 512 seqs * kv heads * (query heads of one / 16, rounded
+ * up) at most 2^23 - 1.  The same call gives the same bits; the order of a sequence's sums goes by
+ * all lengths.  Nothing in a hole or past a length has an effect, NaN included; K and V of the
+ * positions attended to are finite (an infinity or NaN there gives NaN where it enters).
  */
 int64_t mtl_paged_attention_workspace_bytes(int64_t seqs, int32_t n_heads, int32_t kv_heads,
                                             int32_t head_dim, int64_t width, int32_t page_size);

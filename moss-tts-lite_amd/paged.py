@@ -59,7 +59,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``out`` like q, and with ``return_lse`` also the fp32 ``[seqs, heads]`` logarithm of the
     softmax sums, with which the result joins that of other keys.  A sequence without positions
     gives 0 and -inf.  Lengths past the table's width count as that width.  The same call gives
-    the same bits; the order of a sequence's sums goes by all lengths of the call."""
+    the same bits; the order of a sequence's sums goes by all lengths of the call.  What lies in
+    a hole or past a length has no effect, NaN included; K and V of the positions attended to
+    are finite (an infinity or NaN there gives NaN where it enters)."""
     op = ops.overload("paged_attention_lse" if return_lse else "paged_attention")
     return op(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale)
 
