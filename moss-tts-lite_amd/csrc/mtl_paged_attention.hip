@@ -24,11 +24,12 @@
 //
 // Measured, head_dim 128, bf16, a memory rate of 7.1 TB/s for such reads: one sequence of 131 000
 // positions and 4 kv heads (537 MB) 81 + 5 us in the two launches, 6.6 TB/s in the first; 128
-// ragged sequences (594 MB) 97 + 5 us, 6.1 TB/s; 256 sequences in e4m3 (322 MB) 55 + 5 us, 5.9
-// TB/s, where what bounds it is also that half the bytes come of the same number of loads; a
-// short table (300 positions) 6 us, which is a launch and three trips to the memory (length and
-// page ids, tile, output).
-// The counters show no byte of the cache read twice.
+// ragged sequences (594 MB) 97 + 5 us, 6.1 TB/s; ragged sequences in e4m3 (322 MB) 55 + 5 us, 5.8
+// TB/s.  About 10 us of that do not grow with the bytes (two launches; lengths, page ids and the
+// first tile, which wait for one another; the join), the rest streams at 7 TB/s: 307 MB take 53
+// to 56 us in bf16 and 55 to 58 in e4m3, as one sequence or as 64 equal ones, in pages of 16, 64
+// or 256.  A short table (300 positions) takes 6 us, which is a launch and three trips to the
+// memory (length and page ids, tile, output).  The counters show no byte of the cache read twice.
 //
 // Tried and slower: 3 or 4 waves on each of a CU's four parts (their registers spill), the next
 // sequence's first tile loaded ahead (even), 6, 8 or 12 waves in 256 workgroups, shares in tiles

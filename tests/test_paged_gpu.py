@@ -93,6 +93,57 @@ def test_attention_many_sequences_split(dev, B):
     check_attention(attend_case(B, 4, 2, 64, 16, "bf16", "bf16", lens, dev, B))
 
 
+def widen(a, width):
+    """The case with a table of `width` entries a row, holes behind its own."""
+    t = a["table"]
+    wide = torch.full((t.shape[0], width), -1, dtype=torch.int32, device=t.device)
+    wide[:, :t.shape[1]] = t
+    return {**a, "table": wide}
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_attention_edges_of_long_tables(dev, page, kv):
+    # the lengths of a table whose sequences are shared among the workgroups
+    lens = EDGES + [511, 512, 513, 640]
+    check_attention(widen(attend_case(len(lens), 8, 2, 128, page, "bf16", kv, lens, dev, page),
+                          1024 // page))
+
+
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (7, 1), (16, 1), (17, 1), (40, 2), (96, 2), (32, 8)])
+@pytest.mark.parametrize("typ,kv,D", [("bf16", "bf16", 128), ("f16", "f16", 64),
+                                      ("f16", "e4m3", 128), ("bf16", "e4m3", 64)])
+def test_attention_heads_and_types_of_long_tables(dev, H, Hkv, typ, kv, D):
+    check_attention(attend_case(4, H, Hkv, D, 16, typ, kv, [1500, 0, 700, 129], dev, H))
+
+
+@pytest.mark.parametrize("H,Hkv", [(600, 600), (256, 256), (514, 257)])
+def test_attention_many_kv_heads(dev, H, Hkv):
+    # no more than a piece or two for each kv head
+    check_attention(attend_case(3, H, Hkv, 64, 16, "bf16", "bf16", [600, 0, 150], dev, 3))
+
+
+def test_attention_holes_and_layouts_of_long_tables(dev):
+    a = attend_case(5, 8, 2, 128, 16, "bf16", "bf16", [900, 300, 640, 200, 48], dev, 21)
+    t = a["table"]
+    t[0, 0] = t[0, 7] = t[0, 8] = -1                 # at the start, a whole tile
+    t[0, 30:50] = a["k_pages"].shape[0]              # whole blocks
+    t[1, 18] = -3                                    # the partly filled last page
+    t[3, :] = 2 ** 31 - 1                            # nothing left
+    a["lens"][4] = 2 ** 31 - 1                       # past the table; its other entries are -1
+    t[4, 2] = t[4, 1]
+    want = check_attention(a)
+    token_first = {x: a[x].transpose(1, 2).contiguous().transpose(1, 2)
+                   for x in ("k_pages", "v_pages")}
+    assert torch.equal(paged.paged_attention(**{**a, **token_first}), want)
+    both = torch.stack([a["k_pages"], a["v_pages"]], 1)
+    assert torch.equal(paged.paged_attention(**{**a, "k_pages": both[:, 0], "v_pages": both[:, 1]}),
+                       want)
+    wide = torch.zeros(5, 12, 128, dtype=torch.bfloat16, device=dev)
+    wide[:, 2:10] = a["q"]
+    assert torch.equal(paged.paged_attention(**{**a, "q": wide[:, 2:10]}), want)
+
+
 def test_attention_peaked_scores(dev):
     # one position holds nearly all the weight, far below or above the others
     check_attention(attend_case(3, 8, 2, 128, 16, "bf16", "bf16", [400, 33, 1000], dev, 1,
@@ -331,6 +382,15 @@ def test_write_heads_and_rows(dev, H, Hkv, rows, pad):
 def test_write_a_prompt_of_each_sequence(dev):
     n = 90
     check_write(dev, 3 * n, 8, 2, 128, 16, "bf16", "bf16", True,
+                positions=torch.arange(n).repeat(3) + 3, n_seqs=4,
+                seqs=torch.tensor([2, 0, 3], dtype=torch.int32).repeat_interleave(n))
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(8, 2, 128), (30, 6, 64), (1, 1, 64)])
+def test_write_many_rows(dev, H, Hkv, D):
+    # a workgroup takes all heads of a row, in turns
+    n = 175
+    check_write(dev, 3 * n, H, Hkv, D, 32, "bf16", "e4m3" if D == 64 else "bf16", True,
                 positions=torch.arange(n).repeat(3) + 3, n_seqs=4,
                 seqs=torch.tensor([2, 0, 3], dtype=torch.int32).repeat_interleave(n))
 
