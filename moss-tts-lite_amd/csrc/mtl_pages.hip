@@ -86,7 +86,8 @@ __device__ __forceinline__ uint32_t held_mask(const int32_t* refs, int64_t p0, i
   return c.held();
 }
 
-// What an entry of a call to fork or truncate moves: held pages from the first on.
+// What an entry of a call to fork or truncate moves: pages first .. held - 1, none where held is
+// not past first (a refused call's spans are empty: row and from may lie outside the table).
 struct Span {
   int row, from, first, held;            // row: the table row written; from: the one read
 };
@@ -235,8 +236,9 @@ __global__ void __launch_bounds__(kThreads) pages_move_kernel(
   const bool ok = !bad;
   if (t == 0) status[0] = ok ? 0 : 2;
   if (t < n) {
-    Span s{FORK ? y : x, x, FORK ? 0 : pages_of(y, st.page_size), 0};
+    Span s{FORK ? y : x, x, 0, 0};
     if (ok) {
+      if (!FORK) s.first = pages_of(y, st.page_size);
       s.held = pages_of(len, st.page_size);
       st.lens[s.row] = FORK ? (int)len : y;
     }

@@ -1,0 +1,93 @@
+"""The paged cache on the device where a call goes past the usual: refused bookkeeping calls with
+wild arguments, compared with everything around the state they must leave alone."""
+import pytest
+import torch
+
+from moss_tts_lite_amd import paged
+from tests._paged import Pages
+
+pytestmark = pytest.mark.gpu
+
+PAGE = 16
+
+
+def ints(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+# ------------------------------------------------------------------------------ refused calls
+class Guarded:
+    """Sequences in the middle of larger buffers, so that a write beside the state shows: every
+    page is held by somebody, every entry of the buffers names a page or its place."""
+
+    def __init__(self, dev, seqs, width, lens, ahead=70):
+        self.dev, self.seqs, self.width = dev, seqs, width
+        pages = seqs * width + 8
+        gen = torch.Generator().manual_seed(seqs)
+        self.all = {
+            "table": torch.randint(0, pages, (seqs + 2 * ahead, width), generator=gen),
+            "lens": torch.randint(0, 50, (seqs + 2 * ahead,), generator=gen),
+            "refs": torch.randint(1, 5, (pages + 2 * ahead,), generator=gen)}
+        self.all = {k: v.int().to(dev) for k, v in self.all.items()}
+        self.table = self.all["table"][ahead:ahead + seqs]
+        self.lens = self.all["lens"][ahead:ahead + seqs]
+        self.refs = self.all["refs"][ahead:ahead + pages]
+        self.lens.copy_(ints([lens(i) for i in range(seqs)], dev))
+        self.plain = Pages(self.table, self.lens, self.refs, PAGE)
+
+    def refused(self, op, a, b):
+        """The call, by name; it must be refused, by the plain form too, and change nothing."""
+        assert getattr(self.plain, op)(a, b) == 2
+        was = {k: v.clone() for k, v in self.all.items()}
+        call = getattr(paged, "pages_" + op)
+        st = call(self.table, self.lens, self.refs, ints(a, self.dev), ints(b, self.dev), PAGE)
+        assert int(st) == 2
+        for k, v in self.all.items():
+            assert torch.equal(v, was[k]), (op, a[:4], b[:4], k)
+
+
+WILD = [-1, -PAGE, -2 * PAGE + 1, -2 * PAGE, -1000, -2 ** 31 + 15, -2 ** 31, 2 ** 31 - 1]
+
+
+# one launch (entries times width at most 1024), and a launch that decides and one that moves
+@pytest.mark.parametrize("seqs,width", [(6, 4), (40, 70)])
+def test_refused_truncates_change_nothing(dev, seqs, width):
+    g = Guarded(dev, seqs, width, lambda i: (7 * i + 5) % (width * PAGE))
+    many = list(range(seqs))
+    for y in WILD:
+        for s in (0, seqs // 2, seqs - 1, seqs, -1, 2 ** 31 - 1, -2 ** 31):
+            g.refused("truncate", [s], [y])
+            keep = [0] * seqs
+            if 0 <= s < seqs:
+                keep[s] = y
+                g.refused("truncate", many, keep)
+            else:
+                g.refused("truncate", many + [s], keep + [y])
+    g.refused("truncate", many + [3], [0] * (seqs + 1))           # one twice
+    g.refused("truncate", many, [y for y in (WILD * 8)[:seqs]])
+
+
+@pytest.mark.parametrize("seqs,width", [(6, 4), (40, 70)])
+def test_refused_forks_change_nothing(dev, seqs, width):
+    half = seqs // 2
+    g = Guarded(dev, seqs, width, lambda i: 0 if i >= half else 11 * i + 1)
+    kids = list(range(half, seqs))
+    parents = [i % half for i in range(len(kids))]
+    for x in (seqs, -1, 2 ** 31 - 1, -2 ** 31, half):
+        g.refused("fork", [x] + parents[1:], kids)                # half: a child as a parent
+    for y in (seqs, -1, 2 ** 31 - 1, -2 ** 31, 0, kids[-1]):
+        g.refused("fork", parents, [y] + kids[1:])                # 0: not empty; the last one twice
+
+
+@pytest.mark.parametrize("seqs,width", [(6, 4), (40, 70)])
+def test_refused_calls_on_broken_lengths_change_nothing(dev, seqs, width):
+    # lengths that no call leaves behind: negative, or past the table
+    for bad in (-1, -1000, -2 ** 31, width * PAGE + 1, 2 ** 31 - 1):
+        g = Guarded(dev, seqs, width, lambda i: bad if i == 2 else 0)
+        if bad > 0:                                               # the plain form knows no width here
+            g.plain.truncate = g.plain.fork = lambda a, b: 2
+        else:
+            g.plain.fork = lambda a, b: 2
+        g.refused("truncate", [2, 1], [0, 0])
+        g.refused("fork", [2, 2], [1, 0])
+        g.refused("truncate", list(range(seqs)), [0] * seqs)
