@@ -20,6 +20,17 @@ Everything lives and is decided on the device, nothing waits for it, every launc
 current stream and can be captured into a graph.  The bookkeeping calls return a ``status``
 tensor (0 done, 1 not enough free pages, 2 a bad argument), and one that is not 0 has changed
 nothing; :func:`check` reads it and raises.  ``RuntimeError`` for a wrong shape, type or device.
+
+After a refused :func:`pages_extend` the lengths are the old ones, and the position before a
+sequence's end is a token that is there already, on a page that others may hold too.  A loop that
+does not wait for the status makes its rows padding then.  One token of every sequence in ``seqs``::
+
+    status = paged.pages_extend(table, lens, refs, seqs, torch.ones_like(seqs), k, v)
+    rows, n = table[seqs], lens[seqs]
+    at = torch.where(status == 0, n.long() - 1, -1)
+    for l in range(layers):
+        q = paged.paged_write(qkv[l], k[l], v[l], rows, at, None, q_norm, k_norm, cos, sin)
+        out = paged.paged_attention(q, k[l], v[l], rows, n, scale)
 """
 from __future__ import annotations
 
@@ -93,7 +104,8 @@ def pages_extend(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, se
     """Room for ``counts[i]`` more tokens of sequence ``seqs[i]`` (int32 ``[n]``, n <= 1024, no
     sequence twice), in call order (``mtl_pages_extend``): a partly filled last page that other
     sequences hold too is first replaced by a copy, in all layers; then the lowest free pages are
-    taken one after the other.  ``lens`` grows by ``counts``.  Returns the status."""
+    taken one after the other.  ``lens`` grows by ``counts``.  Returns the status; unless it is 0
+    there is no room, and the last positions of the sequences are not to be written."""
     return ops.overload("pages_extend")(table, lens, refs, seqs, counts, k_pages, v_pages)
 
 

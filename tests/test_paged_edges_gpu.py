@@ -1,5 +1,8 @@
 """The paged cache on the device where a call goes past the usual: refused bookkeeping calls with
-wild arguments, compared with everything around the state they must leave alone."""
+wild arguments, compared with everything around the state they must leave alone, and the documented
+decode step when its extend is refused."""
+import textwrap
+
 import pytest
 import torch
 
@@ -91,3 +94,54 @@ def test_refused_calls_on_broken_lengths_change_nothing(dev, seqs, width):
         g.refused("truncate", [2, 1], [0, 0])
         g.refused("fork", [2, 2], [1, 0])
         g.refused("truncate", list(range(seqs)), [0] * seqs)
+
+
+def documented_step():
+    """The step of the module's documentation."""
+    return textwrap.dedent(paged.__doc__.split("in ``seqs``::\n\n", 1)[1])
+
+
+# what a step meets: no pages left; a sequence at the end of its row; a sequence given twice
+@pytest.mark.parametrize("pages,seqs,want", [(5, [0, 1], 1), (40, [0, 1, 3], 2), (40, [1, 1], 2),
+                                             (40, [0, 1], 0)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_the_documented_step_leaves_the_cache_when_it_is_refused(dev, pages, seqs, want, captured):
+    gen = torch.Generator().manual_seed(pages)
+    H, Hkv, D, layers, width = 8, 2, 64, 2, 3
+    k, v, table, lens, refs = paged.new_cache(layers, pages, Hkv, PAGE, D, 5, width, device=dev)
+    for x in (k, v):
+        x.copy_(torch.randn(x.shape, generator=gen))
+    fill = ([0, 1], [32, 20]) if pages == 5 else ([0, 1, 3], [30, 20, width * PAGE])
+    paged.check(paged.pages_extend(table, lens, refs, *(ints(x, dev) for x in fill), k, v))
+    paged.check(paged.pages_fork(table, lens, refs, ints([1], dev), ints([4], dev), PAGE))
+    norm = [torch.ones(D, device=dev).bfloat16() for _ in range(2)]
+    env = dict(paged=paged, torch=torch, k=k, v=v, table=table, lens=lens, refs=refs,
+               seqs=ints(seqs, dev), layers=layers, scale=D ** -0.5, q_norm=norm[0],
+               k_norm=norm[1], cos=torch.ones(width * PAGE, D, device=dev),
+               sin=torch.zeros(width * PAGE, D, device=dev),
+               qkv=torch.randn(layers, len(seqs), (H + 2 * Hkv) * D, generator=gen).bfloat16()
+               .to(dev))
+    was = [x.clone() for x in (k, v, table, lens, refs)]
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            exec(documented_step(), env)
+        for x, y in zip((k, v, table, lens, refs), was):
+            assert torch.equal(x, y)
+        graph.replay()
+    else:
+        exec(documented_step(), env)
+    assert int(env["status"]) == want
+    if want:
+        assert not env["q"].any()
+        for x, y in zip((k, v, table, lens, refs), was):
+            assert torch.equal(x, y)
+        return
+    assert lens.tolist()[:2] == [31, 21]
+    for i, n in zip(seqs, (30, 20)):                 # each row's values, where its token goes
+        at = int(table[i, n // PAGE])
+        got = v[:, at, :, n % PAGE]
+        row = env["qkv"][:, seqs.index(i)].reshape(layers, H + 2 * Hkv, D)[:, H + Hkv:]
+        assert torch.equal(got, row)
+    assert torch.equal(was[1][:, was[2][4, 1]], v[:, table[4, 1]])     # the fork's page is its own
