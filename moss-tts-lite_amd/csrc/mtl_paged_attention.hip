@@ -13,8 +13,9 @@
 //   loads 16 bytes of dims for each of its 8 positions and transposes them with v_perm.
 // * The maximum and sum of the softmax run along (fp32); accumulators are rescaled only when a
 //   maximum grew.  Weights enter the product as two rows-type numbers, the rounded weight and
-//   what the rounding left: the output is then off by its own rounding alone (with one, by
-//   1.4 times that).
+//   what the rounding left: a weight is off by 2^-16 of itself in bf16, by 2^-20 of itself and
+//   2^-39 of the largest in f16, far below the output's own rounding (with one number the output
+//   is off by 1.4 times as much).  f16 ends at 2^-24, so its weights enter 2^15 larger.
 // * A launch of kWorkgroups workgroups, all on the chip at once, shares the blocks of 128
 //   positions of all sequences evenly: the blocks stand in one row, sequence after sequence, and
 //   each workgroup of a kv head finds its piece of that row on the device from the lengths.  A
@@ -171,6 +172,13 @@ __device__ __forceinline__ int clamp_len(int32_t len, int64_t cap) {
   return len < 0 ? 0 : (int)(len < cap ? len : cap);
 }
 
+// What weights are multiplied with as they enter the product, whose sums carry it to the output: in
+// f16 2^15 (the largest weight is 1, f16 ends at 65504 and 2^-24).  As they are, weights more than
+// 16.6 nats below the largest would be 0 in both terms and the others lose up to 2^-24, while
+// their sum counts them in full.
+template <int QT>
+constexpr float kLift = QT == MTL_T_F16 ? 32768.f : 1.f;
+
 // A wave's part of one piece of one sequence, for up to 16 query heads of one kv head.
 template <int QT, int KT, int D, int WAVES, bool ONCE>
 struct Attend {
@@ -301,7 +309,7 @@ struct Attend {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t a, b;
-      two_terms<QT>(s[2 * j], s[2 * j + 1], a, b);
+      two_terms<QT>(s[2 * j] * kLift<QT>, s[2 * j + 1] * kLift<QT>, a, b);
       hi[j] = a;
       lo[j] = b;
     }
@@ -410,7 +418,7 @@ template <int QT, int D>
 __device__ __forceinline__ void write_out(uint16_t* __restrict__ out, float* __restrict__ lse,
                                           int64_t head, int d, floatx4 o, float top, float sum,
                                           float vs) {
-  const float f = sum == 0.f ? 0.f : vs / sum;
+  const float f = sum == 0.f ? 0.f : vs / sum * (1.f / kLift<QT>);
   *reinterpret_cast<u32x2*>(out + head * D + d) =
       u32x2{pack_out<QT>(o[0] * f, o[1] * f), pack_out<QT>(o[2] * f, o[3] * f)};
   if (lse && d == 0)
