@@ -109,12 +109,18 @@ __global__ void __launch_bounds__(256) paged_write_kernel(
     const float* scale = is_v ? pool.v_scale : pool.k_scale;
     if (KT == MTL_T_E4M3 && scale) {
       // x / by rounded once: the product with the rounded reciprocal, corrected by the remainder
-      // (a quotient past 1e30, an infinity or a NaN is stored as 448 or NaN without it)
+      // (a quotient past 1e30, an infinity or a NaN is stored as 448 or NaN without it).  The
+      // reciprocal and the remainder need a scale far from float32's ends; others are divided by.
       const float by = scale[kvh], inv = 1.f / by;
+      if (fabsf(by) > 0x1p-100f && fabsf(by) < 0x1p100f) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = x[j] * inv;
-        x[j] = fabsf(q) < 1e30f ? fmaf(fmaf(-q, by, x[j]), inv, q) : q;
+        for (int j = 0; j < 8; ++j) {
+          const float q = x[j] * inv;
+          x[j] = fabsf(q) < 1e30f ? fmaf(fmaf(-q, by, x[j]), inv, q) : q;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] /= by;
       }
     }
     if (is_v)
