@@ -96,6 +96,8 @@ mtl_page_pool pool_of(const at::Tensor& k, const at::Tensor& v, const OptTensor&
   TORCH_CHECK(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
               "k_pages and v_pages must have the same shape and type");
   check_same_device(k, {&v});
+  TORCH_CHECK(k.size(0) <= INT32_MAX && k.size(1) <= 65535,
+              "at most 2^31 - 1 pages and 65535 kv heads, got ", k.sizes());
   TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, "head_dim must be 64 or 128, got ", k.size(3));
   check_page_size(k.size(2));
   check_scale(k_scale, k, "k_scale");
@@ -159,6 +161,10 @@ at::Tensor attend(const at::Tensor& q, const at::Tensor& k_pages, const at::Tens
               pool.head_dim);
   TORCH_CHECK(h >= 1 && h % pool.kv_heads == 0, "q's ", h, " heads must be a multiple of the ",
               pool.kv_heads, " kv heads");
+  TORCH_CHECK(h <= 65535 && b <= 65535, "at most 65535 heads and 65535 sequences, got ", q.sizes());
+  TORCH_CHECK(tab.width <= (int64_t{1} << 30) / pool.page_size,
+              "a sequence has at most 2^30 positions, the table ", tab.width, " pages of ",
+              pool.page_size);
   TORCH_CHECK(tab.seqs == b && lens.size(0) == b, "q, table and lens must have the same number of "
               "sequences, got ", b, ", ", tab.seqs, " and ", lens.size(0));
   at::Tensor out = at::empty({b, h, q.size(2)}, q.options());
@@ -214,6 +220,8 @@ at::Tensor paged_write(const at::Tensor& qkv, const at::Tensor& k_pages, const a
   const int64_t heads = qkv.size(1) / d - 2 * (int64_t)pool.kv_heads;
   TORCH_CHECK(qkv.size(1) % d == 0 && heads >= 1, "qkv has ", qkv.size(1),
               " columns: (heads + 2 * ", pool.kv_heads, ") * ", d, " are expected");
+  TORCH_CHECK(heads + 2 * (int64_t)pool.kv_heads <= 65535 && rows <= UINT32_MAX / 256,
+              "at most 65535 heads of q, k and v and 2^24 - 1 rows, got ", qkv.sizes());
   check_same_device(qkv, {&k_pages, &table, &positions});
   TORCH_CHECK(positions.scalar_type() == at::kLong && positions.dim() == 1 &&
                   positions.size(0) == rows && positions.is_contiguous(),
@@ -285,6 +293,8 @@ mtl_page_state state_of(const at::Tensor& table, const OptTensor& lens, const at
   check_same_device(table, {&refs});
   TORCH_CHECK(t.seqs <= MTL_PAGES_MAX_SEQS, "at most ", MTL_PAGES_MAX_SEQS, " sequences, got ",
               t.seqs);
+  TORCH_CHECK(t.width <= MTL_PAGES_MAX_WIDTH, "at most ", MTL_PAGES_MAX_WIDTH,
+              " pages a sequence, got ", t.width);
   check_page_size(page_size);
   if (lens.has_value()) {
     check_int32(*lens, 1, "lens");

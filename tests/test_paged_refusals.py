@@ -331,3 +331,32 @@ def test_check_reads_a_status():
     for code, what in ((1, "free pages"), (2, "given twice")):
         with pytest.raises(RuntimeError, match=what):
             paged.check(torch.tensor([code]))
+
+
+# ------------------------------------------------------------------ limits, checked before a device
+@pytest.mark.parametrize("kv", [65536, 1 << 32, (1 << 32) + 8])
+def test_more_kv_heads_than_a_launch_takes(kv):
+    # 2^32 heads of stride 0 were 0 in the launch's 32 bits, and q's heads divided by that
+    k = meta(9, 1, 16, 128).expand(9, kv, 16, 128)
+    with pytest.raises(RuntimeError, match="65535 kv heads"):
+        paged.paged_attention(**attend_args(k_pages=k, v_pages=k))
+    with pytest.raises(RuntimeError, match="65535 kv heads"):
+        paged.paged_write(**write_args(k_pages=k, v_pages=k))
+
+
+def test_more_work_than_a_launch_takes():
+    many = meta(1, 1, 128).expand(2, 65536, 128)
+    with pytest.raises(RuntimeError, match="65535 heads"):
+        paged.paged_attention(**attend_args(q=many))
+    with pytest.raises(RuntimeError, match="65535 sequences"):
+        paged.paged_attention(**attend_args(q=meta(65536, 32, 128), table=i32(65536, 4),
+                                            lens=i32(65536)))
+    with pytest.raises(RuntimeError, match="2\\^30 positions"):
+        paged.paged_attention(**attend_args(table=i32(2, (1 << 26) + 1)))
+    with pytest.raises(RuntimeError, match="rows"):
+        paged.paged_write(**write_args(qkv=meta(1 << 24, 48 * 128), table=i32(1 << 24, 4),
+                                       positions=meta(1 << 24, dtype=torch.int64)))
+    with pytest.raises(RuntimeError, match="pages a sequence"):
+        paged.pages_fork(**book(table=i32(6, (1 << 20) + 1)), parents=i32(2), children=i32(2),
+                         page_size=16)
+    assert paged.paged_attention(**attend_args(table=i32(2, 1 << 26))).shape == (2, 32, 128)
