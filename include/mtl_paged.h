@@ -99,7 +99,7 @@ int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh, const mtl_page_
  * entries round after every step as the reference does).  E4M3 pages store x / scale,
  * limited to +-448, rounded to nearest even.  Rows whose page is a hole, whose position lies
  * past the table or whose sequence is outside it write no page.  No two rows may name the
- * same position of the same sequence.
+ * same position of the same sequence, and no two places of k and v are the same memory.
  */
 int mtl_paged_write(const void* qkv, int64_t ldq, int64_t rows, const mtl_page_pool* pool,
                     const mtl_page_table* table, const int64_t* positions, const int32_t* row_seq,

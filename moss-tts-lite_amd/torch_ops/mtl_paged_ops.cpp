@@ -8,7 +8,6 @@
 // graphs captured from them share nothing.  Meta kernels make the same checks and give the
 // output shapes to tracing.
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -72,6 +71,37 @@ void check_scale(const OptTensor& s, const at::Tensor& pages, const char* name) 
                   s->is_contiguous(),
               name, " must be contiguous float32 [", pages.size(1), "]");
   check_same_device(pages, {&*s});
+}
+
+// Pages that are written (at most 5 dimensions): no two of their elements may be the same memory.
+// Each stride has to pass over all that the smaller ones reach.
+void check_apart(const at::Tensor& t, const char* name) {
+  if (t.numel() == 0) return;
+  std::array<std::pair<int64_t, int64_t>, 5> dims;
+  int64_t n = 0;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) dims[n++] = {t.stride(d), t.size(d)};
+  std::sort(dims.begin(), dims.begin() + n);
+  int64_t reach = 1;
+  for (int64_t i = 0; i < n; ++i) {
+    const auto& [stride, size] = dims[i];
+    TORCH_CHECK(stride >= reach, name, "'s pages overlap, several elements are a single memory "
+                "location: ", t.sizes(), " with strides ", t.strides());
+    reach += (size - 1) * stride;
+  }
+}
+
+// Keys and values that are written, of one type: dense blocks of one storage must not meet.  Where
+// both get the same bytes (`same`) they may be one.
+void check_pools_apart(const at::Tensor& k, const at::Tensor& v, bool same) {
+  if (!k.has_storage() || !v.has_storage() ||
+      k.storage().unsafeGetStorageImpl() != v.storage().unsafeGetStorageImpl() ||
+      !k.is_non_overlapping_and_dense() || !v.is_non_overlapping_and_dense() ||
+      (same && k.storage_offset() == v.storage_offset() && k.strides() == v.strides()))
+    return;
+  TORCH_CHECK(k.storage_offset() + k.numel() <= v.storage_offset() ||
+                  v.storage_offset() + v.numel() <= k.storage_offset(),
+              "k_pages and v_pages share memory");
 }
 
 // One layer's pages [pages, kv_heads, page_size, head_dim] with any strides that keep the
@@ -213,8 +243,9 @@ at::Tensor paged_write(const at::Tensor& qkv, const at::Tensor& k_pages, const a
               qkv.sizes());
   const int32_t type = row_type(qkv, "qkv");
   const mtl_page_pool pool = pool_of(k_pages, v_pages, k_scale, v_scale, type);
-  at::assert_no_internal_overlap(k_pages);
-  at::assert_no_internal_overlap(v_pages);
+  check_apart(k_pages, "k_pages");
+  check_apart(v_pages, "v_pages");
+  check_pools_apart(k_pages, v_pages, false);
   const mtl_page_table tab = table_of(table);
   const int64_t rows = qkv.size(0), d = pool.head_dim;
   const int64_t heads = qkv.size(1) / d - 2 * (int64_t)pool.kv_heads;
@@ -335,7 +366,7 @@ PageBlocks blocks_of(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf ||
                   t.scalar_type() == at::kFloat8_e4m3fn,
               name, " must be bfloat16, float16 or float8_e4m3fn, got ", t.scalar_type());
-  at::assert_no_internal_overlap(t);
+  check_apart(t, name);
   const int64_t e = t.element_size(), p = t.dim() - 4;
   // kv_heads, page_size and head_dim have to fill one block, in any order
   std::array<std::pair<int64_t, int64_t>, 3> dims;
@@ -361,6 +392,7 @@ void check_pools(const at::Tensor& k, const at::Tensor& v, const PageBlocks& kb)
               "k_pages and v_pages must have the same shape and type");
   TORCH_CHECK(kb.layers <= 65535, "at most 65535 layers, got ", kb.layers);
   check_same_device(k, {&v});
+  check_pools_apart(k, v, true);
 }
 
 void copy_blocks(const at::Tensor& k, const at::Tensor& v, const PageBlocks& kb,

@@ -360,3 +360,47 @@ def test_more_work_than_a_launch_takes():
         paged.pages_fork(**book(table=i32(6, (1 << 20) + 1)), parents=i32(2), children=i32(2),
                          page_size=16)
     assert paged.paged_attention(**attend_args(table=i32(2, 1 << 26))).shape == (2, 32, 128)
+
+
+# ------------------------------------------------------------------ memory that two places share
+def test_keys_and_values_in_the_same_memory_are_not_written():
+    both = meta(2 * 9, 8, 16, 128)
+    with pytest.raises(RuntimeError, match="single memory location|share memory"):
+        paged.paged_write(**write_args(k_pages=both[:9], v_pages=both[:9]))
+    with pytest.raises(RuntimeError, match="single memory location|share memory"):
+        paged.paged_write(**write_args(k_pages=both[:9], v_pages=both[4:13]))
+    with pytest.raises(RuntimeError, match="single memory location|share memory"):
+        paged.pages_copy(both[:9], both[4:13], i32(2), i32(2))
+    assert paged.paged_write(**write_args(k_pages=both[:9], v_pages=both[9:])).shape == (5, 32, 128)
+    side = meta(9, 2, 8, 16, 128)
+    assert paged.paged_write(**write_args(k_pages=side[:, 0], v_pages=side[:, 1])).shape == (5, 32, 128)
+    assert paged.paged_attention(**attend_args(k_pages=both[:9], v_pages=both[4:13])).shape == \
+        (2, 32, 128)
+
+
+@pytest.mark.parametrize("strides", [(8 * 16 * 128 - 128, 16 * 128, 128, 1),       # pages meet
+                                     (8 * 16 * 128, 8 * 128, 128, 1),              # heads meet
+                                     (16 * 128, 16 * 128, 128, 1)])
+def test_pages_that_meet_are_not_written(strides):
+    k = torch.as_strided(meta(9 * 8 * 16 * 128), (9, 8, 16, 128), strides)
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged.paged_write(**write_args(k_pages=k))
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged.paged_write(**write_args(v_pages=k))
+    # a page of 17 rows to a head, tokens first, layers inside pages: nothing meets
+    for sizes, st in (((9, 8, 16, 128), (8 * 17 * 128, 17 * 128, 128, 1)),
+                      ((9, 8, 16, 128), (16 * 8 * 128, 128, 8 * 128, 1)),
+                      ((9, 8, 16, 128), (16 * 128, 9 * 16 * 128, 128, 1)),
+                      ((9, 1, 16, 128), (16 * 128, 3, 128, 1))):
+        k = torch.as_strided(meta(9 * 8 * 17 * 128), sizes, st)
+        a = write_args(k_pages=k, v_pages=meta(*sizes))
+        assert paged.paged_write(**a).shape == (5, 48 - 2 * sizes[1], 128)
+
+
+def test_layers_that_meet_are_not_copied():
+    page = 8 * 16 * 128
+    k = torch.as_strided(meta(18 * page), (2, 9, 8, 16, 128), (8 * page, page, 16 * 128, 128, 1))
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged.pages_copy(k, meta(2, 9, 8, 16, 128), i32(2), i32(2))
+    inside = meta(9, 2, 8, 16, 128).transpose(0, 1)
+    paged.pages_copy(inside, meta(2, 9, 8, 16, 128), i32(2), i32(2))
