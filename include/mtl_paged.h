@@ -59,9 +59,9 @@ typedef struct mtl_page_table {
  * step, moss_tts_lite/fast.py:149-162, over pages): for sequence b and query head h, with
  * kv head h / (n_heads / kv_heads),
  *   s_j = scale * k_scale * (q . k_j),  j in [0, lens[b]);  out = v_scale * sum softmax(s)_j v_j
- * fp32 softmax and sums; a weight enters the product with v to 2^-16 of itself (bf16) or to 2^-20 of
- * itself and 2^-39 of the largest (f16).  Lengths past width * page_size (at most 2^30) count as that, negative
- * ones as 0.
+ * fp32 softmax and sums; a weight enters the product with v to 2^-16 of itself (bf16) or to
+ * 2^-20 of itself and 2^-39 of the largest (f16).  Lengths past width * page_size (at most 2^30)
+ * count as that, negative ones as 0.
  *   q    [seqs, n_heads, head_dim] of q_type (bf16 or f16), rows ldq and heads ldh elements
  *        apart (multiples of 8, base 16-byte aligned)
  *   out  [seqs, n_heads, head_dim] of q_type, contiguous, 16-byte aligned; a sequence without

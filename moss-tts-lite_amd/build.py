@@ -1,7 +1,8 @@
 """Build recipe of ``libmtl_hip.so``: every ``csrc/*.hip`` compiled for gfx950.
 
-The library exposes only the plain C ABI declared in ``include/*.h`` (raw device pointers, sizes, a ``hipStream_t``), so it
-links against whichever HIP runtime the process already has loaded (torch's).
+The library exposes only the plain C ABI declared in ``include/*.h`` (raw device
+pointers, sizes, a ``hipStream_t``), so it links against whichever HIP runtime the
+process already has loaded (torch's).
 """
 from __future__ import annotations
 

@@ -30,7 +30,10 @@
 // first tile, which wait for one another; the join), the rest streams at 7 TB/s: 307 MB take 53
 // to 56 us in bf16 and 55 to 58 in e4m3, as one sequence or as 64 equal ones, in pages of 16, 64
 // or 256.  A short table (300 positions) takes 6 us, which is a launch and three trips to the
-// memory (length and page ids, tile, output).  The counters show no byte of the cache read twice.
+// memory (length and page ids, tile, output).  The counters show no byte of the cache read twice
+// with up to 16 query heads to a kv head.  Past that K and V are read for each 16 of them, by
+// workgroups that share no L2: 300 MB take 55 to 60 us with 32 heads over 2 (L2 misses 303 MB) and
+// 89 to 93 with 34 to 64 over 2 (602 MB).
 //
 // Tried and slower: 3 or 4 waves on each of a CU's four parts (their registers spill), the next
 // sequence's first tile loaded ahead (even), 6, 8 or 12 waves in 256 workgroups, shares in tiles
@@ -90,7 +93,7 @@ inline Split split_of(int n_heads, int kv_heads) {
 // every load of a tile can be issued without a condition (under a condition the compiler waits
 // for all loads in flight where its paths join).
 // K and V are read once: loads that leave no trace in the caches read 7.1 TB/s here, others 6.4.
-// With more than 16 query heads to a kv head its rows are read again, from the caches.
+// With more than 16 query heads to a kv head its rows are read again, and the loads leave a trace.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 
 __device__ __forceinline__ Rsrc rows_at(const char* base, int bytes) {

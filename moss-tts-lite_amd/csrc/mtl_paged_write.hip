@@ -157,7 +157,8 @@ extern "C" int mtl_paged_write(const void* qkv, int64_t ldq, int64_t rows,
   // Few rows: a workgroup for each 256 lanes' heads, so that a step's rows reach more CUs; many:
   // one for all heads of a row, which reads cos and sin once.  Rows of 48 heads of 128 split over
   // the heads and whole, in us: 16 rows 2.8 and 4.0, 512 rows 5.4 and 5.8, 1000 rows 8.4 and 8.3,
-  // 3300 rows 18.3 and 16.9.
+  // 3300 rows 18.3 and 16.9.  Where the rule changes sides, 512 rows split and 513 whole: 12 heads
+  // 3.2 and 3.3, 80 heads 6.9 and 7.7, 128 heads 9.2 and 11.3, 44 heads of 64 4.1 and 4.3.
   const int64_t passes = (heads * (pool->head_dim / 8) + 255) / 256;
   const dim3 grid((unsigned)rows, rows <= 512 ? (unsigned)passes : 1);
 #define MTL_RUN(T, KT, D)                                                                    \

@@ -104,7 +104,9 @@ __device__ __forceinline__ void move_page(const mtl_page_state& st, const Span& 
 // A lane an entry: checks, the pages each needs (prefix sum), then the lowest free pages in strips
 // of kStrip counts until there are enough (the next strip on its way meanwhile), then the writes.
 // Bound by the trips to the memory that wait for one another (entry, length, table, count; counts;
-// the writes): 5.2 us for 2 entries, 7.6 for 64.
+// the writes): 5.2 us for 2 entries, 7.6 for 64.  Entries that share a partly filled page count
+// their forerunners one by one: a call of 64 such entries takes 5 us longer, of 256 10, of 1024 35,
+// the copies included.
 __global__ void __launch_bounds__(kThreads) pages_extend_kernel(
     mtl_page_state st, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int n,
     int32_t* __restrict__ copy_src, int32_t* __restrict__ copy_dst, int32_t* __restrict__ copies,
@@ -271,8 +273,9 @@ __device__ __forceinline__ int moved(int p, int live, int64_t pages, const int32
 
 // Plans the moves: one pass over the counts for L, one that ranks movers and free pages below L by
 // prefix sums in strips of kStrip; with ALL it rewrites the table too.  Bound by the trips to the
-// memory one workgroup makes: 7 us for 900 pages, 48 for 70 000, 191 for 300 000, a small part of
-// what the copies of such a pool's pages take.
+// memory one workgroup makes: 7 us for 900 pages, 48 for 70 000, 191 for 300 000.  That is a small
+// part of what the copies take where a large part of such a pool moves, and the most of the call
+// where little does.
 template <bool ALL>
 __global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(
     const int32_t* refs, int64_t pages, int32_t* refs_out, int32_t* __restrict__ live_out,

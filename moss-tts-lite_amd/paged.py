@@ -91,9 +91,10 @@ def paged_write(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     ``cos``, ``sin``: ``[positions, head_dim]`` tables as ``model.rope_tables`` makes them, or
     the same in float32; without norm weights or tables that step is left out.  Computed in fp32
     and rounded once (the dense decoder's kernels round after every step, as the reference
-    does).  ``k_pages`` and ``v_pages`` share no memory.  A row with a negative position, or one past the tables, is padding: q 0, nothing
-    written.  No two rows may name the same position of one sequence, and a page that several
-    sequences hold is not to be written: :func:`pages_extend` copies it first."""
+    does).  A row with a negative position, or one past the tables, is padding: q 0, nothing
+    written.  No two rows may name the same position of one sequence, ``k_pages`` and ``v_pages``
+    share no memory, and a page that several sequences hold is not to be written:
+    :func:`pages_extend` copies it first."""
     return ops.overload("paged_write")(qkv, k_pages, v_pages, table, positions, seqs, q_norm,
                                        k_norm, cos, sin, eps, k_scale, v_scale)
 

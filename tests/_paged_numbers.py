@@ -1,5 +1,6 @@
 """Attention inputs whose outputs are known in closed form, and a check that allows nothing but the
-output's own rounding and float32 sums: for errors that an allowance for random inputs would hide."""
+output's own rounding and float32 sums: for errors that an allowance for random inputs would
+hide."""
 import torch
 
 from tests._paged import TYPES, table_for
@@ -43,7 +44,8 @@ def coded_case(lens, H, Hkv, D, page, typ, kv, code, c=2.0, seed=0, width=0):
         x = torch.zeros(n, D, dtype=torch.float64)
         x[:, 0] = (p % DIM0).double() / DIM0
         k.append(x)
-        v.append(torch.nn.functional.one_hot((p if code == "position" else p // 32) % D, D).double())
+        at = (p if code == "position" else p // 32) % D
+        v.append(torch.nn.functional.one_hot(at, D).double())
     kp, vp, table = spread_pages(k, v, lens, Hkv, page, kv, gen, width=width)
     q = heads_of(len(lens), H, D, typ)
     args = dict(q=q, k_pages=kp, v_pages=vp, table=table,
@@ -52,8 +54,8 @@ def coded_case(lens, H, Hkv, D, page, typ, kv, code, c=2.0, seed=0, width=0):
 
 
 def sink_case(lens, H, Hkv, D, page, typ, kv, c, seed=0, width=0):
-    """Position 0 scores c to 1.875 c above all others and has V = 0: the output is the others' share,
-    which is as small as their weight.  V is large, so that it is no subnormal number."""
+    """Position 0 scores c to 1.875 c above all others and has V = 0: the output is the others'
+    share, which is as small as their weight.  V is large, so that it is no subnormal number."""
     gen = torch.Generator().manual_seed(seed)
     k, v = [], []
     for n in lens:
@@ -89,9 +91,9 @@ def closed_form(q, k, v, c, weights=lambda w: w):
 
 def room(n, typ, drop=0.0):
     """The relative error of sum w v / sum w for V of one sign, n positions, the smallest weight
-    e^-drop of the largest.  Twice, for numerator and sum: sums of n terms in float32 (2^-24 a term),
-    exp2 and the score's own roundings (|s| 2^-22, |s| at most drop + 8).  Once: the weights' two
-    terms (bf16: 2^-8 of 2^-8; f16, cut: 2^-10 of 2^-10, and 2^-39 of the largest weight)."""
+    e^-drop of the largest.  Twice, for numerator and sum: sums of n terms in float32 (2^-24 a
+    term), exp2 and the score's own roundings (|s| 2^-22, |s| at most drop + 8).  Once: the weights'
+    two terms (bf16: 2^-8 of 2^-8; f16, cut: 2^-10 of 2^-10, and 2^-39 of the largest weight)."""
     terms = 2.0 ** -16 if typ == "bf16" else 2.0 ** -20 + 2.0 ** -39 * 2.718281828 ** drop
     return 2 * (n * 2.0 ** -24 + (drop + 8) * 2.0 ** -22 + 2.0 ** -22) + terms
 

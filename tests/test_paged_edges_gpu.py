@@ -38,13 +38,15 @@ class Guarded:
         self.lens.copy_(ints([lens(i) for i in range(seqs)], dev))
         self.plain = Pages(self.table, self.lens, self.refs, PAGE)
 
-    def refused(self, op, a, b):
+    def refused(self, op, a, b, why=2):
         """The call, by name; it must be refused, by the plain form too, and change nothing."""
-        assert getattr(self.plain, op)(a, b) == 2
+        plain = getattr(self.plain, op)(a, b)
+        assert (plain[0] if op == "extend" else plain) == why
         was = {k: v.clone() for k, v in self.all.items()}
         call = getattr(paged, "pages_" + op)
-        st = call(self.table, self.lens, self.refs, ints(a, self.dev), ints(b, self.dev), PAGE)
-        assert int(st) == 2
+        last = self.extend_pools if op == "extend" else (PAGE,)
+        st = call(self.table, self.lens, self.refs, ints(a, self.dev), ints(b, self.dev), *last)
+        assert int(st) == why
         for k, v in self.all.items():
             assert torch.equal(v, was[k]), (op, a[:4], b[:4], k)
 
@@ -87,13 +89,31 @@ def test_refused_calls_on_broken_lengths_change_nothing(dev, seqs, width):
     # lengths that no call leaves behind: negative, or past the table
     for bad in (-1, -1000, -2 ** 31, width * PAGE + 1, 2 ** 31 - 1):
         g = Guarded(dev, seqs, width, lambda i: bad if i == 2 else 0)
-        if bad > 0:                                               # the plain form knows no width here
+        if bad > 0:                                   # the plain form knows no width here
             g.plain.truncate = g.plain.fork = lambda a, b: 2
         else:
             g.plain.fork = lambda a, b: 2
         g.refused("truncate", [2, 1], [0, 0])
         g.refused("fork", [2, 2], [1, 0])
         g.refused("truncate", list(range(seqs)), [0] * seqs)
+
+
+@pytest.mark.parametrize("seqs,width", [(6, 4), (40, 70)])
+def test_refused_extends_change_nothing(dev, seqs, width):
+    g = Guarded(dev, seqs, width, lambda i: (7 * i + 5) % (width * PAGE))
+    k = torch.randn(1, g.refs.numel(), 1, PAGE, 64, device=dev).bfloat16()
+    was = k.clone()
+    g.extend_pools = k, k
+    many = list(range(seqs))
+    for c in (-1, -PAGE, -1000, -2 ** 31, 2 ** 31 - 1, width * PAGE + 1):
+        g.refused("extend", [1], [c])
+        g.refused("extend", many, [0] * (seqs - 1) + [c])
+    for s in (seqs, -1, 2 ** 31 - 1, -2 ** 31):
+        g.refused("extend", [s], [1])
+        g.refused("extend", many + [s], [0] * (seqs + 1))
+    g.refused("extend", many + [3], [0] * (seqs + 1))
+    g.refused("extend", [0], [PAGE], 1)                           # no page is free
+    assert torch.equal(k, was)
 
 
 def documented_step():

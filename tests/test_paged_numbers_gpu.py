@@ -87,8 +87,8 @@ def stored(x, scale):
     return (x.float() / scale).clamp(-448, 448).to(torch.float8_e4m3fn)
 
 
-SCALES = [1.0, 0.05, 3e-5, 2.0 ** -100, 1e-37, 2.0 ** -126, 5e-39, 2e-39, 1e-40, 2.0 ** -149, 0.0, 1e20,
-          2.0 ** 100, 1e37, 3e38, float("inf"), -0.3]
+SCALES = [1.0, 0.05, 3e-5, 2.0 ** -100, 1e-37, 2.0 ** -126, 5e-39, 2e-39, 1e-40, 2.0 ** -149, 0.0,
+          1e20, 2.0 ** 100, 1e37, 3e38, float("inf"), -0.3]
 
 
 @pytest.mark.parametrize("typ", ["bf16", "f16"])
@@ -100,10 +100,11 @@ def test_e4m3_values_are_divided_with_one_rounding(dev, typ):
     x = torch.randn(rows, heads, D, generator=gen) * 3
     x = x * torch.where(scale.isfinite() & (scale != 0), scale.abs(), 1.0)[None, :, None] * 30
     x = x.to(TYPES[typ])
-    x[0, :, :12] = torch.tensor([0.0, -0.0, 1.0, -1.0, float("inf"), float("-inf"), float("nan"), 1e-7,
-                                 6e4, 0.5, 2.0 ** -14, -2.0 ** -24]).to(TYPES[typ])
+    x[0, :, :12] = torch.tensor([0.0, -0.0, 1.0, -1.0, float("inf"), float("-inf"), float("nan"),
+                                 1e-7, 6e4, 0.5, 2.0 ** -14, -2.0 ** -24]).to(TYPES[typ])
     qkv = torch.cat([torch.zeros(rows, 1, D), x.float(), x.float().flip(0)], 1).to(TYPES[typ])
-    k, v = (torch.zeros(rows, heads, 16, D, dtype=torch.float8_e4m3fn, device=dev) for _ in range(2))
+    k, v = (torch.zeros(rows, heads, 16, D, dtype=torch.float8_e4m3fn, device=dev)
+            for _ in range(2))
     table = torch.arange(rows, dtype=torch.int32, device=dev)[:, None]
     paged.paged_write(qkv.reshape(rows, -1).to(dev), k, v, table,
                       torch.full((rows,), 5, device=dev), k_scale=scale.to(dev),
