@@ -1,5 +1,7 @@
 """Paged attention on the device against closed forms that allow nothing but the output's rounding
 and float32 sums: small weights beside a dominant one, and rows whose place shows in the output."""
+import math
+
 import pytest
 import torch
 
@@ -79,6 +81,18 @@ def test_every_row_of_a_long_sequence_is_in_its_place(dev):
     for code in ("position", "tile"):
         args, want = coded_case([60001, 300, 20000], 4, 1, 64, 64, "f16", "f16", code)
         check(args, want, "f16", 60001, 4.0, dev)
+
+
+@pytest.mark.parametrize("typ,kv,D", [("bf16", "bf16", 64), ("f16", "e4m3", 64)])
+def test_a_hundred_million_positions(dev, typ, kv, D):
+    # the same page all along: the softmax of one page, and its sum 2^19 times
+    page, width = 256, 1 << 19
+    args, want = coded_case([page], 2, 1, D, page, typ, kv, "position", c=4.0)
+    long = dict(args, table=args["table"][:, :1].expand(1, width).contiguous(),
+                lens=torch.tensor([page * width], dtype=torch.int32))
+    # 512 workgroups of 4 waves: a wave takes 2^11 tiles in turn, 8 positions of each to a lane, so
+    # the sums have 2^14 terms in turn and those of the join
+    check(long, (want[0], want[1] + math.log(width)), typ, 1 << 14, 8.0, dev)
 
 
 # ------------------------------------------------------------------------------ stored e4m3 values
