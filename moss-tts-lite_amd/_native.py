@@ -101,6 +101,9 @@ _SIGNATURES = {
                                  _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "mtl_pages_copy": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                               _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p]),
+    # mtl_rotary.h
+    "mtl_qk_rotary": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32,
+                             ctypes.c_float, ctypes.c_float, _i32, _c_void_p]),
     # tuning knobs (not part of the headers)
     "mtl_w4_gemm_splits": (_i32, [_i64, _i64]),
     "mtl_w4_gemm_partials": (_i32, [_c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _c_void_p,
@@ -209,6 +212,12 @@ class PageState(ctypes.Structure):
     """``mtl_page_state``: what the page bookkeeping works on."""
     _fields_ = [("table", _c_void_p), ("ld", _i64), ("width", _i64), ("seqs", _i64),
                 ("lens", _c_void_p), ("refs", _c_void_p), ("pages", _i64), ("page_size", _i32)]
+
+
+class RotaryHeads(ctypes.Structure):
+    """``mtl_rotary_heads``: the heads of q or of k, in and out."""
+    _fields_ = [("x", _c_void_p), ("x_row", _i64), ("x_head", _i64), ("out", _c_void_p),
+                ("out_row", _i64), ("out_head", _i64), ("norm", _c_void_p), ("heads", _i32)]
 
 
 class StripGeometry(ctypes.Structure):

@@ -7,39 +7,11 @@
 // the tensors' device.  A workspace belongs to one call, so calls on several streams and
 // graphs captured from them share nothing.  Meta kernels make the same checks and give the
 // output shapes to tracing.
-#include <ATen/ATen.h>
-#include <c10/core/Allocator.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/library.h>
-
-#include <algorithm>
-#include <array>
-#include <tuple>
-
-#include "mtl_gptq.h"
-#include "mtl_paged.h"
+#include "mtl_op_checks.h"
 
 namespace {
 
-using OptTensor = c10::optional<at::Tensor>;
-
-void check_status(int status, const char* what) {
-  TORCH_CHECK(status == 0, what, ": ", mtl_status_string(status), " (status ", status, ")");
-}
-
-int32_t row_type(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, "expected ", name,
-              " to be bfloat16 or float16, got ", t.scalar_type());
-  return t.scalar_type() == at::kBFloat16 ? MTL_T_BF16 : MTL_T_F16;
-}
-
-void check_same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> others) {
-  TORCH_CHECK(a.is_cuda() || a.is_meta(), "the paged cache runs on a HIP device");
-  for (const at::Tensor* t : others)
-    TORCH_CHECK(t->device() == a.device(), "all tensors must be on one HIP device, got ",
-                a.device(), " and ", t->device());
-}
+using namespace mtl_ops;
 
 void check_int32(const at::Tensor& t, int64_t dim, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim, name, " must be a ", dim,
@@ -48,21 +20,10 @@ void check_int32(const at::Tensor& t, int64_t dim, const char* name) {
               " must have unit last stride");
 }
 
-// A dimension's stride, 0 where the dimension has one element and torch's number means nothing.
-int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
-
 void check_page_size(int64_t ps) {
   TORCH_CHECK(ps == 16 || ps == 32 || ps == 64 || ps == 128 || ps == 256,
               "page_size must be 16, 32, 64, 128 or 256, got ", ps);
 }
-
-// The tensors' memory: null for meta tensors, which make the checks only.
-template <class T>
-T* ptr(const at::Tensor& t) {
-  return t.is_meta() ? nullptr : static_cast<T*>(t.data_ptr());
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 void check_scale(const OptTensor& s, const at::Tensor& pages, const char* name) {
   if (!s.has_value()) return;
@@ -71,24 +32,6 @@ void check_scale(const OptTensor& s, const at::Tensor& pages, const char* name) 
                   s->is_contiguous(),
               name, " must be contiguous float32 [", pages.size(1), "]");
   check_same_device(pages, {&*s});
-}
-
-// Pages that are written (at most 5 dimensions): no two of their elements may be the same memory.
-// Each stride has to pass over all that the smaller ones reach.
-void check_apart(const at::Tensor& t, const char* name) {
-  if (t.numel() == 0) return;
-  std::array<std::pair<int64_t, int64_t>, 5> dims;
-  int64_t n = 0;
-  for (int64_t d = 0; d < t.dim(); ++d)
-    if (t.size(d) > 1) dims[n++] = {t.stride(d), t.size(d)};
-  std::sort(dims.begin(), dims.begin() + n);
-  int64_t reach = 1;
-  for (int64_t i = 0; i < n; ++i) {
-    const auto& [stride, size] = dims[i];
-    TORCH_CHECK(stride >= reach, name, "'s pages overlap, several elements are a single memory "
-                "location: ", t.sizes(), " with strides ", t.strides());
-    reach += (size - 1) * stride;
-  }
 }
 
 // Keys and values that are written, of one type: dense blocks of one storage must not meet.  Where
@@ -161,20 +104,6 @@ mtl_page_table table_of(const at::Tensor& table) {
   TORCH_CHECK(t.seqs <= 1 || table.stride(0) >= t.width, "table rows must not overlap");
   return t;
 }
-
-hipStream_t stream_of(const at::Tensor& t) {
-  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-// Memory of a call's own from torch's caching allocator, without a tensor around it.
-struct Workspace {
-  c10::DataPtr data;
-  int64_t bytes;
-  Workspace(const at::Tensor& like, int64_t n)
-      : data(n > 0 ? c10::GetAllocator(like.device().type())->allocate(n) : c10::DataPtr()),
-        bytes(n) {}
-  void* get() const { return data.get(); }
-};
 
 // out, and where lse is not null the log-sum-exp
 at::Tensor attend(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
