@@ -104,6 +104,10 @@ _SIGNATURES = {
     # mtl_rotary.h
     "mtl_qk_rotary": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32,
                              ctypes.c_float, ctypes.c_float, _i32, _c_void_p]),
+    # mtl_sample.h
+    "mtl_sample_workspace_bytes": (_i64, [_i64, _i64, _i32, _c_void_p]),
+    "mtl_sample": (_i32, [_c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p,
+                          _c_void_p, _c_void_p, _i64, _c_void_p]),
     # tuning knobs (not part of the headers)
     "mtl_w4_gemm_splits": (_i32, [_i64, _i64]),
     "mtl_w4_gemm_partials": (_i32, [_c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _c_void_p,
@@ -220,6 +224,13 @@ class RotaryHeads(ctypes.Structure):
                 ("out_row", _i64), ("out_head", _i64), ("norm", _c_void_p), ("heads", _i32)]
 
 
+class SampleSettings(ctypes.Structure):
+    """``mtl_sample_settings``: how the rows draw."""
+    _fields_ = [("temperature", _c_void_p), ("top_k", _c_void_p), ("top_p", _c_void_p),
+                ("min_p", _c_void_p), ("temperature_all", ctypes.c_float), ("top_k_all", _i32),
+                ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float)]
+
+
 class StripGeometry(ctypes.Structure):
     """``mtl_strip_geometry``: the strip GEMV's launch shape (0 = automatic per field)."""
     _fields_ = [("strips_per_wg", ctypes.c_int32), ("blocks_per_wave", ctypes.c_int32),
@@ -246,7 +257,7 @@ LAYOUT_ROWS, LAYOUT_TILED, LAYOUT_STRIP, LAYOUT_STRIP_QSZ = 0, 1, 2, 3
 XPART_HALVES = 1 << 30                # MTL_XPART_HALVES, OR'ed into mtl_w4_gemm_residual's xsplits
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL = 0, 1, 2
 META_GPTQ, META_QSZ = 0, 1
-T_BF16, T_F16, T_E4M3 = 0, 1, 2
+T_BF16, T_F16, T_E4M3, T_F32 = 0, 1, 2, 3
 
 _lib = None
 

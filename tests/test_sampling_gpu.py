@@ -1,0 +1,222 @@
+"""The draw of tokens on the device against its definition in float64."""
+import math
+
+import pytest
+import torch
+
+from moss_tts_lite_amd import sampling
+from tests._sampling import reference
+
+pytestmark = pytest.mark.gpu
+
+# Two float64 evaluations of a border differ by some 2^-48 of the whole: sums of up to 2^20 weights,
+# weights in whole units of 2^-42 with random roundings.  A draw nearer than this to a border may go
+# either way; the seeds here have none that near, which `check` makes sure of.
+NEAR = 2.0 ** -30
+
+
+def logits_of(gen, rows, vocab, typ, spread=2.0, peaks=20):
+    x = spread * torch.randn(rows, vocab, generator=gen)
+    for r in range(rows):
+        at = torch.randperm(vocab, generator=gen)[:min(peaks, vocab)]
+        x[r, at] += 6 + torch.randn(len(at), generator=gen)
+    return x.to(typ)
+
+
+def check(dev, logits, u, **kw):
+    token, logprob = sampling.sample(logits.to(dev), u.to(dev), return_logprob=True, **{
+        k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in kw.items()})
+    assert token.dtype == torch.int64 and logprob.dtype == torch.float32
+    ref = reference(logits, u, **kw)
+    for r, (tok, lp, near) in enumerate(ref):
+        assert near > NEAR, (r, near)
+        assert int(token[r]) == tok, (r, int(token[r]), ref[r])
+        if math.isinf(lp):
+            assert float(logprob[r]) == lp
+        else:                              # one rounding, and that of the largest logits' distance
+            assert abs(float(logprob[r]) - lp) <= 2 ** -23 * abs(lp) + 1e-9, (r, lp)
+    return token
+
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+SETTINGS = [dict(), dict(top_k=1), dict(top_k=5), dict(top_p=0.8), dict(min_p=0.05),
+            dict(top_k=40, top_p=0.9), dict(top_k=300), dict(top_k=50, min_p=0.02),
+            dict(top_k=700, top_p=0.95, min_p=0.001), dict(top_p=0.999), dict(temperature=0.0),
+            dict(temperature=1.7, top_p=0.6), dict(temperature=0.05), dict(top_p=0.0),
+            dict(min_p=1.5), dict(min_p=1.0), dict(temperature=40.0, top_p=0.99, top_k=2000)]
+
+
+@pytest.mark.parametrize("kw", SETTINGS, ids=str)
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 1025, 8193, 40001])
+def test_settings(dev, vocab, typ, kw):
+    gen = torch.Generator().manual_seed(vocab)
+    check(dev, logits_of(gen, 4, vocab, typ), torch.rand(4, generator=gen), **kw)
+
+
+@pytest.mark.parametrize("vocab", [32767, 32768, 32769, 151936, 262145, 1 << 20])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=50, temperature=1.5), dict(top_p=0.95),
+                                dict(min_p=0.0001), dict(top_k=5000, top_p=0.9)], ids=str)
+def test_large_vocabularies(dev, vocab, kw):
+    gen = torch.Generator().manual_seed(vocab + 1)
+    typ = TYPES[vocab % 3]
+    check(dev, logits_of(gen, 2, vocab, typ), torch.rand(2, generator=gen), **kw)
+
+
+@pytest.mark.parametrize("vocab", [600, 33000])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=7), dict(top_k=400), dict(top_p=0.5),
+                                dict(top_p=0.25, top_k=600), dict(min_p=0.5)], ids=str)
+def test_equal_logits(dev, vocab, kw):
+    # the order goes by index, and borders are met exactly: whole numbers of equal weights
+    for value in (0.0, -3.5, 1e4):
+        x = torch.full((3, vocab), value, dtype=torch.float16)
+        x[1, ::2] = -0.0 if value == 0 else value    # -0 is 0
+        x[2, : vocab // 2] = float("-inf")
+        u = torch.tensor([0.0, 0.499, 0.9999])
+        for r in range(3):
+            live = [i for i in range(vocab) if x[r, i] != float("-inf")]
+            n = min(kw.get("top_k", 0) or len(live), len(live))
+            p = kw.get("top_p", 1.0)
+            if p < 1:                                # tokens j with j <= p n
+                n = min(n, int(math.floor(p * n)) + 1)
+            want = live[min(int(float(u[r]) * n), n - 1)]
+            tok = sampling.sample(x[r:r + 1].to(dev), u[r:r + 1].to(dev), **kw)
+            assert int(tok) == want, (value, r)
+
+
+def test_two_levels_of_many_ties(dev):
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randint(0, 3, (6, 5000), generator=gen).float() * 2
+    for typ in TYPES:
+        for kw in (dict(top_k=1000), dict(top_k=3000), dict(top_p=0.3), dict(top_p=0.93),
+                   dict(min_p=0.1), dict(min_p=0.2), dict(top_k=2500, top_p=0.7)):
+            check(dev, x.to(typ), torch.rand(6, generator=gen), **kw)
+
+
+def test_masked_rows(dev):
+    inf = float("inf")
+    gen = torch.Generator().manual_seed(8)
+    x = logits_of(gen, 9, 3000, torch.float32)
+    x[0] = -inf                                      # nothing is left
+    x[1] = float("nan")
+    x[2, 1:] = -inf                                  # one token
+    x[3, :2999] = -inf
+    x[4, ::2] = float("nan")
+    x[5, 5:2990] = -inf                              # fewer than top_k
+    x[6, [17, 40]] = inf                             # infinities share
+    x[7] = torch.finfo(torch.float32).min            # the type's lowest value is a number
+    x[8, 100:] = torch.finfo(torch.float32).min
+    u = torch.rand(9, generator=gen)
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9), dict(min_p=0.1), dict(temperature=0.0),
+               dict(top_k=50, top_p=0.51, min_p=0.01), dict(top_k=2000)):
+        tok = check(dev, x, u, **kw)
+        assert tok[:4].tolist() == [-1, -1, 0, 2999]
+        assert int(tok[4]) % 2 == 1 and int(tok[6]) in (17, 40)
+
+
+def test_a_setting_for_each_row(dev):
+    gen = torch.Generator().manual_seed(2)
+    rows = 24
+    x = logits_of(gen, rows, 12000, torch.bfloat16)
+    pick = lambda *z: torch.tensor([z[int(i)] for i in torch.randint(0, len(z), (rows,),
+                                                                    generator=gen)])
+    kw = dict(temperature=pick(0.0, 0.7, 1.0, 1.5, -1.0), top_k=pick(0, 1, 20, 500, 20000, -3).int(),
+              top_p=pick(1.0, 0.9, 0.3, 2.0), min_p=pick(0.0, 0.01, 0.2))
+    u = torch.rand(rows, generator=gen)
+    a = check(dev, x, u, **kw)
+    for r in range(rows):                            # a row draws the same by itself, by numbers
+        one = sampling.sample(x[r:r + 1].to(dev), u[r:r + 1].to(dev),
+                              *(float(kw[n][r]) if n != "top_k" else int(kw[n][r])
+                                for n in ("temperature", "top_k", "top_p", "min_p")))
+        assert int(one) == int(a[r])
+
+
+def test_random_numbers_at_the_ends(dev):
+    gen = torch.Generator().manual_seed(4)
+    x = logits_of(gen, 1, 2000, torch.float32).expand(6, 2000)
+    u = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, 2.0, -1.0, float("nan")])
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9)):
+        ref = reference(x[:2], torch.tensor([0.0, 1 - 2.0 ** -24]), **kw)
+        got = sampling.sample(x.to(dev), u.to(dev), **kw).tolist()
+        assert got == [ref[0][0], ref[1][0], ref[1][0], ref[1][0], ref[0][0], ref[0][0]]
+
+
+def test_extreme_temperatures(dev):
+    gen = torch.Generator().manual_seed(6)
+    x = logits_of(gen, 3, 5000, torch.float32)
+    u = torch.rand(3, generator=gen)
+    for t in (1e-30, 1e-3, 1e30):
+        for kw in (dict(), dict(top_k=40), dict(top_p=0.49)):
+            check(dev, x, u, temperature=t, **kw)
+    inf = sampling.sample(x.to(dev), u.to(dev), torch.full((3,), float("inf"), device=dev))
+    assert ((inf >= 0) & (inf < 5000)).all()
+    nan = sampling.sample(x.to(dev), u.to(dev), torch.full((3,), float("nan"), device=dev))
+    assert torch.equal(nan.cpu(), x.argmax(-1))
+
+
+def test_every_token_is_drawn_as_often_as_it_should(dev):
+    # by index the draw is exact: u on a grid finds each token for its share of the grid
+    x = torch.tensor([[0.0, 1.0, -1.0, 2.0, 0.5, float("-inf")]])
+    n = 60000
+    u = (torch.arange(n).double() / n).float()
+    tok = sampling.sample(x.to(dev).expand(n, 6), u.to(dev), 0.8, top_k=4)
+    w = torch.exp(x[0].double() / 0.8)
+    w[[2, 5]] = 0
+    share = torch.bincount(tok.cpu(), minlength=6).double() / n
+    assert ((share - w / w.sum()).abs() <= 2.0 / n).all()
+
+
+def test_views(dev):
+    gen = torch.Generator().manual_seed(7)
+    x = logits_of(gen, 5, 4001, torch.bfloat16)
+    u = torch.rand(5, generator=gen).to(dev)
+    want = sampling.sample(x.to(dev), u, top_k=30)
+    wide = torch.empty(5, 4010, dtype=torch.bfloat16, device=dev)
+    wide[:, 3:4004] = x.to(dev)
+    assert torch.equal(sampling.sample(wide[:, 3:4004], u, top_k=30), want)
+    assert torch.equal(sampling.sample(x.to(dev).t().contiguous().t(), u, top_k=30), want)
+    assert torch.equal(sampling.sample(x.to(dev).flip(0), u.flip(0), top_k=30), want.flip(0))
+    assert sampling.sample(x[:0].to(dev), u[:0]).shape == (0,)
+
+
+def test_past_32_bit_offsets(dev):
+    rows, vocab = 4200, 1 << 19                      # 2.2e9 logits
+    x = torch.full((rows, vocab), -20.0, dtype=torch.bfloat16, device=dev)
+    x[:, 3] = 5.0
+    x[rows - 1, 3], x[rows - 1, vocab - 1] = -20.0, 5.0
+    tok = sampling.sample(x, torch.full((rows,), 0.5, device=dev), top_k=20)
+    assert (tok[:-1] == 3).all() and int(tok[-1]) == vocab - 1
+
+
+def test_repeats_captures_and_streams(dev):
+    gen = torch.Generator().manual_seed(9)
+    x = logits_of(gen, 20, 50000, torch.bfloat16).to(dev)
+    u = torch.rand(20, generator=gen).to(dev)
+    t = torch.linspace(0.2, 2, 20).to(dev)
+    for kw in (dict(top_k=50), dict(top_p=0.97), dict()):
+        want = sampling.sample(x, u, t, return_logprob=True, **kw)
+        graphs = []
+        torch.cuda.synchronize()
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                got = sampling.sample(x, u, t, return_logprob=True, **kw)
+            graphs.append((g, got, torch.cuda.Stream()))
+        for _ in range(3):
+            for g, got, s in graphs:
+                with torch.cuda.stream(s):
+                    got[0].fill_(-5)
+                    g.replay()
+            again = sampling.sample(x, u, t, return_logprob=True, **kw)
+            torch.cuda.synchronize()
+            for a in (again, *(got for _, got, _ in graphs)):
+                assert torch.equal(a[0], want[0]) and torch.equal(a[1], want[1])
+
+
+def test_schemas(dev):
+    from moss_tts_lite_amd import ops
+
+    x, u = torch.randn(3, 100, device=dev), torch.rand(3, device=dev)
+    for name in ("sample", "sample_logprob"):
+        torch.library.opcheck(ops.overload(name), (x, u, None, None, u, None, 0.7, 5),
+                              test_utils=("test_schema", "test_faketensor"))
