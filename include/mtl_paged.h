@@ -84,6 +84,33 @@ int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh, const mtl_page_
                         int64_t ws_bytes, void* stream);
 
 /*
+ * mtl_paged_attention for sequences that share a prefix: sequences groups[g] .. groups[g + 1] - 1
+ * are a group, whose first shared[g] positions lie in the same pages or hold the same K and V
+ * (copies of a partly filled page), and are read once for all of its queries, through the table
+ * row of its first sequence that reaches them all (or, where none does, of its longest).  The
+ * result is that of mtl_paged_attention, with sums in another order.
+ *   groups   int32 [n_groups + 1] (device), ascending from 0 to seqs; a sequence outside of them
+ *            is attended by itself
+ *   shared   int32 [n_groups] (device), counted in whole multiples of 16; past a sequence's own
+ *            length nothing counts for it, negative ones count as 0.  A group of one sequence
+ *            shares nothing
+ *   workspace  mtl_paged_attention_shared_workspace_bytes(...) bytes, 16-byte aligned, any
+ *            content, one launch at a time
+ * Limits: seqs, n_groups and n_heads at most 65535, seqs * n_heads at most 2^26 - 1, and with w =
+ * n_heads / kv_heads columns a sequence, (seqs (w / 16 + 2) + n_groups) * (width * page_size / 128
+ * + 2) below 2^27.  K and V that any sequence of a group attends to are finite (an infinity or NaN
+ * there may give NaN in all of the group).
+ */
+int64_t mtl_paged_attention_shared_workspace_bytes(int64_t seqs, int64_t n_groups, int32_t n_heads,
+                                                   int32_t kv_heads, int32_t head_dim,
+                                                   int64_t width, int32_t page_size);
+int mtl_paged_attention_shared(const void* q, int64_t ldq, int64_t ldh, const mtl_page_pool* pool,
+                               const mtl_page_table* table, const int32_t* lens,
+                               const int32_t* groups, const int32_t* shared, int64_t n_groups,
+                               int32_t n_heads, int32_t q_type, float scale, void* out, float* lse,
+                               void* workspace, int64_t ws_bytes, void* stream);
+
+/*
  * q/k RMSNorm, RoPE and the page write of new tokens, each row at its own position of its own
  * sequence (mtl_qk_norm_rope_kv_rows over pages; moss_tts_lite/fast.py:226-237).
  *   qkv        [rows, ldq] of type (bf16 or f16), each row q | k | v

@@ -87,6 +87,11 @@ _SIGNATURES = {
     "mtl_paged_attention": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32,
                                    _i32, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p, _i64,
                                    _c_void_p]),
+    "mtl_paged_attention_shared_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i64,
+                                                          _i32]),
+    "mtl_paged_attention_shared": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
+                                          _c_void_p, _c_void_p, _i64, _i32, _i32, ctypes.c_float,
+                                          _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "mtl_paged_write": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64,
                                ctypes.c_float, _i32, _i32, _c_void_p, _c_void_p]),

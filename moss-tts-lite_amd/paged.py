@@ -77,6 +77,26 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return op(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale)
 
 
+def paged_attention_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                           table: torch.Tensor, lens: torch.Tensor, groups: torch.Tensor,
+                           shared: torch.Tensor, scale: float,
+                           k_scale: torch.Tensor | None = None,
+                           v_scale: torch.Tensor | None = None, return_lse: bool = False):
+    """:func:`paged_attention` for sequences that share a prefix, read once for all of them
+    (``mtl_paged_attention_shared``): forks of one sequence, requests on one prompt.
+
+    Sequences ``groups[g]`` to ``groups[g + 1] - 1`` (int32 ``[n + 1]``, ascending from 0 to the
+    number of sequences) are a group, and its first ``shared[g]`` positions (int32 ``[n]``) lie in
+    the same pages for all of them, or in copies of these: a page that :func:`pages_extend` copied
+    holds the same K and V up to where the fork was made.  They are read through the table row of
+    the group's first sequence that reaches them all.  Shorter and empty sequences of a group
+    attend to what their length holds.  Results are those of :func:`paged_attention`, with sums in
+    another order, and the same call gives the same bits.  K and V that any sequence of a group
+    attends to are finite (an infinity or NaN there may give NaN in all of the group)."""
+    op = ops.overload("paged_attention_shared_lse" if return_lse else "paged_attention_shared")
+    return op(q, k_pages, v_pages, table, lens, groups, shared, scale, k_scale, v_scale)
+
+
 def paged_write(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                 table: torch.Tensor, positions: torch.Tensor, seqs: torch.Tensor | None = None,
                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,

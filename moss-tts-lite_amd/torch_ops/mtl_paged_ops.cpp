@@ -1,6 +1,7 @@
 // torch dispatcher operators of the paged key-value cache over the C ABI in mtl_paged.h:
-// mtl::paged_attention(_lse), mtl::paged_write, mtl::pages_extend, mtl::pages_fork,
-// mtl::pages_truncate, mtl::pages_compact and mtl::pages_copy.
+// mtl::paged_attention(_lse), mtl::paged_attention_shared(_lse), mtl::paged_write,
+// mtl::pages_extend, mtl::pages_fork, mtl::pages_truncate, mtl::pages_compact and
+// mtl::pages_copy.
 //
 // Host code only, as mtl_torch_ops.cpp: each operator checks its tensors, takes outputs and
 // workspaces from torch's caching allocator and calls the C entry on torch's current stream of
@@ -105,10 +106,17 @@ mtl_page_table table_of(const at::Tensor& table) {
   return t;
 }
 
+// Which sequences share a prefix, and how much of it.
+struct Groups {
+  const at::Tensor& starts;
+  const at::Tensor& shared;
+};
+
 // out, and where lse is not null the log-sum-exp
 at::Tensor attend(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
                   const at::Tensor& table, const at::Tensor& lens, double scale,
-                  const OptTensor& k_scale, const OptTensor& v_scale, at::Tensor* lse) {
+                  const OptTensor& k_scale, const OptTensor& v_scale, at::Tensor* lse,
+                  const Groups* groups = nullptr) {
   TORCH_CHECK(q.dim() == 3, "q must be [sequences, heads, head_dim], got ", q.sizes());
   const int32_t type = row_type(q, "q");
   const mtl_page_pool pool = pool_of(k_pages, v_pages, k_scale, v_scale, type);
@@ -126,6 +134,21 @@ at::Tensor attend(const at::Tensor& q, const at::Tensor& k_pages, const at::Tens
               pool.page_size);
   TORCH_CHECK(tab.seqs == b && lens.size(0) == b, "q, table and lens must have the same number of "
               "sequences, got ", b, ", ", tab.seqs, " and ", lens.size(0));
+  int64_t n_groups = 0;
+  if (groups) {
+    check_int32(groups->starts, 1, "groups");
+    check_int32(groups->shared, 1, "shared");
+    check_same_device(q, {&groups->starts, &groups->shared});
+    n_groups = groups->shared.size(0);
+    TORCH_CHECK(groups->starts.size(0) == n_groups + 1, "groups must be int32 [", n_groups + 1,
+                "], one more than shared, got ", groups->starts.sizes());
+    TORCH_CHECK(n_groups <= 65535, "at most 65535 groups, got ", n_groups);
+    const int64_t columns = (h / pool.kv_heads + 15) / 16 + 2;
+    TORCH_CHECK(b * h < (1 << 26) && (b * columns + n_groups) *
+                        (tab.width * pool.page_size / 128 + 2) < (1 << 27),
+                "too many sequences, groups or pages for one call: q ", q.sizes(), ", table ",
+                table.sizes());
+  }
   at::Tensor out = at::empty({b, h, q.size(2)}, q.options());
   if (lse) *lse = at::empty({b, h}, q.options().dtype(at::kFloat));
   if (q.is_meta() || b == 0) return out;
@@ -135,6 +158,18 @@ at::Tensor attend(const at::Tensor& q, const at::Tensor& k_pages, const at::Tens
   if (q.stride(2) != 1 || step(q, 0) % 8 || step(q, 1) % 8 || !aligned16(q.data_ptr())) {
     q2 = q.contiguous();
     if (!aligned16(q2.data_ptr())) q2 = q2.clone();
+  }
+  if (groups) {
+    const Workspace ws(q, mtl_paged_attention_shared_workspace_bytes(
+                              b, n_groups, (int32_t)h, pool.kv_heads, pool.head_dim, tab.width,
+                              pool.page_size));
+    check_status(mtl_paged_attention_shared(
+                     q2.data_ptr(), step(q2, 0), step(q2, 1), &pool, &tab, ptr<int32_t>(lens),
+                     ptr<int32_t>(groups->starts), ptr<int32_t>(groups->shared), n_groups,
+                     (int32_t)h, type, (float)scale, out.data_ptr(),
+                     lse ? ptr<float>(*lse) : nullptr, ws.get(), ws.bytes, stream_of(q)),
+                 "mtl_paged_attention_shared");
+    return out;
   }
   const Workspace ws(q, mtl_paged_attention_workspace_bytes(
                             b, (int32_t)h, pool.kv_heads, pool.head_dim, tab.width,
@@ -160,6 +195,25 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_lse(
     const OptTensor& v_scale) {
   at::Tensor lse;
   at::Tensor out = attend(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale, &lse);
+  return {out, lse};
+}
+
+at::Tensor paged_attention_shared(const at::Tensor& q, const at::Tensor& k_pages,
+                                  const at::Tensor& v_pages, const at::Tensor& table,
+                                  const at::Tensor& lens, const at::Tensor& groups,
+                                  const at::Tensor& shared, double scale, const OptTensor& k_scale,
+                                  const OptTensor& v_scale) {
+  const Groups g{groups, shared};
+  return attend(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale, nullptr, &g);
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention_shared_lse(
+    const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+    const at::Tensor& table, const at::Tensor& lens, const at::Tensor& groups,
+    const at::Tensor& shared, double scale, const OptTensor& k_scale, const OptTensor& v_scale) {
+  const Groups g{groups, shared};
+  at::Tensor lse;
+  at::Tensor out = attend(q, k_pages, v_pages, table, lens, scale, k_scale, v_scale, &lse, &g);
   return {out, lse};
 }
 
@@ -434,6 +488,12 @@ TORCH_LIBRARY_FRAGMENT(mtl, m) {
   m.def("paged_attention_lse(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, "
         "Tensor lens, float scale, Tensor? k_scale=None, Tensor? v_scale=None) "
         "-> (Tensor, Tensor)");
+  m.def("paged_attention_shared(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, "
+        "Tensor lens, Tensor groups, Tensor shared, float scale, Tensor? k_scale=None, "
+        "Tensor? v_scale=None) -> Tensor");
+  m.def("paged_attention_shared_lse(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, "
+        "Tensor lens, Tensor groups, Tensor shared, float scale, Tensor? k_scale=None, "
+        "Tensor? v_scale=None) -> (Tensor, Tensor)");
   m.def("paged_write(Tensor qkv, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, "
         "Tensor positions, Tensor? seqs=None, Tensor? q_norm=None, Tensor? k_norm=None, "
         "Tensor? cos=None, Tensor? sin=None, float eps=1e-6, Tensor? k_scale=None, "
@@ -452,6 +512,8 @@ TORCH_LIBRARY_FRAGMENT(mtl, m) {
 #define MTL_PAGED_IMPLS(m)                   \
   m.impl("paged_attention", &paged_attention); \
   m.impl("paged_attention_lse", &paged_attention_lse); \
+  m.impl("paged_attention_shared", &paged_attention_shared); \
+  m.impl("paged_attention_shared_lse", &paged_attention_shared_lse); \
   m.impl("paged_write", &paged_write);         \
   m.impl("pages_extend", &pages_extend);       \
   m.impl("pages_fork", &pages_fork);           \
