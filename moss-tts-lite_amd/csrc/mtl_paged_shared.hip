@@ -23,11 +23,19 @@ namespace mtl {
 
 constexpr int kSharedWaves = 4;
 constexpr int kSharedBlock = kTile * kSharedWaves;
-constexpr int kStash = 1024;            // sequences whose lengths a workgroup keeps in LDS
+constexpr int kStage = 64;              // positions of a tile in LDS
+constexpr int kSharedWorkgroups = 512;  // 2 on each of 256 CUs: all their registers' room
+constexpr int kStash = 512;             // sequences and groups that a workgroup keeps in LDS
+constexpr int kNarrow = 32;             // columns up to which waves take positions, not columns
+constexpr int kWide = 64;               // columns of an item, at most
 
-// What a block costs, by its sets of 16 columns.
-__host__ __device__ constexpr int block_cost(int sets) {
-  return sets <= 1 ? 4 : sets <= 2 ? 6 : 10;
+// What a block of an item costs by its columns, and an item by itself.
+__host__ __device__ constexpr int block_cost(int columns) {
+  return columns <= 16 ? 3 : columns <= kNarrow ? 4 : 8;
+}
+constexpr int kItemCost = 12;
+__host__ __device__ constexpr int item_cost(int columns, int blocks) {
+  return blocks ? kItemCost + blocks * block_cost(columns) : 0;
 }
 
 struct SharedCall {
@@ -55,92 +63,132 @@ struct Group {
   int begin, end, shared;               // shared: 0 where nothing is attended together
 };
 
-__device__ __forceinline__ Group group_at(const SharedCall& a, int i) {
-  Group g;
-  g.begin = min(max(a.groups[i], 0), a.seqs);
-  g.end = min(max(a.groups[i + 1], g.begin), a.seqs);
-  g.shared = g.end - g.begin > 1 ? clamp_len(a.shared[i], a.cap) & ~15 : 0;
-  return g;
-}
+// Lengths and groups: in LDS where there is room, since everything that is decided from them waits
+// for one entry after the other.
+struct Lists {
+  int lens[kStash], groups[kStash + 1], shared[kStash];
+  int2 own[kStash];                     // a sequence's own positions [x, y)
+};
 
-// The group of a sequence: -1 for none.
-__device__ __forceinline__ int group_of(const SharedCall& a, int seq, Group& g) {
-  int lo = 0, hi = a.n_groups;          // groups below lo begin at or before seq
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.groups[mid] <= seq) lo = mid + 1;
-    else hi = mid;
+struct Batch {
+  const SharedCall& a;
+  Lists& l;
+  bool near;
+
+  __device__ __forceinline__ Batch(const SharedCall& a, Lists& l)
+      : a(a), l(l), near(a.seqs <= kStash && a.n_groups <= kStash) {
+    if (!near) return;
+    for (int i = threadIdx.x; i < max(a.seqs, a.n_groups + 1); i += kSharedWaves * 64) {
+      if (i < a.seqs) l.lens[i] = clamp_len(a.lens[i], a.cap);
+      if (i <= a.n_groups) l.groups[i] = a.groups[i];
+      if (i < a.n_groups) l.shared[i] = a.shared[i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.seqs; i += kSharedWaves * 64) l.own[i] = find_own(i);
+    __syncthreads();
   }
-  g = Group{seq, seq + 1, 0};
-  if (lo == 0) return -1;
-  const Group x = group_at(a, lo - 1);
-  if (seq < x.begin || seq >= x.end) return -1;
-  g = x;
-  return lo - 1;
-}
+
+  __device__ __forceinline__ int len(int s) const {
+    return near ? l.lens[s] : clamp_len(a.lens[s], a.cap);
+  }
+  __device__ __forceinline__ int start(int i) const { return near ? l.groups[i] : a.groups[i]; }
+
+  __device__ __forceinline__ Group group(int i) const {
+    Group g;
+    g.begin = min(max(start(i), 0), a.seqs);
+    g.end = min(max(start(i + 1), g.begin), a.seqs);
+    g.shared = g.end - g.begin > 1 ? clamp_len(near ? l.shared[i] : a.shared[i], a.cap) & ~15 : 0;
+    return g;
+  }
+
+  // The group of a sequence: -1 for none.
+  __device__ __forceinline__ int group_of(int seq, Group& g) const {
+    int lo = 0, hi = a.n_groups;        // groups below lo begin at or before seq
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (start(mid) <= seq) lo = mid + 1;
+      else hi = mid;
+    }
+    g = Group{seq, seq + 1, 0};
+    if (lo == 0) return -1;
+    const Group x = group(lo - 1);
+    if (seq < x.begin || seq >= x.end) return -1;
+    g = x;
+    return lo - 1;
+  }
+
+  __device__ __forceinline__ int2 find_own(int seq) const {
+    Group g;
+    group_of(seq, g);
+    const int n = len(seq);
+    return make_int2(min(g.shared, n), n);
+  }
+  __device__ __forceinline__ int2 own_of(int seq) const {
+    return near ? l.own[seq] : find_own(seq);
+  }
+};
 
 __device__ __forceinline__ int blocks_in(int positions) {
   return (positions + kSharedBlock - 1) / kSharedBlock;
 }
 
-// The cost of `columns` columns over `blocks` blocks.
+// The cost of `columns` columns over `blocks` blocks, WIDE columns an item.
 template <int WIDE>
 __device__ __forceinline__ int cost_of(int columns, int blocks) {
-  const int rest = columns % WIDE;
-  return blocks * (columns / WIDE * block_cost(WIDE / 16) +
-                   (rest ? block_cost((rest + 15) / 16) : 0));
+  return columns / WIDE * item_cost(WIDE, blocks) +
+         (columns % WIDE ? item_cost(columns % WIDE, blocks) : 0);
 }
 
 // Where the items lie in the row, as every wave finds it: a lane adds up a run of groups and a run
 // of sequences.
 template <int WIDE>
 struct Row {
-  int per_group, per_seq, groups_upto, seqs_upto, shared_cost, total, pieces;
+  int per_group, per_seq, groups_upto, seqs_upto, shared_cost, total, pieces, each, longer;
 
-  __device__ __forceinline__ Row(const SharedCall& a, int2* stash) {
+  __device__ __forceinline__ Row(const SharedCall& a, const Batch& batch) {
     const int lane = threadIdx.x & 63;
     per_group = (a.n_groups + 63) / 64;
     per_seq = (a.seqs + 63) / 64;
-    int cost = 0;
+    int cost = 0, widest = min(a.per_kv, WIDE);
     for (int i = 0; i < per_group; ++i) {
       const int64_t at = (int64_t)lane * per_group + i;
       if (at >= a.n_groups) break;
-      const Group g = group_at(a, (int)at);
-      cost += cost_of<WIDE>((g.end - g.begin) * a.per_kv, blocks_in(g.shared));
+      const Group g = batch.group((int)at);
+      const int columns = (g.end - g.begin) * a.per_kv;
+      cost += cost_of<WIDE>(columns, blocks_in(g.shared));
+      if (g.shared) widest = max(widest, min(columns, WIDE));
     }
+    const int most = block_cost(__builtin_amdgcn_readfirstlane((int)wave_max_valu((float)widest)));
     groups_upto = wave_scan(cost);
     shared_cost = __builtin_amdgcn_readlane(groups_upto, 63);
     cost = 0;
     for (int i = 0; i < per_seq; ++i) {
       const int64_t at = (int64_t)lane * per_seq + i;
       if (at >= a.seqs) break;
-      const int2 own = own_of(a, (int)at);
-      if (stash && at < kStash) stash[at] = own;
+      const int2 own = batch.own_of((int)at);
       cost += cost_of<WIDE>(a.per_kv, blocks_in(own.y - own.x));
     }
     seqs_upto = wave_scan(cost);
     total = shared_cost + __builtin_amdgcn_readlane(seqs_upto, 63);
     // no piece is shorter than a block
-    pieces = max(1, min(a.pieces, total / block_cost(WIDE / 16)));
+    pieces = max(1, min(a.pieces, total / most));
+    each = total / pieces;
+    longer = total - each * pieces;
   }
 
-  // A sequence's own positions [x, y).
-  static __device__ __forceinline__ int2 own_of(const SharedCall& a, int seq) {
-    Group g;
-    group_of(a, seq, g);
-    const int len = clamp_len(a.lens[seq], a.cap);
-    return make_int2(min(g.shared, len), len);
-  }
-
+  // Pieces differ by one in length at most.
   __device__ __forceinline__ int start(int piece) const {
-    return (int)((int64_t)piece * total / pieces);
+    return piece * each + min(piece, longer);
   }
   __device__ __forceinline__ int piece_of(int at) const {
-    return (int)((((int64_t)at + 1) * pieces - 1) / max(total, 1));
+    const int head = longer * (each + 1);
+    return at < head ? at / (each + 1) : longer + (at - head) / max(each, 1);
   }
-  // The pieces that an item of `blocks` blocks of cost `each` from `base` on lies in.
-  __device__ __forceinline__ int2 pieces_of(int base, int blocks, int each) const {
-    return blocks ? make_int2(piece_of(base), piece_of(base + (blocks - 1) * each))
+  // The pieces that an item of `columns` columns and `blocks` blocks from `base` on lies in.
+  __device__ __forceinline__ int2 pieces_of(int base, int blocks, int columns) const {
+    base += kItemCost;
+    return blocks ? make_int2(piece_of(base),
+                              piece_of(base + (blocks - 1) * block_cost(columns)))
                   : make_int2(0, -1);
   }
 };
@@ -161,110 +209,124 @@ struct Columns {
   float m[N], l[N], c;                                  // c: scale to base 2
   int seen[N];                                          // positions that a lane's column attends to
   int r, g, k_lane, v_lane, v_row;
+  int k_place, v_place;                                 // of a lane's first pieces in LDS
+  int at_run, token_bytes;                              // of the run that a lane finds
+  uint64_t base, page_bytes;
 
-  struct Tile {                                         // two halves of 16 positions
-    int page[2], rows[2];
-  };
-  struct Ends {
-    const char* k;
-    const char* v;
-    int shift;
+  // Where the rows of a tile lie.  A tile is up to four runs of 16 positions, each in one page; lane
+  // i finds run i % 4 in K (i / 4 even) or in V, in vector registers: for each run anew in scalar
+  // ones it is 130 instructions a tile, a third of all the wave's.
+  struct Where {
+    uint32_t lo, hi;
+    int bytes, rows;
   };
 
-  __device__ __forceinline__ void lane(const PagePool& pool) {
+  __device__ __forceinline__ void lane(const PagePool& pool, const char* k, const char* v) {
     const int thread = fresh(threadIdx.x);
     r = thread & 15;
     g = (thread & 63) >> 4;
     k_lane = r * (int)pool.k_token * E + 16 * g;
     v_row = (int)pool.v_token * E;
     v_lane = 4 * g * v_row + r * VD * E;
+    k_place = r * RB + ((g ^ swap(r)) << 4);
+    const int bytes = r * VD * E;
+    v_place = 4 * g * RB + (((bytes >> 4) ^ swap(4 * g)) << 4) + (bytes & 15);
+    const bool of_v = thread & 4;
+    at_run = (thread & 3) * 16;
+    base = reinterpret_cast<uintptr_t>(of_v ? v : k);
+    page_bytes = (of_v ? pool.v_page : pool.k_page) * E;
+    token_bytes = (int)(of_v ? pool.v_token : pool.k_token) * E;
   }
 
-  __device__ __forceinline__ void ids(const int32_t* __restrict__ row, int shift, int p0, int limit,
-                                      Tile& t) const {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int p = p0 + 16 * h;
-      t.page[h] = p < limit ? uniform_load(row, p >> shift) : -1;
-    }
+  // The page of the lane's run of the tile at p0 < end.
+  __device__ __forceinline__ int page_id(const int32_t* __restrict__ row, int shift, int p0,
+                                         int end) const {
+    return row[max(min(p0 + at_run, end - 1), 0) >> shift];
   }
 
-  __device__ __forceinline__ void count(int p0, int end, int n_pages, Tile& t) const {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool there = (uint32_t)t.page[h] < (uint32_t)n_pages;
-      t.rows[h] = there ? min(max(end - (p0 + 16 * h), 0), 16) : 0;
-      t.page[h] = there ? t.page[h] : 0;
-    }
+  __device__ __forceinline__ Where where(const PagePool& pool, int page, int p0, int end) const {
+    const int p = p0 + at_run;
+    Where x;
+    x.rows = (uint32_t)page < (uint32_t)pool.pages ? min(max(end - p, 0), 16) : 0;
+    const uint64_t at = base + (uint64_t)(uint32_t)(x.rows ? page : 0) * page_bytes +
+                        (uint64_t)(p & (pool.page_size - 1)) * (uint32_t)token_bytes;
+    x.lo = (uint32_t)at;
+    x.hi = (uint32_t)(at >> 32) & 0xffffu;
+    x.bytes = x.rows * token_bytes;
+    return x;
   }
 
-  __device__ __forceinline__ void load_k(const PagePool& pool, const Ends& e, const Tile& t,
-                                         int p0) {
+  static __device__ __forceinline__ Rsrc rows_of(const Where& x, int i) {
+    const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(x.hi, i) << 32 |
+                        (uint32_t)__builtin_amdgcn_readlane(x.lo, i);
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(at), 0,
+                                             __builtin_amdgcn_readlane(x.bytes, i), 0x00027000);
+  }
+
+  __device__ __forceinline__ void load_k(const Where& x) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const Rsrc rows = rows_at(e.k + (t.page[h] * pool.k_page +
-                                       ((p0 + 16 * h) & (pool.page_size - 1)) * pool.k_token) * E,
-                                t.rows[h] * (int)pool.k_token * E);
+      const Rsrc rows = rows_of(x, h);
 #pragma unroll
       for (int s = 0; s < KL; ++s) load_row<false>(rows, k_lane + 64 * s, kf[h][s]);
     }
   }
 
-  __device__ __forceinline__ void load_v(const PagePool& pool, const Ends& e, const Tile& t,
-                                         int p0) {
+  __device__ __forceinline__ void load_v(const Where& x) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const Rsrc rows = rows_at(e.v + (t.page[h] * pool.v_page +
-                                       ((p0 + 16 * h) & (pool.page_size - 1)) * pool.v_token) * E,
-                                t.rows[h] * (int)pool.v_token * E);
+      const Rsrc rows = rows_of(x, 4 + h);
 #pragma unroll
       for (int j = 0; j < 4; ++j) load_row<false>(rows, v_lane + j * v_row, vf[4 * h + j]);
     }
   }
 
-  __device__ __forceinline__ void scores(const u32x4 (&q)[QS], float (&s)[8]) const {
-    floatx4 a[2] = {};
+  // Two chains of products a set, all in turn.
+  template <int M>
+  __device__ __forceinline__ void scores(float (&s)[M][8]) const {
+    floatx4 a[M][2] = {};
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t(&x)[4] = kf[h][i];
-        if (E == 2)
-          a[h] = mfma<QT>(u32x4{x[0], x[1], x[2], x[3]}, q[i], a[h]);
-        else
-          a[h] = mfma<QT>(u32x4{widen<QT, false>(x[0]), widen<QT, true>(x[0]),
-                                widen<QT, false>(x[1]), widen<QT, true>(x[1])},
-                          q[(2 * i) % QS], a[h]);
-      }
-      if (E == 1) {
+      for (int part = 0; part < (E == 2 ? 1 : 2); ++part) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t(&x)[4] = kf[h][i];
-          a[h] = mfma<QT>(u32x4{widen<QT, false>(x[2]), widen<QT, true>(x[2]),
-                                widen<QT, false>(x[3]), widen<QT, true>(x[3])},
-                          q[(2 * i + 1) % QS], a[h]);
+          const uint32_t x0 = x[2 * part], x1 = x[2 * part + 1];
+          const u32x4 k = E == 2 ? u32x4{x[0], x[1], x[2], x[3]}
+                                 : u32x4{widen<QT, false>(x0), widen<QT, true>(x0),
+                                         widen<QT, false>(x1), widen<QT, true>(x1)};
+#pragma unroll
+          for (int n = 0; n < M; ++n)
+            a[n][h] = mfma<QT>(k, qf[n][E == 2 ? i : (2 * i + part) % QS], a[n][h]);
         }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = a[j >> 2][j & 3] * c;
+    for (int n = 0; n < M; ++n)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[n][j] = a[n][j >> 2][j & 3];
   }
 
   // Rows that do not count, and positions past a column's end: score -inf.
-  __device__ __forceinline__ void mask(const Tile& t, int p0, int n, float (&s)[8]) const {
+  __device__ __forceinline__ void mask(int rows0, int rows1, int p0, int n, float (&s)[8]) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int at = 4 * g + (j & 3);
-      s[j] = at < t.rows[j >> 2] && p0 + 16 * (j >> 2) + at < seen[n] ? s[j] : -__builtin_inff();
+      s[j] = at < (j < 4 ? rows0 : rows1) && p0 + 16 * (j >> 2) + at < seen[n] ? s[j]
+                                                                               : -__builtin_inff();
     }
   }
 
-  // Running softmax of one set of columns; s becomes the weights.
+  // Running softmax of one set of columns; s, products of q and k, become the weights.  The factor c
+  // is above 0, so the largest product is the largest score.
   __device__ __forceinline__ void weights(int n, float (&s)[8]) {
-    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
-                      fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    top = xor32_max(xor16_max(top));
-    if (__any(top > m[n])) {
+    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), s[2]), fmaxf(fmaxf(s[3], s[4]), s[5]));
+    top = fmaxf(fmaxf(top, s[6]), s[7]);
+    top = xor32_max(xor16_max(top)) * c;
+    // in bf16 weights may grow to 2^8 before all sums are brought to the new maximum (f16 has no
+    // room above 1): pieces are short, and the maximum grows in nearly every tile of one
+    if (__any(top > m[n] + (QT == MTL_T_BF16 ? 8.f : 0.f))) {
       const float mn = fmaxf(m[n], top);
       const float a = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
       l[n] *= a;
@@ -274,7 +336,7 @@ struct Columns {
     }
     const float mu = m[n] == -__builtin_inff() ? 0.f : m[n];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = __builtin_amdgcn_exp2f(s[j] - mu);
+    for (int j = 0; j < 8; ++j) s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -mu));
     l[n] += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   }
 
@@ -305,57 +367,164 @@ struct Columns {
     }
   }
 
-  // This wave's tiles of positions [begin, end) for the first M sets of columns.  least: the
-  // smallest `seen` of all columns.
+  // 32 positions from p0 on, in kf and vf, for M sets of columns.  rows0, rows1: how many of each 16
+  // count; least: the smallest `seen` of all columns; k_done is called when kf is used up.
+  template <int M, class F>
+  __device__ __forceinline__ void tile(int rows0, int rows1, int p0, int least, F&& k_done) {
+    float s[M][8];
+    scores<M>(s);
+    k_done();
+    if (rows0 + rows1 < kTile || p0 + kTile > least) {
+#pragma unroll
+      for (int n = 0; n < M; ++n) mask(rows0, rows1, p0, n, s[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < M; ++n) weights(n, s[n]);
+    u32x4 hi[M], lo[M];
+#pragma unroll
+    for (int n = 0; n < M; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x, y;
+        two_terms<QT>(s[n][2 * j] * kLift<QT>, s[n][2 * j + 1] * kLift<QT>, x, y);
+        hi[n][j] = x;
+        lo[n][j] = y;
+      }
+#pragma unroll
+    for (int d = 0; d < VD; d += 2) {     // no product waits for the one before
+      const u32x4 v0 = value(d), v1 = value(d + 1);
+#pragma unroll
+      for (int n = 0; n < M; ++n) {
+        acc[n][d] = mfma<QT>(v0, hi[n], acc[n][d]);
+        acc[n][d + 1] = mfma<QT>(v1, hi[n], acc[n][d + 1]);
+      }
+#pragma unroll
+      for (int n = 0; n < M; ++n) {
+        acc[n][d] = mfma<QT>(v0, lo[n], acc[n][d]);
+        acc[n][d + 1] = mfma<QT>(v1, lo[n], acc[n][d + 1]);
+      }
+    }
+  }
+
+  // This wave's tiles from p0 to `end`, every fourth, for M sets of columns.  page0, page: of the
+  // first two.
   template <int M>
-  __device__ __forceinline__ void run(const PagePool& pool, const Ends& e,
-                                      const int32_t* __restrict__ row, int begin, int end,
-                                      int least) {
+  __device__ __forceinline__ void run(const PagePool& pool, const int32_t* __restrict__ row,
+                                      int shift, int p0, int end, int least, int page0, int page) {
     constexpr int kStep = kSharedWaves * kTile;
-    int p0 = begin + wave_id() * kTile;
     if (p0 >= end) return;
-    Tile t, next;
-    ids(row, e.shift, p0, end, t);
-    count(p0, end, pool.pages, t);
-    load_k(pool, e, t, p0);
-    load_v(pool, e, t, p0);
+    Where x = where(pool, page0, p0, end);
+    load_k(x);
+    load_v(x);
     while (true) {
       const int p1 = p0 + kStep;
-      const bool more = p1 < end;
-      ids(row, e.shift, p1, end, next);
-      count(p1, end, pool.pages, next);
-      float s[M][8];
-#pragma unroll
-      for (int n = 0; n < M; ++n) scores(qf[n], s[n]);
-      if (more) load_k(pool, e, next, p1);
-      if (t.rows[0] + t.rows[1] < kTile || p0 + kTile > least) {
-#pragma unroll
-        for (int n = 0; n < M; ++n) mask(t, p0, n, s[n]);
+      const int rows0 = __builtin_amdgcn_readlane(x.rows, 0);
+      const int rows1 = __builtin_amdgcn_readlane(x.rows, 1);
+      if (p1 < end) {
+        x = where(pool, page, p1, end);
+        page = page_id(row, shift, p1 + kStep, end);
       }
-#pragma unroll
-      for (int n = 0; n < M; ++n) weights(n, s[n]);
-      u32x4 hi[M], lo[M];
-#pragma unroll
-      for (int n = 0; n < M; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t x, y;
-          two_terms<QT>(s[n][2 * j] * kLift<QT>, s[n][2 * j + 1] * kLift<QT>, x, y);
-          hi[n][j] = x;
-          lo[n][j] = y;
-        }
-#pragma unroll
-      for (int d = 0; d < VD; ++d) {
-        const u32x4 v = value(d);
-#pragma unroll
-        for (int n = 0; n < M; ++n) acc[n][d] = mfma<QT>(v, hi[n], acc[n][d]);
-#pragma unroll
-        for (int n = 0; n < M; ++n) acc[n][d] = mfma<QT>(v, lo[n], acc[n][d]);
-      }
-      if (!more) return;
-      load_v(pool, e, next, p1);
-      t = next;
+      tile<M>(rows0, rows1, p0, least, [&] { if (p1 < end) load_k(x); });
+      if (p1 >= end) return;
+      load_v(x);
       p0 = p1;
+    }
+  }
+
+  // --- tiles of kStage positions in LDS, which all waves of the workgroup go through, each with
+  // columns of its own.  Pieces of 16 bytes of a row lie in an order that goes by the row, so that
+  // 16 lanes that read one piece of 16 rows (K), or one row (V), meet all banks once.
+  static constexpr int RB = D * E, PIECES = RB / 16, LOADS = kStage * PIECES / 256;
+  static constexpr int kStageBytes = kStage * RB;       // of K, and again of V
+
+  // What a row's pieces are exchanged by; rows 16 apart have the same.
+  static __device__ __forceinline__ int swap(int row) { return row / (256 / RB) & (PIECES - 1); }
+
+  // A wave brings one run of 16 rows of K (or V), 1 KB at a time; x[i] goes to LDS in its place.
+  __device__ __forceinline__ void fetch(const Where& t, int run, int token, uint32_t (&x)[LOADS][4])
+      const {
+    const int lane = fresh(threadIdx.x) & 63, row = lane / PIECES;
+    const Rsrc rows = rows_of(t, run);
+    const int at = row * token * E, piece = ((lane % PIECES) ^ swap(row)) << 4;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)     // rows 64 / PIECES apart exchange by 4 more
+      load_row<false>(rows, at + (piece ^ (i << 6)) + i * (64 / PIECES) * token * E, x[i]);
+  }
+
+  __device__ __forceinline__ void put(char* to, const uint32_t (&x)[LOADS][4]) const {
+    char* mine = to + wave_id() * 16 * RB + (fresh(threadIdx.x) & 63) * 16;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      *reinterpret_cast<u32x4*>(mine + i * 1024) = u32x4{x[i][0], x[i][1], x[i][2], x[i][3]};
+  }
+
+  // kf (vf) of 32 positions from row `first` of the tile on.  Addresses are formed anew from two
+  // that a lane keeps: all of them, kept over the loop, do not fit the registers.
+  __device__ __forceinline__ void take_k(const char* k, int first) {
+    const int at = fresh(k_place);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < KL; ++s) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(k + (at ^ s << 6) + (first + 16 * h) * RB);
+        kf[h][s][0] = x.x; kf[h][s][1] = x.y; kf[h][s][2] = x.z; kf[h][s][3] = x.w;
+      }
+  }
+
+  __device__ __forceinline__ void take_v(const char* v, int first) {
+    const int at = fresh(v_place);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int row = j & 3, other = PIECES == 16 ? row : PIECES == 8 ? row >> 1 : 0;
+      const char* from = v + (at ^ other << 4) + (first + 16 * (j >> 2) + row) * RB;
+      if (VW == 4) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(from);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vf[j][w] = x[w];
+      } else if (VW == 2) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(from);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vf[j][w] = x[w];
+      } else {
+        vf[j][0] = *reinterpret_cast<const uint32_t*>(from);
+      }
+    }
+  }
+
+  // Positions [begin, end): of each tile in LDS this wave takes the first or second 32.
+  __device__ __forceinline__ void run_wide(const PagePool& pool, const int32_t* __restrict__ row,
+                                           int shift, int begin, int end, int least, int half,
+                                           char* lds, int page0, int page) {
+    if (begin >= end) return;
+    uint32_t kx[LOADS][4], vx[LOADS][4];
+    Where x = where(pool, page0, begin, end);
+    fetch(x, wave_id(), (int)pool.k_token, kx);
+    fetch(x, 4 + wave_id(), (int)pool.v_token, vx);
+    __syncthreads();                    // what was read there before
+    put(lds, kx);
+    put(lds + kStageBytes, vx);
+    __syncthreads();
+    int buffer = 0;
+    for (int p0 = begin; p0 < end; p0 += kStage) {
+      const int p1 = p0 + kStage;
+      const bool more = p1 < end;
+      const int rows0 = __builtin_amdgcn_readlane(x.rows, 2 * half);
+      const int rows1 = __builtin_amdgcn_readlane(x.rows, 2 * half + 1);
+      if (more) {
+        x = where(pool, page, p1, end);
+        page = page_id(row, shift, p1 + kStage, end);
+        fetch(x, wave_id(), (int)pool.k_token, kx);
+        fetch(x, 4 + wave_id(), (int)pool.v_token, vx);
+      }
+      const char* k = lds + buffer * 2 * kStageBytes;
+      take_k(k, 32 * half);
+      tile<N>(rows0, rows1, p0 + 32 * half, least, [&] { take_v(k + kStageBytes, 32 * half); });
+      buffer ^= 1;
+      if (more) {
+        put(lds + buffer * 2 * kStageBytes, kx);
+        put(lds + buffer * 2 * kStageBytes + kStageBytes, vx);
+      }
+      __syncthreads();
     }
   }
 };
@@ -364,105 +533,132 @@ struct Columns {
 template <int QT, int KT, int D, int N>
 struct Piece {
   using Wave = Columns<QT, KT, D, N>;
-  static constexpr int WIDE = 16 * N, LD = D + 4;
+  // LDS of two waves' sums, or of two tiles of K and V
+  static constexpr int kSumBytes = N * 64 * (Wave::VD * 16 + 8);
+  static constexpr int kJoinBytes = 2 * kSumBytes;
+  static constexpr int kBytes = N > 1 && 4 * Wave::kStageBytes > kJoinBytes ? 4 * Wave::kStageBytes
+                                                                            : kJoinBytes;
   const SharedCall& a;
+  const Batch& batch;
   const PagePool& pool;
-  float* lds;
+  char* lds;
   int kvh;
-  typename Wave::Ends ends;
+  float by;                             // 1 / per_kv
+  const char* k_end;                    // the kv head's K and V in the first page
+  const char* v_end;
+  int shift;
+  uint32_t sign;
   Wave w;
 
-  __device__ __forceinline__ Piece(const SharedCall& a, const PagePool& pool, int kvh, float* lds)
-      : a(a), pool(pool), lds(lds), kvh(kvh) {
-    ends.shift = __builtin_ctz(pool.page_size);
-    ends.k = static_cast<const char*>(pool.k) + kvh * pool.k_head * w.E;
-    ends.v = static_cast<const char*>(pool.v) + kvh * pool.v_head * w.E;
-    w.c = a.scale * (pool.k_scale ? uniform_load(pool.k_scale, kvh) : 1.f) * kLog2e;
+  __device__ __forceinline__ Piece(const Batch& batch, const PagePool& pool, int kvh, char* lds)
+      : a(batch.a), batch(batch), pool(pool), lds(lds), kvh(kvh), by(1.f / batch.a.per_kv) {
+    shift = __builtin_ctz(pool.page_size);
+    k_end = static_cast<const char*>(pool.k) + kvh * pool.k_head * w.E;
+    v_end = static_cast<const char*>(pool.v) + kvh * pool.v_head * w.E;
+    // a factor below 0 is the queries' sign; 0 is as good as the smallest number, beside which a
+    // masked -infinity stays one
+    const float c = a.scale * (pool.k_scale ? uniform_load(pool.k_scale, kvh) : 1.f) * kLog2e;
+    sign = c < 0.f ? 0x80008000u : 0u;
+    w.c = fmaxf(fabsf(c), 0x1p-126f);
   }
 
+  // n / per_kv for n < 2^20: (n + 1/2) / per_kv lies further from a whole number than float32 is off.
+  __device__ __forceinline__ int sequences_in(int n) const { return (int)((n + 0.5f) * by); }
+
   // Columns c0 .. c0 + columns - 1 of the sequences from `first` on, over positions [begin, end) of
-  // the row of `leader`.  whole: where the parts of an uncut item lie; cut: a cut one's.
+  // the row of `leader`; columns that are not there go along as the first one, and no further.  whole: where the parts of an uncut item lie; cut: a cut one's.
   __device__ __forceinline__ void attend(int first, int c0, int columns, int leader, int begin,
                                          int end, float* whole, float* whole_ml, int64_t cut) {
-    w.lane(pool);
+    // wide: two waves beside each other take the columns, two take the positions
+    const bool wide = N > 1 && columns > kNarrow;
+    const int sets = (columns + 15) / 16;
+    const int from = wide ? (wave_id() & 1) * 32 : 0;
+    w.lane(pool, k_end, v_end);
+    const int32_t* row = a.table + leader * a.ldt;
+    const int p0 = wide ? begin : begin + wave_id() * kTile;
+    const int page0 = w.page_id(row, shift, p0, end);
+    const int page1 = w.page_id(row, shift, p0 + (wide ? kStage : kSharedBlock), end);
+    const int seq0 = first + c0 / a.per_kv, skip = c0 % a.per_kv;
     int least = INT_MAX;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int at = 16 * n + w.r;
+      const int at = from + 16 * n + w.r;
       const bool there = at < columns;
-      const int c = c0 + at, seq = first + (there ? c / a.per_kv : 0);
-      const uint16_t* q = a.q + seq * a.ldq + (kvh * a.per_kv + c % a.per_kv) * a.ldh;
+      const int on = there ? sequences_in(skip + at) : 0, seq = seq0 + on;
+      const int head = kvh * a.per_kv + (there ? skip + at - on * a.per_kv : 0);
+      const uint16_t* q = a.q + seq * a.ldq + head * a.ldh;
 #pragma unroll
       for (int s = 0; s < w.QS; ++s) {
         const int d = w.E == 2 ? 32 * s + 8 * w.g : 64 * (s >> 1) + 16 * w.g + 8 * (s & 1);
-        w.qf[n][s] = there ? *reinterpret_cast<const u32x4*>(q + d) : u32x4{0, 0, 0, 0};
+        w.qf[n][s] = *reinterpret_cast<const u32x4*>(q + d) ^ sign;
       }
-      w.seen[n] = there ? clamp_len(a.lens[seq], a.cap) : INT_MAX;
+      const int len = batch.len(seq);
+      w.seen[n] = there ? len : INT_MAX;
       least = min(least, w.seen[n]);
     }
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
     least = __builtin_amdgcn_readfirstlane(least);
     w.clear();
-    const int32_t* row = a.table + leader * a.ldt;
-    const int sets = (columns + 15) / 16;
-    if (N == 1 || sets == 1) w.template run<1>(pool, ends, row, begin, end, least);
-    else if (N == 2 || sets == 2) w.template run<(N < 2 ? N : 2)>(pool, ends, row, begin, end, least);
-    else w.template run<N>(pool, ends, row, begin, end, least);
-    join(first, c0, columns, sets, whole, whole_ml, cut);
-  }
-
-  // Joins the waves through LDS, a set of columns at a time.
-  __device__ __forceinline__ void join(int first, int c0, int columns, int sets, float* whole,
-                                       float* whole_ml, int64_t cut) {
-    float* ml = lds + kSharedWaves * 16 * LD;
-    const int thread = fresh(threadIdx.x), wave = wave_id();
-    const int r = thread & 15, g = (thread & 63) >> 4;
+    if (wide) w.run_wide(pool, row, shift, p0, end, least, wave_id() >> 1, lds, page0, page1);
+    else if (sets == 1) w.template run<1>(pool, row, shift, p0, end, least, page0, page1);
+    else w.template run<N>(pool, row, shift, p0, end, least, page0, page1);
+    take_in(2, sets);
+    if (!wide) take_in(1, sets);
+    if (wave_id() >= (wide ? 2 : 1)) return;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      if (n >= sets) break;
+      const int at = from + 16 * n + w.r;
       const float l = xor32_add(xor16_add(w.l[n]));
-      __syncthreads();                 // what was read there before
-      float* o = lds + (wave * 16 + r) * LD + w.VD * 4 * g;
+      if (at >= columns) continue;
+      const int on = sequences_in(skip + at);
+      const int64_t head = (int64_t)(seq0 + on) * a.n_heads + kvh * a.per_kv + skip + at -
+                           on * a.per_kv;
+      float* to = (cut < 0 ? whole + head * D : a.cut + (cut + at) * D) + w.VD * 4 * w.g;
+      float* to_ml = cut < 0 ? whole_ml + 2 * head : a.cut_ml + 2 * (cut + at);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int d = 0; d < w.VD; d += 4)
-          *reinterpret_cast<floatx4*>(o + i * w.VD + d) = floatx4{
+          *reinterpret_cast<floatx4*>(to + i * w.VD + d) = floatx4{
               w.acc[n][d][i], w.acc[n][d + 1][i], w.acc[n][d + 2][i], w.acc[n][d + 3][i]};
-      if (g == 0) {
-        ml[2 * (wave * 16 + r)] = w.m[n];
-        ml[2 * (wave * 16 + r) + 1] = l;
-      }
-      __syncthreads();
-      const int there = min(16, columns - 16 * n);
-      for (int i = thread; i < there * (D / 4); i += kSharedWaves * 64) {
-        const int h = i / (D / 4), d = 4 * (i % (D / 4));
-        float top = -__builtin_inff();
+      if (w.g == 0) *reinterpret_cast<float2*>(to_ml) = make_float2(w.m[n], l);
+    }
+  }
+
+  // Waves `half` .. 2 half - 1 hand their sums to waves 0 .. half - 1, through LDS as the lanes have
+  // them.
+  __device__ __forceinline__ void take_in(int half, int sets) {
+    const int lane = fresh(threadIdx.x) & 63, wave = wave_id();
+    __syncthreads();                    // what was read there before
+    if (wave >= half && wave < 2 * half) {
+      char* to = lds + (wave - half) * kSumBytes + lane * 16;
 #pragma unroll
-        for (int x = 0; x < kSharedWaves; ++x) top = fmaxf(top, ml[2 * (x * 16 + h)]);
-        const float mu = top == -__builtin_inff() ? 0.f : top;
-        float sum = 0.f;
-        floatx4 s = {0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < N; ++n) {
+        if (n >= sets) break;
 #pragma unroll
-        for (int x = 0; x < kSharedWaves; ++x) {
-          const float e = __builtin_amdgcn_exp2f(ml[2 * (x * 16 + h)] - mu);
-          sum = fmaf(ml[2 * (x * 16 + h) + 1], e, sum);
-          s += e * *reinterpret_cast<const floatx4*>(lds + (x * 16 + h) * LD + d);
-        }
-        const int at = 16 * n + h, c = c0 + at;
-        const int64_t head = (int64_t)(first + c / a.per_kv) * a.n_heads + kvh * a.per_kv +
-                             c % a.per_kv;
-        float* to = cut < 0 ? whole + head * D : a.cut + (cut + at) * D;
-        float* to_ml = cut < 0 ? whole_ml + 2 * head : a.cut_ml + 2 * (cut + at);
-        *reinterpret_cast<floatx4*>(to + d) = s;
-        if (d == 0) {
-          to_ml[0] = top;
-          to_ml[1] = sum;
-        }
+        for (int d = 0; d < w.VD; ++d)
+          *reinterpret_cast<floatx4*>(to + (n * w.VD + d) * 1024) = w.acc[n][d];
+        *reinterpret_cast<float2*>(to + N * w.VD * 1024 + n * 512 - lane * 8) =
+            make_float2(w.m[n], w.l[n]);
       }
     }
     __syncthreads();
+    if (wave >= half) return;
+    const char* from = lds + wave * kSumBytes + lane * 16;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (n >= sets) break;
+      const float2 ml = *reinterpret_cast<const float2*>(from + N * w.VD * 1024 + n * 512 - lane * 8);
+      const float top = fmaxf(w.m[n], ml.x), mu = top == -__builtin_inff() ? 0.f : top;
+      const float e0 = __builtin_amdgcn_exp2f(w.m[n] - mu), e1 = __builtin_amdgcn_exp2f(ml.x - mu);
+      w.m[n] = top;
+      w.l[n] = w.l[n] * e0 + ml.y * e1;
+#pragma unroll
+      for (int d = 0; d < w.VD; ++d)
+        w.acc[n][d] = w.acc[n][d] * e0 +
+                      *reinterpret_cast<const floatx4*>(from + (n * w.VD + d) * 1024) * e1;
+    }
   }
 
   // The table row that a group's shared positions are read through, and how many of them any of its
@@ -472,7 +668,7 @@ struct Piece {
     int best = -1, at = g.begin;
     for (int s0 = g.begin; s0 < g.end; s0 += 64) {
       const int s = s0 + lane;
-      const int len = s < g.end ? min(clamp_len(a.lens[s], a.cap), g.shared) : -1;
+      const int len = s < g.end ? min(batch.len(s), g.shared) : -1;
       int most = len;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
@@ -488,7 +684,9 @@ struct Piece {
 };
 
 // The blocks [x, y) of an item that fall into a piece: blocks that begin within [lo, hi).
-__device__ __forceinline__ int2 blocks_within(int base, int blocks, int each, int lo, int hi) {
+__device__ __forceinline__ int2 blocks_within(int base, int blocks, int columns, int lo, int hi) {
+  const int each = block_cost(columns);
+  base += kItemCost;
   const int x = lo <= base ? 0 : (lo - base + each - 1) / each;
   const int y = hi <= base ? 0 : (hi - base + each - 1) / each;
   return make_int2(min(max(x, 0), blocks), min(max(y, 0), blocks));
@@ -496,7 +694,8 @@ __device__ __forceinline__ int2 blocks_within(int base, int blocks, int each, in
 
 // What the second launch goes by.
 template <int WIDE>
-__device__ __forceinline__ void write_items(const SharedCall& a, const Row<WIDE>& row) {
+__device__ __forceinline__ void write_items(const Batch& batch, const Row<WIDE>& row) {
+  const SharedCall& a = batch.a;
   const int lane = threadIdx.x & 63;
   const int before_groups = __builtin_amdgcn_update_dpp(0, row.groups_upto, 0x138, 0xf, 0xf, false);
   const int before_seqs = __builtin_amdgcn_update_dpp(0, row.seqs_upto, 0x138, 0xf, 0xf, false);
@@ -505,14 +704,14 @@ __device__ __forceinline__ void write_items(const SharedCall& a, const Row<WIDE>
     for (int i = 0; i < row.per_group; ++i) {
       const int64_t at = (int64_t)lane * row.per_group + i;
       if (at >= a.n_groups) break;
-      const Group g = group_at(a, (int)at);
+      const Group g = batch.group((int)at);
       const int blocks = blocks_in(g.shared), columns = (g.end - g.begin) * a.per_kv;
       if (!blocks) continue;
       const int id = g.begin * a.per_kv / WIDE + (int)at;
       for (int c = 0, t = 0; c < columns; c += WIDE, ++t) {
-        const int each = block_cost((min(WIDE, columns - c) + 15) / 16);
-        if (id + t < a.tiles) a.item_tiles[id + t] = row.pieces_of(base, blocks, each);
-        base += blocks * each;
+        const int n = min(WIDE, columns - c);
+        if (id + t < a.tiles) a.item_tiles[id + t] = row.pieces_of(base, blocks, n);
+        base += item_cost(n, blocks);
       }
     }
   } else if (wave_id() == 1) {
@@ -522,85 +721,94 @@ __device__ __forceinline__ void write_items(const SharedCall& a, const Row<WIDE>
       if (at >= a.seqs) break;
       const int s = (int)at;
       Group g;
-      const int group = group_of(a, s, g);
-      const int len = clamp_len(a.lens[s], a.cap), blocks = blocks_in(len - min(g.shared, len));
+      const int group = batch.group_of(s, g);
+      const int len = batch.len(s), blocks = blocks_in(len - min(g.shared, len));
       a.seq_items[s] = g.shared ? make_int2(g.begin * a.per_kv / WIDE + group,
                                             (s - g.begin) * a.per_kv)
                                 : make_int2(-1, 0);
       for (int c = 0, t = 0; c < a.per_kv; c += WIDE, ++t) {
-        const int each = block_cost((min(WIDE, a.per_kv - c) + 15) / 16);
-        a.item_own[at * a.own_tiles + t] = row.pieces_of(base, blocks, each);
-        base += blocks * each;
+        const int n = min(WIDE, a.per_kv - c);
+        a.item_own[at * a.own_tiles + t] = row.pieces_of(base, blocks, n);
+        base += item_cost(n, blocks);
       }
     }
   }
 }
 
 template <int QT, int KT, int D, int N>
-__global__ void __launch_bounds__(kSharedWaves * 64, N == 1 ? 2 : 1) paged_shared_kernel(
-    SharedCall a, PagePool pool) {
-  constexpr int WIDE = 16 * N;
-  __shared__ float lds[kSharedWaves * 16 * (D + 4) + 2 * kSharedWaves * 16];
-  __shared__ int2 stash[kStash];
+__global__ void __launch_bounds__(kSharedWaves * 64, 2) paged_shared_kernel(SharedCall a,
+                                                                            PagePool pool) {
+  constexpr int WIDE = N == 1 ? 16 : kWide;
+  __shared__ __align__(16) char lds[Piece<QT, KT, D, N>::kBytes];
+  __shared__ Lists lists;
   const int units = pool.kv_heads;
   const int kvh = blockIdx.x % units, piece = blockIdx.x / units;
-  const Row<WIDE> row(a, wave_id() == 0 ? stash : nullptr);
+  const Batch batch(a, lists);
+  const Row<WIDE> row(a, batch);
   if (piece == a.pieces) {
-    if (kvh == 0) write_items<WIDE>(a, row);
+    if (kvh == 0) write_items<WIDE>(batch, row);
     return;
   }
   if (piece >= row.pieces || row.total <= 0) return;
-  __syncthreads();
   const int lo = row.start(piece), hi = row.start(piece + 1);
   if (lo >= hi) return;
-  Piece<QT, KT, D, N> p(a, pool, kvh, lds);
+  Piece<QT, KT, D, N> p(batch, pool, kvh, lds);
   const int64_t slot = (int64_t)blockIdx.x * 2 * WIDE;
   const int64_t heads = (int64_t)a.seqs * a.n_heads;
-  if (lo < row.shared_cost) {
-    const int from = __builtin_ctzll(__ballot(lo < row.groups_upto));
-    int base = from ? __builtin_amdgcn_readlane(row.groups_upto, from - 1) : 0;
-    for (int64_t i = (int64_t)from * row.per_group; i < a.n_groups && base < hi; ++i) {
-      const Group g = group_at(a, (int)i);
-      const int blocks = blocks_in(g.shared), columns = (g.end - g.begin) * a.per_kv;
+  // Items from the first that reaches into the piece on: groups, then sequences.  One place in the
+  // code attends to both, which keeps the code within the instruction cache.
+  bool own = lo >= row.shared_cost;
+  int from = __builtin_ctzll(__ballot(own ? lo < row.shared_cost + row.seqs_upto
+                                          : lo < row.groups_upto));
+  int base = own ? row.shared_cost : 0;
+  if (from) base += __builtin_amdgcn_readlane(own ? row.seqs_upto : row.groups_upto, from - 1);
+  int64_t i = (int64_t)from * (own ? row.per_seq : row.per_group);
+  while (base < hi) {
+    int first, columns, leader, begin, end, blocks;
+    if (!own) {
+      if (i >= a.n_groups) {
+        own = true;
+        i = 0;
+        base = row.shared_cost;
+        continue;
+      }
+      Group g = batch.group((int)i++);  // out of LDS: the same in all lanes
+      g.begin = __builtin_amdgcn_readfirstlane(g.begin);
+      g.end = __builtin_amdgcn_readfirstlane(g.end);
+      g.shared = __builtin_amdgcn_readfirstlane(g.shared);
+      first = g.begin;
+      columns = (g.end - g.begin) * a.per_kv;
+      blocks = blocks_in(g.shared);
       const int cost = cost_of<WIDE>(columns, blocks);
-      if (base + cost > lo) {
-        const int2 lead = p.leader(g);
-        const int full = blocks * block_cost(N);
-        const int skip = lo > base ? max(min((lo - base) / full, columns / WIDE), 0) : 0;
-        int at = base + skip * full;
-        for (int c = skip * WIDE; c < columns && at < hi; c += WIDE) {
-          const int n = min(WIDE, columns - c), each = block_cost((n + 15) / 16);
-          const int2 b = blocks_within(at, blocks, each, lo, hi);
-          if (b.x < b.y)
-            p.attend(g.begin, c, n, lead.x, b.x * kSharedBlock,
-                     min(b.y * kSharedBlock, lead.y), a.whole, a.whole_ml,
-                     b.x == 0 && b.y == blocks ? -1 : slot + (b.x == 0) * WIDE);
-          at += blocks * each;
-        }
+      if (base + cost <= lo) {
+        base += cost;
+        continue;
       }
-      base += cost;
+      const int2 lead = p.leader(g);
+      leader = __builtin_amdgcn_readfirstlane(lead.x);
+      begin = 0;
+      end = __builtin_amdgcn_readfirstlane(lead.y);
+    } else {
+      if (i >= a.seqs) break;
+      const int2 at = batch.own_of((int)i);
+      leader = first = (int)i++;
+      columns = a.per_kv;
+      begin = __builtin_amdgcn_readfirstlane(at.x);
+      end = __builtin_amdgcn_readfirstlane(at.y);
+      blocks = blocks_in(end - begin);
     }
-  }
-  if (hi > row.shared_cost) {
-    const int from = lo <= row.shared_cost
-                         ? 0 : __builtin_ctzll(__ballot(lo < row.shared_cost + row.seqs_upto));
-    int base = row.shared_cost +
-               (from ? __builtin_amdgcn_readlane(row.seqs_upto, from - 1) : 0);
-    for (int64_t s = (int64_t)from * row.per_seq; s < a.seqs && base < hi; ++s) {
-      int2 own = s < kStash ? stash[s] : Row<WIDE>::own_of(a, (int)s);
-      own.x = __builtin_amdgcn_readfirstlane(own.x);
-      own.y = __builtin_amdgcn_readfirstlane(own.y);
-      const int blocks = blocks_in(own.y - own.x);
-      for (int c = 0; c < a.per_kv; c += WIDE) {
-        const int n = min(WIDE, a.per_kv - c), each = block_cost((n + 15) / 16);
-        const int2 b = blocks_within(base, blocks, each, lo, hi);
-        if (b.x < b.y)
-          p.attend((int)s, c, n, (int)s, own.x + b.x * kSharedBlock,
-                   min(own.x + b.y * kSharedBlock, own.y), a.whole + heads * D,
-                   a.whole_ml + 2 * heads,
-                   b.x == 0 && b.y == blocks ? -1 : slot + (b.x == 0) * WIDE);
-        base += blocks * each;
-      }
+    const int full = max(item_cost(WIDE, blocks), 1);
+    const int skip = lo > base ? max(min((lo - base) / full, columns / WIDE), 0) : 0;
+    base += skip * full;
+    for (int c = skip * WIDE; c < columns; c += WIDE) {
+      const int n = min(WIDE, columns - c);
+      const int2 b = blocks_within(base, blocks, n, lo, hi);
+      if (b.x < b.y)
+        p.attend(first, c, n, leader, begin + b.x * kSharedBlock,
+                 min(begin + b.y * kSharedBlock, end), a.whole + (own ? heads * D : 0),
+                 a.whole_ml + (own ? 2 * heads : 0),
+                 b.x == 0 && b.y == blocks ? -1 : slot + (b.x == 0) * WIDE);
+      base += item_cost(n, blocks);
     }
   }
 }
@@ -619,26 +827,43 @@ __global__ void __launch_bounds__(256) paged_shared_join_kernel(SharedCall a, in
   const int kvh = h / a.per_kv, hc = h % a.per_kv;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
   float top = -__builtin_inff(), total = 0.f;
-  auto add = [&](const float* part, const float* ml) {
-    const float2 x = *reinterpret_cast<const float2*>(ml);
-    const floatx4 y = *reinterpret_cast<const floatx4*>(part + 4 * lane);
-    const float t = fmaxf(top, x.x), mu = t == -__builtin_inff() ? 0.f : t;
-    const float e0 = __builtin_amdgcn_exp2f(top - mu), e1 = __builtin_amdgcn_exp2f(x.x - mu);
-    total = total * e0 + x.y * e1;
-    o = o * e0 + y * e1;
-    top = t;
+  // Parts at(0) .. at(n - 1), several on their way at a time.
+  auto add = [&](int n, auto&& at) {
+    constexpr int kAhead = 8;
+    for (int i = 0; i < n; i += kAhead) {
+      float2 ml[kAhead];
+      floatx4 y[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        ml[j] = make_float2(-__builtin_inff(), 0.f);
+        y[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (i + j < n) at(i + j, ml[j], y[j]);
+      }
+      float t = top;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) t = fmaxf(t, ml[j].x);
+      const float mu = t == -__builtin_inff() ? 0.f : t;
+      const float e0 = __builtin_amdgcn_exp2f(top - mu);
+      total *= e0;
+      o *= e0;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float e = __builtin_amdgcn_exp2f(ml[j].x - mu);
+        total = fmaf(ml[j].y, e, total);
+        o += y[j] * e;
+      }
+      top = t;
+    }
   };
   auto item = [&](int2 pieces, int64_t whole, int column) {
-    if (pieces.x == pieces.y) {
-      add(a.whole + whole * D, a.whole_ml + 2 * whole);
-      return;
-    }
-    const int last = min(pieces.y, a.pieces - 1);
-#pragma unroll 4
-    for (int p = max(pieces.x, 0); p <= last; ++p) {
-      const int64_t at = (((int64_t)p * kv_heads + kvh) * 2 + (p == pieces.x)) * WIDE + column;
-      add(a.cut + at * D, a.cut_ml + 2 * at);
-    }
+    const int last = min(pieces.y, a.pieces - 1), begin = max(pieces.x, 0);
+    add(last - begin + 1, [&](int i, float2& ml, floatx4& y) {
+      const int64_t cut = (((int64_t)(begin + i) * kv_heads + kvh) * 2 + (i == 0)) * WIDE + column;
+      const bool is_whole = pieces.x == pieces.y;
+      ml = *reinterpret_cast<const float2*>(is_whole ? a.whole_ml + 2 * whole : a.cut_ml + 2 * cut);
+      y = *reinterpret_cast<const floatx4*>((is_whole ? a.whole + whole * D : a.cut + cut * D) +
+                                            4 * lane);
+    });
   };
   const int2 own = a.item_own[(int64_t)seq * a.own_tiles + hc / WIDE], in = a.seq_items[seq];
   if (in.x >= 0) {
@@ -659,11 +884,10 @@ struct SharedPlan {
 static SharedPlan shared_plan(int64_t seqs, int64_t groups, int n_heads, int kv_heads) {
   SharedPlan p;
   const int64_t per_kv = n_heads / kv_heads, columns = seqs * per_kv;
-  p.sets = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
-  p.wide = 16 * p.sets;
+  p.sets = columns <= 16 ? 1 : 2;
+  p.wide = columns <= 16 ? 16 : kWide;
   p.own_tiles = (int)((per_kv + p.wide - 1) / p.wide);
-  const int workgroups = p.sets == 1 ? 512 : 256;
-  p.pieces = kv_heads < workgroups ? workgroups / kv_heads : 1;
+  p.pieces = kv_heads < kSharedWorkgroups ? kSharedWorkgroups / kv_heads : 1;
   p.tiles = columns / p.wide + groups + 1;
   p.rows = 2 * seqs * n_heads + (int64_t)p.pieces * kv_heads * 2 * p.wide;
   return p;
@@ -674,15 +898,14 @@ static void launch_shared(const SharedCall& a, const PagePool& p, const SharedPl
                           hipStream_t stream) {
   const unsigned grid = (unsigned)((s.pieces + 1) * p.kv_heads);
   const unsigned joins = (unsigned)(((int64_t)a.seqs * a.n_heads * (D / 4) + 255) / 256);
-#define MTL_RUN(N)                                                                          \
+#define MTL_RUN(N, WIDE)                                                                    \
   do {                                                                                      \
     paged_shared_kernel<QT, KT, D, N><<<grid, kSharedWaves * 64, 0, stream>>>(a, p);        \
-    paged_shared_join_kernel<QT, D, 16 * N><<<joins, 256, 0, stream>>>(a, p.kv_heads,       \
-                                                                       p.v_scale);          \
+    paged_shared_join_kernel<QT, D, WIDE><<<joins, 256, 0, stream>>>(a, p.kv_heads,         \
+                                                                     p.v_scale);            \
   } while (0)
-  if (s.sets == 1) MTL_RUN(1);
-  else if (s.sets == 2) MTL_RUN(2);
-  else MTL_RUN(4);
+  if (s.sets == 1) MTL_RUN(1, 16);
+  else MTL_RUN(2, kWide);
 #undef MTL_RUN
 }
 
@@ -701,7 +924,7 @@ static bool shared_sizes_ok(int64_t seqs, int64_t groups, int32_t n_heads, int32
   // the row of all items' blocks, and the launches' threads, within 32 bits
   const int64_t blocks = (width * page_size + kSharedBlock - 1) / kSharedBlock;
   const int64_t items = p.tiles + seqs * p.own_tiles;
-  return items <= INT32_MAX / block_cost(4) / (blocks + 1) &&
+  return items <= INT32_MAX / kItemCost / (blocks + 1) &&
          seqs * n_heads <= (int64_t)UINT32_MAX / 64 && (int64_t)(p.pieces + 1) * kv_heads <= 1 << 23;
 }
 
