@@ -1,17 +1,22 @@
 // Drawing tokens from logits: temperature, top-k, top-p and min-p (gfx950).
 //
 // Everything is decided by sums of weights, and a row has as many borders as tokens: with float32
-// sums (2^-24 of the whole) one row in some thousands would draw another token than the definition,
-// so weights and sums are of 64 bits.  Sums that come together by atomics are whole numbers
-// (weights in units of 2^-44), whose order changes nothing.
+// sums (2^-24 of the whole) one row in some thousands would draw another token than the definition.
+// Weights are of 64 bits and their sums whole numbers of 2^-44, whose order changes nothing.
 //
-// A workgroup takes a row.  It never sorts the row:
-// * The row is cut into slices; the largest logit of each gives a bound that at least n tokens
-//   reach (n slices' largest do).  Only slices that reach it are read again, and give a short list
-//   of candidates, in which every token counts those ahead of it and their weight.
-// * Where a list of at most kCandidates cannot settle the row (a wide top-p, many equal logits),
-//   the border token is found by counting or weighing the row by digits of its logits' ordered
-//   keys, kBins at a time, and the draw follows in a last pass by index.
+// The work is one read of the logits; no row is ever sorted:
+// * A first launch cuts rows into slices of 32 tokens and keeps the largest logit of each (rows of
+//   up to kMaxSlices tokens need none: they fit LDS).
+// * Rows that need the sum of all weights (top-p without a small top-k; no filter) are weighed in a
+//   second launch: a sum for each 8192 tokens, and for top-p by the logits' distance to the
+//   largest, in steps of 1/32 octave.
+// * In the last launch a workgroup takes a row.  The slices' largest logits give a bound that at
+//   least n tokens reach (n slices' largest do); the slices that reach it are read again and give a
+//   short list, in which every token counts those ahead of it and their weight.  Where a list cannot
+//   settle a top-p row, its border lies in one step, whose tokens are weighed by digits of their
+//   ordered keys; then the draw falls into one chunk of 8192, which is read again.
+// * What neither settles (a large top-k, a wide min-p, thousands of equal logits) takes passes over
+//   the whole row.
 #include "mtl_common.h"
 #include "mtl_paged.h"
 #include "mtl_sample.h"
@@ -20,23 +25,57 @@ namespace mtl {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kThreads = 1024;         // of a row, where it does not fit a smaller workgroup
+constexpr int kSmallThreads = 256;
+constexpr int kSmallVocab = 4096;
+constexpr int kChunk = 8192;            // tokens of a workgroup of the first two launches
+constexpr int kChunkThreads = 256;
 constexpr int kCandidates = 512;
 constexpr int kFew = 256;               // tokens that a list is made for
 constexpr int kBins = 2048;
 constexpr int kMaxSlices = 8192;
 constexpr int kMaxVocab = 1 << 20;
+constexpr int kMaxChunks = kMaxVocab / kChunk;
 constexpr int kMaxRows = 65535;
+
+constexpr int kSteps = 1024;
 
 struct SampleCall {
   const void* x;
   int64_t ld;
   int vocab, slice, slices, unit;       // unit: weights are counted in 2^-unit
+  int chunks;                           // 0: one launch does it all
+  int weighed;                          // rows that need the sum of their weights have it
   const float* u;
   mtl_sample_settings s;
   int64_t* token;
   float* logprob;
+  float* tops;                          // [rows][slices]
+  u64* sums;                            // [rows][chunks]
+  u64* steps;                           // [rows][chunks][kSteps]; null: no row can need them
+};
+
+// A row's settings.
+struct Settings {
+  float temperature, p, m;
+  int k;
+
+  __device__ __forceinline__ Settings(const SampleCall& c, int64_t r) {
+    const mtl_sample_settings& s = c.s;
+    temperature = s.temperature ? s.temperature[r] : s.temperature_all;
+    k = s.top_k ? s.top_k[r] : s.top_k_all;
+    p = s.top_p ? s.top_p[r] : s.top_p_all;
+    m = s.min_p ? s.min_p[r] : s.min_p_all;
+    k = k <= 0 || k > c.vocab ? c.vocab : k;
+  }
+  // The first of the order is all that stays.
+  __device__ __forceinline__ bool greedy() const {
+    return !(temperature > 0.f) || k == 1 || !(p > 0.f) || !(m <= 1.f);
+  }
+  __device__ __forceinline__ bool by_steps(int vocab) const { return k == vocab && p < 1.f; }
+  __device__ __forceinline__ bool weighed(int vocab) const {
+    return !greedy() && k == vocab && (p < 1.f || !(m > 0.f));
+  }
 };
 
 // ------------------------------------------------------------------------------ logits
@@ -97,23 +136,31 @@ struct Logits {
 struct Weight {
   float top;
   double by;                            // 1 / temperature
+  __device__ __forceinline__ Weight(float top, float temperature)
+      : top(top), by(1.0 / (double)fminf(temperature, 3.4028234663852886e38f)) {}
   __device__ __forceinline__ double operator()(float x) const {
     return x == top ? 1.0 : x == -__builtin_inff() ? 0.0 : exp(((double)x - (double)top) * by);
   }
 };
 
+// A weight (at most 1) in whole units of 2^-unit, unit <= 44: the sum with 2^52 rounds to them.
+__device__ __forceinline__ u64 whole_units(double w, int unit) {
+  const double one = __longlong_as_double((u64)(1023 + unit) << 52);
+  return (u64)__double_as_longlong(fma(w, one, 0x1p52)) - (u64)__double_as_longlong(0x1p52);
+}
+
 // Steps of the distance to the largest logit, 32 to an octave: the same or a later one for a
 // smaller logit.
-constexpr int kSteps = 1024;
+constexpr int kFirstStep = 117 * 32 - 1;
 __device__ __forceinline__ int step_of(float top, float x) {
   if (x == top) return 0;
-  const int s = (int)(__float_as_uint(top - x) >> 18) - (117 * 32 - 1);
+  const int s = (int)(__float_as_uint(top - x) >> 18) - kFirstStep;
   return min(max(s, 0), kSteps - 1);
 }
 
 // ------------------------------------------------------------------------------ workgroup steps
 // Inclusive sums over the workgroup in thread order, and their total; every thread takes part.
-template <class V>
+template <int WAVES, class V>
 __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
   const int lane = threadIdx.x & 63, wave = wave_id();
 #pragma unroll
@@ -126,7 +173,7 @@ __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
   __syncthreads();
   V before = 0, sum = 0;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < WAVES; ++i) {
     if (i == wave) before = sum;
     sum += part[i];
   }
@@ -134,13 +181,14 @@ __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
   return before + v;
 }
 
+template <int WAVES>
 __device__ __forceinline__ float block_max(float v, float* part) {
   v = wave_max_valu(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) part[wave_id()] = v;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) v = fmaxf(v, part[i]);
+  for (int i = 0; i < WAVES; ++i) v = fmaxf(v, part[i]);
   return v;
 }
 
@@ -157,18 +205,21 @@ struct Shared {
     } list;
   };
   union {
-    double d[kWaves];
-    u64 u[kWaves];
-    int i[kWaves];
-    float f[kWaves];
+    double d[kThreads / 64];
+    u64 u[kThreads / 64];
+    int i[kThreads / 64];
+    float f[kThreads / 64];
   } part;
+  u64 chunk[kMaxChunks];                // what stays of each chunk
+  int ties[kMaxChunks];
   int n, m, first;
   u64 above;
 };
 
 // ------------------------------------------------------------------------------ a row
-template <int T>
+template <int T, int THREADS>
 struct Draw {
+  static constexpr int WAVES = THREADS / 64;
   const SampleCall& c;
   const int64_t row;
   Shared& sh;
@@ -176,8 +227,13 @@ struct Draw {
   Weight weight;
   int k;
   double p, m, u;
+  bool weighed;
 
-  __device__ Draw(const SampleCall& c, int64_t row, Shared& sh) : c(c), row(row), sh(sh), x(c, row) {}
+  __device__ Draw(const SampleCall& c, int64_t row, Shared& sh, float top, const Settings& s,
+                  float u)
+      : c(c), row(row), sh(sh), x(c, row), weight(top, s.temperature), k(s.k), p(s.p), m(s.m),
+        u(u >= 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0),
+        weighed(c.weighed && s.weighed(c.vocab)) {}
 
   __device__ void result(int token, double logprob) {
     c.token[row] = token;
@@ -188,7 +244,7 @@ struct Draw {
   __device__ void greedy() {
     if (threadIdx.x == 0) sh.first = c.vocab;
     __syncthreads();
-    for (int s = threadIdx.x; s < c.slices; s += kThreads) {
+    for (int s = threadIdx.x; s < c.slices; s += THREADS) {
       if (sh.top[s] != weight.top) continue;
       for (int i = s * c.slice; i < min(c.vocab, (s + 1) * c.slice); ++i)
         if (x.at(i) == weight.top) {
@@ -200,24 +256,27 @@ struct Draw {
     if (threadIdx.x == 0) result(sh.first, 0.0);
   }
 
-  // Calls f(index, logit) for all tokens of the row, a thread's slices one after the other.
+  // Calls f(index, logit) for all tokens of the row.
   template <class F>
   __device__ __forceinline__ void all(F&& f) const {
-    for (int s = threadIdx.x; s < c.slices; s += kThreads)
-      for (int i = s * c.slice; i < (s + 1) * c.slice; i += 8) {
-        float v[8];
-        x.load(i, v);
+    for (int i = threadIdx.x * 8; i < c.vocab; i += THREADS * 8) {
+      float v[8];
+      x.load(i, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f(i + j, v[j]);
-      }
+      for (int j = 0; j < 8; ++j) f(i + j, v[j]);
+    }
   }
 
   // The sum of all weights.
   __device__ double total() {
-    double sum = 0, whole;
-    all([&](int, float v) { sum += weight(v); });
-    block_scan(sum, sh.part.d, whole);
-    return whole;
+    u64 sum = 0, whole;
+    if (weighed) {
+      for (int i = threadIdx.x; i < c.chunks; i += THREADS) sum += c.sums[row * c.chunks + i];
+    } else {
+      all([&](int, float v) { sum += whole_units(weight(v), c.unit); });
+    }
+    block_scan<WAVES>(sum, sh.part.u, whole);
+    return ldexp((double)whole, -c.unit);
   }
 
   // Draws from a list of candidates; false where a list cannot settle the row.
@@ -226,25 +285,35 @@ struct Draw {
     const int t = threadIdx.x;
     const bool k_set = k < c.vocab;
     const int want = k_set ? min(k, kFew) : kFew;
-    for (int i = t; i < kSteps; i += kThreads) l.steps[i] = 0;
+    for (int i = t; i < kSteps; i += THREADS) l.steps[i] = 0;
     if (t == 0) sh.n = sh.m = 0;
     __syncthreads();
     int finite = 0;
-    for (int s = t; s < c.slices; s += kThreads)
+    for (int s = t; s < c.slices; s += THREADS)
       if (sh.top[s] != -__builtin_inff()) {
         atomicAdd(&l.steps[step_of(weight.top, sh.top[s])], 1u);
         ++finite;
       }
     __syncthreads();
     // the first step that `want` slices reach, or the last
-    int slices;
-    const int upto = block_scan((int)l.steps[t], sh.part.i, slices);
+    constexpr int EACH = kSteps / THREADS;
+    int mine = 0, slices;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) mine += (int)l.steps[t * EACH + i];
+    int upto = block_scan<WAVES>(mine, sh.part.i, slices) - mine;
     if (t == 0) sh.first = kSteps - 1;
     __syncthreads();
-    if (upto >= want) atomicMin(&sh.first, t);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      upto += (int)l.steps[t * EACH + i];
+      if (upto >= want) {
+        atomicMin(&sh.first, t * EACH + i);
+        break;
+      }
+    }
     __syncthreads();
     const int last = sh.first;
-    for (int s = t; s < c.slices; s += kThreads)
+    for (int s = t; s < c.slices; s += THREADS)
       if (sh.top[s] != -__builtin_inff() && step_of(weight.top, sh.top[s]) <= last) {
         const int at = atomicAdd(&sh.m, 1);
         if (at < kCandidates) l.active[at] = s;
@@ -252,9 +321,9 @@ struct Draw {
     __syncthreads();
     const int active = sh.m;
     if (active > kCandidates) return false;
-    for (int i = t; i < active * c.slice; i += kThreads) {
+    for (int i = t; i < active * c.slice; i += THREADS) {
       const int e = l.active[i / c.slice] * c.slice + i % c.slice;
-      const float v = e < c.vocab ? x.at(e) : -__builtin_inff();
+      const float v = c.slice == 1 ? sh.top[e] : e < c.vocab ? x.at(e) : -__builtin_inff();
       if (v != -__builtin_inff() && step_of(weight.top, v) <= last) {
         const int at = atomicAdd(&sh.n, 1);
         if (at < kCandidates) {
@@ -267,94 +336,122 @@ struct Draw {
     const int n = sh.n;
     if (n > kCandidates) return false;
     // by index, so that sums have one order
-    if (t < n) {
+    for (int i = t; i < n; i += THREADS) {
       int to = 0;
-      const int mine = l.at[0][t];
+      const int mine = l.at[0][i];
       for (int j = 0; j < n; ++j) to += l.at[0][j] < mine;
-      l.x[1][to] = l.x[0][t];
+      l.x[1][to] = l.x[0][i];
       l.at[1][to] = mine;
-      l.w[to] = weight(l.x[0][t]);
+      l.w[to] = weight(l.x[0][i]);
     }
     __syncthreads();
-    int rank = 0;
-    double before = 0, w = 0;
-    float v = 0;
-    if (t < n) {
-      v = l.x[1][t];
-      w = l.w[t];
+    constexpr int ROUNDS = (kCandidates + THREADS - 1) / THREADS;   // a thread's, side by side
+    int rank[ROUNDS];
+    double before[ROUNDS], w[ROUNDS], in_k = 0, mass;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int i = t * ROUNDS + r;
+      rank[r] = 0;
+      before[r] = w[r] = 0;
+      if (i >= n) continue;
+      const float v = l.x[1][i];
+      w[r] = l.w[i];
       for (int j = 0; j < n; ++j) {
         const float y = l.x[1][j];
-        if (y > v || (y == v && j < t)) {
-          ++rank;
-          before += l.w[j];
+        if (y > v || (y == v && j < i)) {
+          ++rank[r];
+          before[r] += l.w[j];
         }
       }
+      if (rank[r] < k) in_k += w[r];
     }
-    double mass;
-    const bool in_k = t < n && rank < k;
-    block_scan(in_k ? w : 0.0, sh.part.d, mass);
+    block_scan<WAVES>(in_k, sh.part.d, mass);
     if (last < kSteps - 1 && !(k_set && k <= n)) {    // tokens outside the list may count
       if (k_set) return false;
-      int low;
-      block_scan((int)(t < n && !(w >= m)), sh.part.i, low);
-      if (!low && p >= 1) return false;
+      int low = 0, any;
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) low |= t * ROUNDS + r < n && !(w[r] >= m);
+      block_scan<WAVES>(low, sh.part.i, any);
+      if (!any && p >= 1) return false;
       const double whole = p < 1 ? total() : 0.0;
-      if (!low && !(mass > p * whole)) return false;
+      if (!any && !(mass > p * whole)) return false;
       mass = whole;
     }
-    const bool keep = in_k && (p >= 1 || before <= p * mass) && (w >= m || rank == 0);
-    double whole;
-    const double upto_w = block_scan(keep ? w : 0.0, sh.part.d, whole);
+    bool keep[ROUNDS];
+    double kept = 0, whole;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      keep[r] = t * ROUNDS + r < n && rank[r] < k && (p >= 1 || before[r] <= p * mass) &&
+                (w[r] >= m || rank[r] == 0) && w[r] > 0;
+      kept += keep[r] ? w[r] : 0.0;
+    }
+    double upto_w = block_scan<WAVES>(kept, sh.part.d, whole) - kept;
     if (t == 0) {
       sh.first = kCandidates;
       sh.m = -1;
     }
     __syncthreads();
-    if (keep && w > 0) {
-      atomicMax(&sh.m, t);                            // the last one, where rounding leaves none
-      if (upto_w > u * whole) atomicMin(&sh.first, t);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      if (!keep[r]) continue;
+      upto_w += w[r];
+      atomicMax(&sh.m, t * ROUNDS + r);               // the last one, where rounding leaves none
+      if (upto_w > u * whole) atomicMin(&sh.first, t * ROUNDS + r);
     }
     __syncthreads();
-    if (t == min(sh.first, sh.m)) result(l.at[1][t], log(w / whole));
+    const int pick = min(sh.first, sh.m);
+    if (t == 0) result(l.at[1][pick], log(l.w[pick] / whole));
     return true;
   }
 
-  // A border in the order of keys: the key at which `limit` is passed, going down from the largest,
-  // and what lies above it.  WEIGH: weights in units of 2^-unit, else tokens.
-  template <bool WEIGH>
-  __device__ void border(uint32_t lo, u64 limit, uint32_t& key, u64& above) {
-    uint32_t hi = x.key(weight.top);
-    above = 0;
+  // A border in the order of keys from `lo` to `hi`: the key at which `limit` is passed, going down,
+  // and what lies above it (`above` at first lies above hi).  each(f) calls f(logit) for all tokens
+  // in question.  WEIGH: weights in units of 2^-unit, else tokens.
+  template <bool WEIGH, class Each>
+  __device__ void border(Each&& each, uint32_t lo, uint32_t hi, u64 limit, uint32_t& key,
+                         u64& above) {
+    constexpr int EACH = kBins / THREADS;
     while (true) {
       const uint32_t range = hi - lo;
       const int shift = range < kBins ? 0 : 21 - __builtin_clz(range);
       const int bins = (int)(range >> shift) + 1;
       __syncthreads();
-      for (int i = threadIdx.x; i < kBins; i += kThreads) sh.sums[i] = 0;
+      for (int i = threadIdx.x; i < kBins; i += THREADS) sh.sums[i] = 0;
       if (threadIdx.x == 0) {
         sh.first = kBins;
         sh.m = -1;
       }
       __syncthreads();
-      all([&](int, float v) {
+      each([&](float v) {
         const uint32_t b = x.key(v);
         if (v != -__builtin_inff() && b >= lo && b <= hi)
-          atomicAdd(&sh.sums[(b - lo) >> shift],
-                    WEIGH ? (u64)rint(ldexp(weight(v), c.unit)) : (u64)1);
+          atomicAdd(&sh.sums[(b - lo) >> shift], WEIGH ? whole_units(weight(v), c.unit) : (u64)1);
       });
       __syncthreads();
-      const int j = 2 * threadIdx.x;                  // bins from the largest key down
-      const u64 a = j < bins ? sh.sums[bins - 1 - j] : 0;
-      const u64 b = j + 1 < bins ? sh.sums[bins - 2 - j] : 0;
-      u64 all_of;
-      const u64 upto = block_scan(a + b, sh.part.u, all_of), ahead = above + upto - a - b;
-      const bool at_a = WEIGH ? ahead + a > limit : ahead + a >= limit;
-      const bool at_b = WEIGH ? ahead + a + b > limit : ahead + a + b >= limit;
-      if (at_a || at_b) atomicMin(&sh.first, at_a ? j : j + 1);
-      if (a || b) atomicMax(&sh.m, b ? j + 1 : j);
+      const int j0 = EACH * threadIdx.x;              // bins from the largest key down
+      u64 mine = 0, all_of;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) mine += j0 + i < bins ? sh.sums[bins - 1 - j0 - i] : 0;
+      u64 ahead = above + block_scan<WAVES>(mine, sh.part.u, all_of) - mine;
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const u64 here = j0 + i < bins ? sh.sums[bins - 1 - j0 - i] : 0;
+        if (here) atomicMax(&sh.m, j0 + i);
+        if (!found && (WEIGH ? ahead + here > limit : ahead + here >= limit)) {
+          found = true;
+          atomicMin(&sh.first, j0 + i);
+        }
+        ahead += here;
+      }
       __syncthreads();
       const int pick = min(sh.first, max(sh.m, 0));
-      if (pick == j || pick == j + 1) sh.above = pick == j ? ahead : ahead + a;
+      ahead -= mine;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        if (pick == j0 + i) sh.above = ahead;
+        ahead += j0 + i < bins ? sh.sums[bins - 1 - j0 - i] : 0;
+      }
       __syncthreads();
       above = sh.above;
       lo += (uint32_t)(bins - 1 - pick) << shift;
@@ -364,38 +461,45 @@ struct Draw {
     key = lo;
   }
 
+  // How many tokens of weight w stay behind a weight of `above` under `limit`.
+  __device__ __forceinline__ int that_stay(double limit, u64 above, double w) const {
+    const double room = (limit - ldexp((double)above, -c.unit)) / w;
+    return room < (double)c.vocab ? max((int)floor(room) + 1, 1) : c.vocab;
+  }
+
   // Draws by passes over the row.
   __device__ void by_passes() {
-    uint32_t key = x.key(-__builtin_inff()) + 1, at;
+    auto row_of = [&](auto&& f) { all([&](int, float v) { f(v); }); };
+    const uint32_t low = x.key(-__builtin_inff()) + 1, high = x.key(weight.top);
+    uint32_t key = low, at;
     int ties = c.vocab;                               // of that key, how many stay
-    u64 above;
     if (k < c.vocab) {
-      border<false>(key, (u64)k, at, above);
+      u64 above = 0;
+      border<false>(row_of, low, high, (u64)k, at, above);
       key = at;
       ties = k - (int)above;
     }
     if (p < 1) {
       // the weight of what top-k left
-      double sum = 0, mass;
+      u64 sum = 0, whole, above = 0;
       int same = 0, all_same;
       all([&](int, float v) {
-        if (x.key(v) > key) sum += weight(v);
-        same += x.key(v) == key && v != -__builtin_inff();
+        if (v == -__builtin_inff()) return;
+        if (x.key(v) > key) sum += whole_units(weight(v), c.unit);
+        same += x.key(v) == key;
       });
-      block_scan(sum, sh.part.d, mass);
-      block_scan(same, sh.part.i, all_same);
-      mass += (double)min(ties, all_same) * weight(x.of_key(key));
-      border<true>(key, (u64)ldexp(p * mass, c.unit), at, above);
-      const double w = weight(x.of_key(at));
-      const double room = (p * mass - ldexp((double)above, -c.unit)) / w;
-      const int stay = room < (double)c.vocab ? max((int)floor(room) + 1, 1) : c.vocab;
+      block_scan<WAVES>(sum, sh.part.u, whole);
+      block_scan<WAVES>(same, sh.part.i, all_same);
+      const double limit = p * (ldexp((double)whole, -c.unit) +
+                                (double)min(ties, all_same) * weight(x.of_key(key)));
+      border<true>(row_of, low, high, (u64)ldexp(limit, c.unit), at, above);
+      const int stay = that_stay(limit, above, weight(x.of_key(at)));
       ties = at == key ? min(ties, stay) : stay;
       key = at;
     }
     // by index: each thread a run of slices
-    const int per = (c.slices + kThreads - 1) / kThreads;
-    const int begin = min(c.vocab, (int)threadIdx.x * per * c.slice);
-    const int end = min(c.vocab, begin + per * c.slice);
+    const int per = (c.slices + THREADS - 1) / THREADS * c.slice;
+    const int begin = min(c.vocab, (int)threadIdx.x * per), end = min(c.vocab, begin + per);
     const double wk = weight(x.of_key(key));
     double sum = 0;
     int same = 0;
@@ -414,23 +518,12 @@ struct Draw {
       }
     }
     int all_same;
-    const int had = block_scan(same, sh.part.i, all_same) - same;
-    const bool tie_stays = wk >= m || x.of_key(key) == weight.top;
-    if (tie_stays) sum += (double)min(max(ties - had, 0), same) * wk;
+    const int had = block_scan<WAVES>(same, sh.part.i, all_same) - same;
+    if (wk >= m || x.of_key(key) == weight.top) sum += (double)min(max(ties - had, 0), same) * wk;
     double whole;
-    const double upto = block_scan(sum, sh.part.d, whole);
+    const double upto = block_scan<WAVES>(sum, sh.part.d, whole);
     const double goal = u * whole;
-    if (threadIdx.x == 0) {
-      sh.first = kThreads;
-      sh.m = -1;
-    }
-    __syncthreads();
-    if (sum > 0) {
-      atomicMax(&sh.m, (int)threadIdx.x);
-      if (upto > goal) atomicMin(&sh.first, (int)threadIdx.x);
-    }
-    __syncthreads();
-    if ((int)threadIdx.x != min(sh.first, sh.m)) return;
+    if (!mine_is_it(sum > 0, upto > goal)) return;
     // within the run that the draw falls into
     double run = upto - sum, w_last = 0;
     int last = -1, seen = had;
@@ -448,46 +541,313 @@ struct Draw {
     }
     result(last, log(w_last / whole));
   }
+
+  // The first thread that passes the goal, or, where rounding leaves none, the last with something.
+  __device__ __forceinline__ bool mine_is_it(bool some, bool passes) {
+    if (threadIdx.x == 0) {
+      sh.first = THREADS;
+      sh.m = -1;
+    }
+    __syncthreads();
+    if (some) {
+      atomicMax(&sh.m, (int)threadIdx.x);
+      if (passes) atomicMin(&sh.first, (int)threadIdx.x);
+    }
+    __syncthreads();
+    return (int)threadIdx.x == min(sh.first, sh.m);
+  }
+
+  // Draws from a weighed row: top-p alone, or no filter.  False where min-p cuts deeper.
+  __device__ bool by_chunks() {
+    uint32_t key = x.key(-__builtin_inff()) + 1;
+    int ties = c.vocab;
+    const u64* sums = c.sums + row * c.chunks;
+    u64 mine = (int)threadIdx.x < c.chunks ? sums[threadIdx.x] : 0, whole;
+    block_scan<WAVES>(mine, sh.part.u, whole);
+    if (p < 1) {
+      // the step of the border, of all chunks together
+      static_assert(kSteps % THREADS == 0, "a thread's steps");
+      constexpr int EACH = kSteps / THREADS;
+      const u64* steps = c.steps + row * c.chunks * kSteps;
+      const double limit = p * ldexp((double)whole, -c.unit);
+      const u64 limit_units = (u64)ldexp(limit, c.unit);
+      u64 of[EACH] = {}, sum = 0, total;
+      for (int i = 0; i < c.chunks; ++i)
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) of[e] += steps[i * kSteps + threadIdx.x * EACH + e];
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) sum += of[e];
+      u64 ahead = block_scan<WAVES>(sum, sh.part.u, total) - sum;
+      if (threadIdx.x == 0) {
+        sh.first = kSteps - 1;
+        sh.above = 0;
+      }
+      __syncthreads();
+      bool found = false;
+      const u64 ahead0 = ahead;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        if (!found && ahead + of[e] > limit_units) {
+          found = true;
+          atomicMin(&sh.first, (int)threadIdx.x * EACH + e);
+        }
+        ahead += of[e];
+      }
+      __syncthreads();
+      const int step = sh.first;
+      ahead = ahead0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        if (step == (int)threadIdx.x * EACH + e) sh.above = ahead;
+        ahead += of[e];
+      }
+      __syncthreads();
+      u64 above = sh.above;
+      // its tokens lie in slices that reach it, and between two keys (two off for rounding)
+      auto in_step = [&](auto&& f) {
+        for (int s = threadIdx.x / 4; s < c.slices; s += THREADS / 4) {
+          if (step_of(weight.top, sh.top[s]) > step) continue;
+          for (int i = (threadIdx.x & 3) * 8; i < c.slice; i += 32) {
+            float v[8];
+            x.load(s * c.slice + i, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (step_of(weight.top, v[j]) == step) f(s * c.slice + i + j, v[j]);
+          }
+        }
+      };
+      const float far = step == kSteps - 1 ? __builtin_inff()
+                                           : __uint_as_float((uint32_t)(step + 1 + kFirstStep) << 18);
+      const float near = step == 0 ? 0.f : __uint_as_float((uint32_t)(step + kFirstStep) << 18);
+      const uint32_t low = key, high = x.key(weight.top);
+      const uint32_t lo = max(x.key(weight.top - far), low + 2) - 2;
+      border<true>([&](auto&& f) { in_step([&](int, float v) { f(v); }); }, lo,
+                   min(x.key(weight.top - near) + 2, high), limit_units, key, above);
+      const double wk = weight(x.of_key(key));
+      if (!(wk >= m)) return false;
+      ties = that_stay(limit, above, wk);
+      // what stays of each chunk
+      __syncthreads();
+      for (int i = threadIdx.x; i < c.chunks; i += THREADS) {
+        sh.chunk[i] = 0;
+        sh.ties[i] = 0;
+      }
+      __syncthreads();
+      in_step([&](int i, float v) {
+        if (v == -__builtin_inff()) return;
+        const uint32_t b = x.key(v);
+        if (b > key) atomicAdd(&sh.chunk[i / kChunk], whole_units(weight(v), c.unit));
+        if (b == key) atomicAdd(&sh.ties[i / kChunk], 1);
+      });
+      for (int i = wave_id(); i < c.chunks; i += WAVES) {       // its earlier steps
+        u64 v = 0;
+        for (int e = threadIdx.x & 63; e < step; e += 64) v += steps[i * kSteps + e];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.chunk[i], v);
+      }
+      __syncthreads();
+      int has = (int)threadIdx.x < c.chunks ? sh.ties[threadIdx.x] : 0, all_has;
+      const int had = block_scan<WAVES>(has, sh.part.i, all_has) - has;
+      mine = 0;
+      if ((int)threadIdx.x < c.chunks) {
+        mine = sh.chunk[threadIdx.x] +
+               (u64)min(max(ties - had, 0), has) * whole_units(wk, c.unit);
+        sh.ties[threadIdx.x] = had;
+      }
+    } else if ((int)threadIdx.x < c.chunks) {
+      sh.ties[threadIdx.x] = 0;
+    }
+    u64 upto = block_scan<WAVES>(mine, sh.part.u, whole);
+    const u64 goal = (u64)(u * (double)whole);
+    if (mine_is_it(mine > 0, upto > goal)) {
+      sh.n = threadIdx.x;
+      sh.above = upto - mine;
+    }
+    __syncthreads();
+    // the draw falls into chunk sh.n, a thread 8 tokens of it
+    static_assert(kChunk <= 8 * kThreads, "a thread's tokens");
+    constexpr int EACH = kChunk / THREADS;
+    const int chunk = sh.n, begin = chunk * kChunk + threadIdx.x * EACH;
+    u64 w[EACH], sum = 0;
+    int tied = 0, same = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i += 8) {
+      float v[8];
+      x.load(min(begin + i, c.vocab), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool there = begin + i + j < c.vocab && v[j] != -__builtin_inff();
+        const uint32_t b = x.key(v[j]);
+        w[i + j] = there && b >= key ? whole_units(weight(v[j]), c.unit) : 0;
+        if (there && b == key) {
+          tied |= 1 << (i + j);
+          ++same;
+        }
+      }
+    }
+    int all_same;
+    int left = ties - sh.ties[chunk] - (block_scan<WAVES>(same, sh.part.i, all_same) - same);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (tied >> i & 1 && left-- <= 0) w[i] = 0;
+      sum += w[i];
+    }
+    const u64 before = sh.above;
+    u64 chunk_whole;
+    upto = before + block_scan<WAVES>(sum, sh.part.u, chunk_whole);
+    if (!mine_is_it(sum > 0, upto > goal)) return true;
+    u64 run = upto - sum;
+    int last = -1;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (w[i] && run <= goal) {
+        run += w[i];
+        last = begin + i;
+      }
+    // the weight itself, not in whole units: it may be small
+    result(last, log(weight(x.at(last)) / ldexp((double)whole, -c.unit)));
+    return true;
+  }
 };
 
+// The largest logit of each slice.
 template <int T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleCall c) {
-  __shared__ Shared sh;
-  Draw<T> d(c, blockIdx.x, sh);
-  const mtl_sample_settings& s = c.s;
-  const int64_t r = d.row;
-  const float temperature = s.temperature ? s.temperature[r] : s.temperature_all;
-  const int k = s.top_k ? s.top_k[r] : s.top_k_all;
-  const float p = s.top_p ? s.top_p[r] : s.top_p_all, m = s.min_p ? s.min_p[r] : s.min_p_all;
-  const float u = c.u[r];
-  float top = -__builtin_inff();
-  for (int i = threadIdx.x; i < c.slices; i += kThreads) {
-    float best = -__builtin_inff();
-    for (int e = i * c.slice; e < (i + 1) * c.slice; e += 8) {
-      float v[8];
-      d.x.load(e, v);
+__global__ void __launch_bounds__(kChunkThreads) sample_tops_kernel(SampleCall c) {
+  const int64_t row = blockIdx.y;
+  const Logits<T> x(c, row);
+  const int lanes = c.slice / 8;                      // of a slice: 4 or 16
+  float v[kChunk / kChunkThreads / 8][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) best = fmaxf(best, v[j]);
-    }
-    sh.top[i] = best;
-    top = fmaxf(top, best);
+  for (int i = 0; i < kChunk / kChunkThreads / 8; ++i) {
+    const int at = blockIdx.x * kChunk + (i * kChunkThreads + (int)threadIdx.x) * 8;
+    x.load(min(at, c.vocab), v[i]);
   }
-  top = block_max(top, sh.part.f);
-  d.weight.top = top;
-  d.weight.by = 1.0 / (double)fminf(temperature, 3.4028234663852886e38f);
-  d.k = k <= 0 || k > c.vocab ? c.vocab : k;
-  d.p = p;
-  d.m = m;
-  d.u = u >= 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
+#pragma unroll
+  for (int i = 0; i < kChunk / kChunkThreads / 8; ++i) {
+    const int at = blockIdx.x * kChunk + (i * kChunkThreads + (int)threadIdx.x) * 8;
+    float best = v[i][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) best = fmaxf(best, v[i][j]);
+    best = fmaxf(best, dpp_f32<kDppXor1>(best));
+    best = fmaxf(best, dpp_f32<kDppXor2>(best));
+    if (lanes == 16) {
+      best = fmaxf(best, dpp_f32<kDppHalfMirror>(best));
+      best = fmaxf(best, dpp_f32<kDppMirror>(best));
+    }
+    if (at < c.vocab && threadIdx.x % lanes == 0) c.tops[row * c.slices + at / c.slice] = best;
+  }
+}
+
+// Each chunk's weights, and by steps, of rows that need them.
+template <int T>
+__global__ void __launch_bounds__(kChunkThreads) sample_weights_kernel(SampleCall c) {
+  constexpr int WAVES = kChunkThreads / 64;
+  __shared__ u64 steps[kSteps];
+  __shared__ union {
+    float f[WAVES];
+    u64 u[WAVES];
+  } part;
+  const int64_t row = blockIdx.y;
+  const Settings s(c, row);
+  if (!s.weighed(c.vocab)) return;
+  const bool by_steps = s.by_steps(c.vocab);
+  const Logits<T> x(c, row);
+  float v[kChunk / kChunkThreads / 8][8];
+#pragma unroll
+  for (int i = 0; i < kChunk / kChunkThreads / 8; ++i) {
+    const int at = blockIdx.x * kChunk + (i * kChunkThreads + (int)threadIdx.x) * 8;
+    x.load(min(at, c.vocab), v[i]);
+  }
+  float top = -__builtin_inff();
+  for (int i = threadIdx.x; i < c.slices; i += kChunkThreads)
+    top = fmaxf(top, c.tops[row * c.slices + i]);
+  top = block_max<WAVES>(top, part.f);
+  if (by_steps)
+    for (int i = threadIdx.x; i < kSteps; i += kChunkThreads) steps[i] = 0;
+  __syncthreads();
+  const Weight weight(top, s.temperature);
+  // Less than this part of the whole lies behind the border whatever the rest is: all such tokens
+  // together weigh less than half of 1 - p, and the whole at least 1.
+  const u64 least = (u64)ldexp(fmax(1.0 - (double)s.p, 0.0) / (2.0 * c.vocab), c.unit);
+  u64 sum = 0;
+#pragma unroll
+  for (int i = 0; i < kChunk / kChunkThreads / 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const u64 w = whole_units(weight(v[i][j]), c.unit);
+      sum += w;
+      if (by_steps && w > least) atomicAdd(&steps[step_of(top, v[i][j])], w);
+    }
+  u64 whole;
+  block_scan<WAVES>(sum, part.u, whole);
+  if (threadIdx.x == 0) c.sums[row * c.chunks + blockIdx.x] = whole;
+  if (!by_steps) return;
+  __syncthreads();
+  u64* to = c.steps + (row * c.chunks + blockIdx.x) * kSteps;
+  for (int i = threadIdx.x; i < kSteps; i += kChunkThreads) to[i] = steps[i];
+}
+
+template <int T, int THREADS>
+__global__ void __launch_bounds__(THREADS) sample_kernel(SampleCall c) {
+  __shared__ Shared sh;
+  const int64_t row = blockIdx.x;
+  const Settings s(c, row);
+  const float u = c.u[row];
+  const Logits<T> x(c, row);
+  float top = -__builtin_inff();
+  if (c.slice == 1) {
+    for (int i = threadIdx.x; i < c.vocab; i += THREADS) top = fmaxf(top, sh.top[i] = x.at(i));
+  } else {
+    for (int i = threadIdx.x; i < c.slices; i += THREADS)
+      top = fmaxf(top, sh.top[i] = c.tops[row * c.slices + i]);
+  }
+  top = block_max<THREADS / 64>(top, sh.part.f);
+  Draw<T, THREADS> d(c, row, sh, top, s, u);
   if (top == -__builtin_inff()) {
     if (threadIdx.x == 0) d.result(-1, -__builtin_inff());
     return;
   }
-  // settings that leave the first of the order alone
-  if (!(temperature > 0.f) || k == 1 || !(p > 0.f) || !(m <= 1.f)) return d.greedy();
-  if ((d.k < c.vocab || p < 1.f || m > 0.f) && d.by_list()) return;
+  if (s.greedy()) return d.greedy();
+  if ((s.k < c.vocab || s.p < 1.f || s.m > 0.f) && d.by_list()) return;
+  __syncthreads();
+  if (THREADS == kThreads && d.weighed && d.by_chunks()) return;
   __syncthreads();
   d.by_passes();
+}
+
+// What a call needs besides the last launch.
+struct SamplePlan {
+  int slice, chunks;
+  bool weighed, steps;
+  int64_t slices, steps_bytes, sums_bytes, bytes;
+};
+
+static SamplePlan sample_plan(int64_t rows, int64_t vocab, const mtl_sample_settings& s) {
+  SamplePlan p{};
+  p.slice = vocab <= kMaxSlices ? 1 : vocab <= 32 * kMaxSlices ? 32 : 128;
+  p.slices = (vocab + p.slice - 1) / p.slice;
+  if (p.slice == 1) return p;
+  p.chunks = (int)((vocab + kChunk - 1) / kChunk);
+  const bool k_open = s.top_k || s.top_k_all <= 0 || s.top_k_all >= vocab;
+  const bool draws = s.temperature || s.temperature_all > 0.f;
+  p.steps = k_open && draws && (s.top_p || (s.top_p_all < 1.f && s.top_p_all > 0.f));
+  p.weighed = p.steps || (k_open && draws && (s.min_p || !(s.min_p_all > 0.f)));
+  p.steps_bytes = p.steps ? rows * p.chunks * kSteps * 8 : 0;
+  p.sums_bytes = p.weighed ? rows * p.chunks * 8 : 0;
+  p.bytes = p.steps_bytes + p.sums_bytes + rows * p.slices * 4;
+  return p;
+}
+
+template <int T>
+static void launch_sample(const SampleCall& c, int64_t rows, hipStream_t stream) {
+  const dim3 grid(c.chunks, (unsigned)rows);
+  if (c.chunks) sample_tops_kernel<T><<<grid, kChunkThreads, 0, stream>>>(c);
+  if (c.weighed) sample_weights_kernel<T><<<grid, kChunkThreads, 0, stream>>>(c);
+  if (c.vocab <= kSmallVocab)
+    sample_kernel<T, kSmallThreads><<<(unsigned)rows, kSmallThreads, 0, stream>>>(c);
+  else
+    sample_kernel<T, kThreads><<<(unsigned)rows, kThreads, 0, stream>>>(c);
 }
 
 }  // namespace mtl
@@ -496,14 +856,14 @@ using namespace mtl;
 
 extern "C" int64_t mtl_sample_workspace_bytes(int64_t rows, int64_t vocab, int32_t type,
                                               const mtl_sample_settings* settings) {
-  (void)rows, (void)vocab, (void)type, (void)settings;
-  return 0;
+  (void)type;
+  if (!settings || rows < 1 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab) return 0;
+  return sample_plan(rows, vocab, *settings).bytes;
 }
 
 extern "C" int mtl_sample(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int32_t type,
                           const float* u, const mtl_sample_settings* settings, int64_t* token,
                           float* logprob, void* workspace, int64_t ws_bytes, void* stream) {
-  (void)workspace, (void)ws_bytes;
   if (!settings || rows < 0 || vocab < 1 || ld < 0) return MTL_ERR_INVALID_ARG;
   if (type != MTL_T_BF16 && type != MTL_T_F16 && type != MTL_T_F32) return MTL_ERR_UNSUPPORTED;
   if (vocab > kMaxVocab || rows > kMaxRows) return MTL_ERR_SHAPE;
@@ -511,14 +871,20 @@ extern "C" int mtl_sample(const void* logits, int64_t ld, int64_t rows, int64_t 
   if (!logits || !u || !token) return MTL_ERR_INVALID_ARG;
   const int size = type == MTL_T_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % size) return MTL_ERR_ALIGN;
+  const SamplePlan p = sample_plan(rows, vocab, *settings);
+  if (p.bytes > 0 && (!workspace || ws_bytes < p.bytes)) return MTL_ERR_WORKSPACE;
+  if (p.bytes > 0 && !aligned16(workspace)) return MTL_ERR_ALIGN;
   int unit = 44;
   while (unit > 0 && (vocab >> (62 - unit)) > 0) --unit;
-  const int slice = vocab <= 8 * kThreads ? 8 : vocab <= 32 * kMaxSlices ? 32 : 128;
-  const SampleCall c{logits, ld, (int)vocab, slice, (int)((vocab + slice - 1) / slice), unit, u,
-                     *settings, token, logprob};
+  char* ws = static_cast<char*>(workspace);
+  const SampleCall c{logits, ld, (int)vocab, p.slice, (int)p.slices, unit, p.chunks, p.weighed, u,
+                     *settings, token, logprob,
+                     reinterpret_cast<float*>(ws + p.steps_bytes + p.sums_bytes),
+                     reinterpret_cast<u64*>(ws + p.steps_bytes),
+                     p.steps ? reinterpret_cast<u64*>(ws) : nullptr};
   hipStream_t st = (hipStream_t)stream;
-  if (type == MTL_T_BF16) sample_kernel<MTL_T_BF16><<<(unsigned)rows, kThreads, 0, st>>>(c);
-  else if (type == MTL_T_F16) sample_kernel<MTL_T_F16><<<(unsigned)rows, kThreads, 0, st>>>(c);
-  else sample_kernel<MTL_T_F32><<<(unsigned)rows, kThreads, 0, st>>>(c);
+  if (type == MTL_T_BF16) launch_sample<MTL_T_BF16>(c, rows, st);
+  else if (type == MTL_T_F16) launch_sample<MTL_T_F16>(c, rows, st);
+  else launch_sample<MTL_T_F32>(c, rows, st);
   return launch_status();
 }

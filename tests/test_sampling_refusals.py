@@ -32,6 +32,23 @@ def test_c_refusals():
         assert call(**kw) == want, kw
 
 
+def test_workspace():
+    bytes_of = N.load().mtl_sample_workspace_bytes
+    for kw in (dict(), dict(top_p_all=0.9), dict(top_k_all=50), dict(top_k=FAKE)):
+        s = N.SampleSettings(**{**dict(temperature_all=1.0, top_p_all=1.0), **kw})
+        assert bytes_of(2, 8192, N.T_F32, ctypes.byref(s)) == 0     # one launch does it
+        need = bytes_of(2, 9000, N.T_F32, ctypes.byref(s))
+        assert need > 0
+
+        def run(ws, nbytes):
+            return N.load().mtl_sample(FAKE, 9000, 2, 9000, N.T_F32, FAKE, ctypes.byref(s), FAKE,
+                                       None, ws, nbytes, None)
+
+        assert run(FAKE, need - 1) == N.MTL_ERR_WORKSPACE and run(None, need) == N.MTL_ERR_WORKSPACE
+        assert run(FAKE + 8, need) == N.MTL_ERR_ALIGN
+    assert bytes_of(2, 9000, N.T_F32, None) == 0 and bytes_of(0, 9000, N.T_F32, ctypes.byref(s)) == 0
+
+
 @pytest.mark.parametrize("kw,what", [
     (dict(logits=meta(1000)), "rows, vocab"), (dict(logits=meta(3, 0)), "2\\^20"),
     (dict(logits=meta(3, (1 << 20) + 1)), "2\\^20"), (dict(logits=meta(65536, 8), u=meta(65536)), "rows"),
