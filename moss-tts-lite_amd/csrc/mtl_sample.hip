@@ -9,7 +9,7 @@
 //   up to kMaxSlices tokens need none: they fit LDS).
 // * Rows that need the sum of all weights (top-p without a small top-k; no filter) are weighed in a
 //   second launch: a sum for each 8192 tokens, and for top-p by the logits' distance to the
-//   largest, in steps of 1/32 octave.
+//   largest, in steps of 1/128 octave.
 // * In the last launch a workgroup takes a row.  The slices' largest logits give a bound that at
 //   least n tokens reach (n slices' largest do); the slices that reach it are read again and give a
 //   short list, in which every token counts those ahead of it and their weight.  Where a list cannot
@@ -25,13 +25,12 @@ namespace mtl {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;         // of a row, where it does not fit a smaller workgroup
-constexpr int kSmallThreads = 256;
-constexpr int kSmallVocab = 4096;
+constexpr int kThreads = 512;          // of a row
+constexpr int kWaves = kThreads / 64;
 constexpr int kChunk = 8192;            // tokens of a workgroup of the first two launches
 constexpr int kChunkThreads = 256;
-constexpr int kCandidates = 512;
-constexpr int kFew = 256;               // tokens that a list is made for
+constexpr int kCandidates = kThreads;
+constexpr int kFew = 256, kFewer = 64;  // tokens that a list is made for
 constexpr int kBins = 2048;
 constexpr int kMaxSlices = 8192;
 constexpr int kMaxVocab = 1 << 20;
@@ -122,10 +121,16 @@ struct Logits {
     }
   }
 
-  // Whole numbers in the logits' order, without the bits that the type does not have.
-  static __device__ __forceinline__ uint32_t key(float x) {
+  // Whole numbers in the logits' order; key: without the bits that the type does not have.
+  static __device__ __forceinline__ uint32_t order(float x) {
     const uint32_t b = __float_as_uint(x);
-    return (b & 0x80000000u ? ~b : b | 0x80000000u) >> kDrop;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+  }
+  static __device__ __forceinline__ uint32_t key(float x) {
+    return order(x) >> kDrop;
+  }
+  static __device__ __forceinline__ float of_order(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
   }
   static __device__ __forceinline__ float of_key(uint32_t k) {
     k = k << kDrop;
@@ -133,13 +138,30 @@ struct Logits {
   }
 };
 
+// 2^t for t <= 0, to some 2^-50 of itself (0 far below): the whole part into the exponent, 2^f =
+// e^(f ln 2) for the rest, |f| <= 1/2, by its series (the 14th term is below 2^-54).  The library's
+// function takes four times as long, which is what weighing a row costs.
+__device__ __forceinline__ double power_of_two(double t) {
+  const double n = rint(t), r = (t - n) * 0x1.62e42fefa39efp-1;
+  double e = 1.0 / 6227020800.0;
+  constexpr double kTerms[13] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720,
+                                 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800,
+                                 1.0 / 39916800, 1.0 / 479001600};
+#pragma unroll
+  for (int i = 12; i >= 0; --i) e = fma(e, r, kTerms[i]);
+  const int whole = (int)fmax(n, -1000.0);
+  return __longlong_as_double(__double_as_longlong(e) + ((long long)whole << 52));
+}
+
 struct Weight {
   float top;
-  double by;                            // 1 / temperature
+  double by;                            // log2(e) / temperature
   __device__ __forceinline__ Weight(float top, float temperature)
-      : top(top), by(1.0 / (double)fminf(temperature, 3.4028234663852886e38f)) {}
+      : top(top),
+        by(0x1.71547652b82fep+0 / (double)fminf(temperature, 3.4028234663852886e38f)) {}
   __device__ __forceinline__ double operator()(float x) const {
-    return x == top ? 1.0 : x == -__builtin_inff() ? 0.0 : exp(((double)x - (double)top) * by);
+    const double w = power_of_two(fmax(((double)x - (double)top) * by, -2000.0));
+    return x == top ? 1.0 : w;
   }
 };
 
@@ -149,32 +171,49 @@ __device__ __forceinline__ u64 whole_units(double w, int unit) {
   return (u64)__double_as_longlong(fma(w, one, 0x1p52)) - (u64)__double_as_longlong(0x1p52);
 }
 
-// Steps of the distance to the largest logit, 32 to an octave: the same or a later one for a
-// smaller logit.
-constexpr int kFirstStep = 117 * 32 - 1;
+// Steps of the distance to the largest logit, 128 to an octave from 1/4 to 64: the same or a later
+// one for a smaller logit.
+constexpr int kFirstStep = 125 * 128 - 1;
 __device__ __forceinline__ int step_of(float top, float x) {
   if (x == top) return 0;
-  const int s = (int)(__float_as_uint(top - x) >> 18) - kFirstStep;
+  const int s = (int)(__float_as_uint(top - x) >> 16) - kFirstStep;
   return min(max(s, 0), kSteps - 1);
 }
 
 // ------------------------------------------------------------------------------ workgroup steps
-// Inclusive sums over the workgroup in thread order, and their total; every thread takes part.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 scan_step(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((u64)hi << 32 | lo);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+
+// Inclusive sums over a wave (all lanes active), and over the workgroup in thread order with their
+// total.
+template <class V>
+__device__ __forceinline__ V lanes_upto(V v) {
+  v = scan_step<0x111, 0xf>(v);         // row_shr:1, 2, 4, 8; row_bcast:15, 31
+  v = scan_step<0x112, 0xf>(v);
+  v = scan_step<0x114, 0xf>(v);
+  v = scan_step<0x118, 0xf>(v);
+  v = scan_step<0x142, 0xa>(v);
+  return scan_step<0x143, 0xc>(v);
+}
+
 template <int WAVES, class V>
 __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
-  const int lane = threadIdx.x & 63, wave = wave_id();
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V y = __shfl_up(v, o);
-    if (lane >= o) v += y;
-  }
+  v = lanes_upto(v);
   __syncthreads();
-  if (lane == 63) part[wave] = v;
+  if ((threadIdx.x & 63) == 63) part[wave_id()] = v;
   __syncthreads();
   V before = 0, sum = 0;
 #pragma unroll
   for (int i = 0; i < WAVES; ++i) {
-    if (i == wave) before = sum;
+    if (i == wave_id()) before = sum;
     sum += part[i];
   }
   total = sum;
@@ -199,16 +238,15 @@ struct Shared {
     struct {
       uint32_t steps[kSteps];
       int active[kCandidates];
-      float x[2][kCandidates];
-      int at[2][kCandidates];
-      double w[kCandidates];
+      u64 order[kCandidates];           // (the logit's key, the index from above)
+      u64 w[kCandidates];               // by rank
+      u64 swap[kCandidates];
     } list;
   };
   union {
-    double d[kThreads / 64];
-    u64 u[kThreads / 64];
-    int i[kThreads / 64];
-    float f[kThreads / 64];
+    u64 u[kWaves];
+    int i[kWaves];
+    float f[kWaves];
   } part;
   u64 chunk[kMaxChunks];                // what stays of each chunk
   int ties[kMaxChunks];
@@ -217,9 +255,9 @@ struct Shared {
 };
 
 // ------------------------------------------------------------------------------ a row
-template <int T, int THREADS>
+template <int T>
 struct Draw {
-  static constexpr int WAVES = THREADS / 64;
+  static constexpr int THREADS = kThreads, WAVES = kWaves;
   const SampleCall& c;
   const int64_t row;
   Shared& sh;
@@ -268,7 +306,7 @@ struct Draw {
   }
 
   // The sum of all weights.
-  __device__ double total() {
+  __device__ u64 total() {
     u64 sum = 0, whole;
     if (weighed) {
       for (int i = threadIdx.x; i < c.chunks; i += THREADS) sum += c.sums[row * c.chunks + i];
@@ -276,7 +314,26 @@ struct Draw {
       all([&](int, float v) { sum += whole_units(weight(v), c.unit); });
     }
     block_scan<WAVES>(sum, sh.part.u, whole);
-    return ldexp((double)whole, -c.unit);
+    return whole;
+  }
+
+  // Sorts the values of threads 0 .. m - 1 (a power of two, at least 64), the largest first.
+  __device__ u64 sorted(u64 v, int m) {
+    for (int size = 2; size <= m; size <<= 1)
+      for (int by = size >> 1; by > 0; by >>= 1) {
+        u64 other;
+        if (by < 64) {
+          other = __shfl_xor(v, by);
+        } else {
+          __syncthreads();
+          sh.list.swap[threadIdx.x] = v;
+          __syncthreads();
+          other = sh.list.swap[threadIdx.x ^ by];
+        }
+        const bool first = !(threadIdx.x & by), down = !(threadIdx.x & size);
+        v = (v > other) == (first == down) ? v : other;
+      }
+    return v;
   }
 
   // Draws from a list of candidates; false where a list cannot settle the row.
@@ -284,31 +341,32 @@ struct Draw {
     auto& l = sh.list;
     const int t = threadIdx.x;
     const bool k_set = k < c.vocab;
-    const int want = k_set ? min(k, kFew) : kFew;
+    // a weighed row has another way where its list is too short
+    const int want = k_set ? min(k, kFew) : weighed ? kFewer : kFew;
     for (int i = t; i < kSteps; i += THREADS) l.steps[i] = 0;
-    if (t == 0) sh.n = sh.m = 0;
+    if (t == 0) {
+      sh.n = sh.m = 0;
+      sh.first = kSteps - 1;
+    }
     __syncthreads();
-    int finite = 0;
     for (int s = t; s < c.slices; s += THREADS)
-      if (sh.top[s] != -__builtin_inff()) {
+      if (sh.top[s] != -__builtin_inff())
         atomicAdd(&l.steps[step_of(weight.top, sh.top[s])], 1u);
-        ++finite;
-      }
     __syncthreads();
     // the first step that `want` slices reach, or the last
     constexpr int EACH = kSteps / THREADS;
-    int mine = 0, slices;
+    int mine = 0, all_of;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) mine += (int)l.steps[t * EACH + i];
-    int upto = block_scan<WAVES>(mine, sh.part.i, slices) - mine;
-    if (t == 0) sh.first = kSteps - 1;
-    __syncthreads();
+    int upto = block_scan<WAVES>(mine, sh.part.i, all_of) - mine;
+    if (upto < want && upto + mine >= want) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      upto += (int)l.steps[t * EACH + i];
-      if (upto >= want) {
-        atomicMin(&sh.first, t * EACH + i);
-        break;
+      for (int i = 0; i < EACH; ++i) {
+        upto += (int)l.steps[t * EACH + i];
+        if (upto >= want) {
+          sh.first = t * EACH + i;
+          break;
+        }
       }
     }
     __syncthreads();
@@ -326,82 +384,72 @@ struct Draw {
       const float v = c.slice == 1 ? sh.top[e] : e < c.vocab ? x.at(e) : -__builtin_inff();
       if (v != -__builtin_inff() && step_of(weight.top, v) <= last) {
         const int at = atomicAdd(&sh.n, 1);
-        if (at < kCandidates) {
-          l.x[0][at] = v;
-          l.at[0][at] = e;
-        }
+        if (at < kCandidates) l.order[at] = (u64)x.order(v) << 32 | (uint32_t)~e;
       }
     }
     __syncthreads();
     const int n = sh.n;
     if (n > kCandidates) return false;
-    // by index, so that sums have one order
-    for (int i = t; i < n; i += THREADS) {
-      int to = 0;
-      const int mine = l.at[0][i];
-      for (int j = 0; j < n; ++j) to += l.at[0][j] < mine;
-      l.x[1][to] = l.x[0][i];
-      l.at[1][to] = mine;
-      l.w[to] = weight(l.x[0][i]);
-    }
+    int m_sort = 64;
+    while (m_sort < n) m_sort <<= 1;
+    const u64 mine_is = sorted(t < n ? l.order[t] : 0, m_sort);
+    const float v = x.of_order((uint32_t)(mine_is >> 32));
+    const double w = t < n ? weight(v) : 0.0;
+    const u64 units = whole_units(w, c.unit);
+    u64 mass, whole;
+    const u64 before = block_scan<WAVES>(units, sh.part.u, whole) - units;
+    // the weight of those that top-k left
+    if (t == 0) sh.above = whole;
     __syncthreads();
-    constexpr int ROUNDS = (kCandidates + THREADS - 1) / THREADS;   // a thread's, side by side
-    int rank[ROUNDS];
-    double before[ROUNDS], w[ROUNDS], in_k = 0, mass;
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      const int i = t * ROUNDS + r;
-      rank[r] = 0;
-      before[r] = w[r] = 0;
-      if (i >= n) continue;
-      const float v = l.x[1][i];
-      w[r] = l.w[i];
-      for (int j = 0; j < n; ++j) {
-        const float y = l.x[1][j];
-        if (y > v || (y == v && j < i)) {
-          ++rank[r];
-          before[r] += l.w[j];
-        }
-      }
-      if (rank[r] < k) in_k += w[r];
-    }
-    block_scan<WAVES>(in_k, sh.part.d, mass);
+    if (t == k) sh.above = before;
+    __syncthreads();
+    mass = sh.above;
     if (last < kSteps - 1 && !(k_set && k <= n)) {    // tokens outside the list may count
       if (k_set) return false;
-      int low = 0, any;
-#pragma unroll
-      for (int r = 0; r < ROUNDS; ++r) low |= t * ROUNDS + r < n && !(w[r] >= m);
-      block_scan<WAVES>(low, sh.part.i, any);
-      if (!any && p >= 1) return false;
-      const double whole = p < 1 ? total() : 0.0;
-      if (!any && !(mass > p * whole)) return false;
-      mass = whole;
+      if (t == 0) sh.m = 0;
+      __syncthreads();
+      if (t < n && !(w >= m)) sh.m = 1;
+      __syncthreads();
+      const bool low = sh.m;
+      if (!low && p >= 1) return false;
+      mass = p < 1 ? total() : 0;
+      if (!low && !(whole > (u64)(p * (double)mass))) return false;
     }
-    bool keep[ROUNDS];
-    double kept = 0, whole;
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      keep[r] = t * ROUNDS + r < n && rank[r] < k && (p >= 1 || before[r] <= p * mass) &&
-                (w[r] >= m || rank[r] == 0) && w[r] > 0;
-      kept += keep[r] ? w[r] : 0.0;
+    const bool keep = t < n && t < k && (p >= 1 || before <= (u64)(p * (double)mass)) &&
+                      (w >= m || t == 0) && units > 0;
+    // the draw goes by index: sorted by it, each with its rank
+    __syncthreads();
+    l.w[t] = units;
+    const u64 by_index = sorted(
+        keep ? (u64)(kMaxVocab - (int)~(uint32_t)mine_is) << 16 | (uint32_t)t : 0, m_sort);
+    __syncthreads();
+    const int rank = (int)(by_index & 0xffff);
+    const u64 here = by_index ? l.w[rank] : 0;
+    const u64 upto_w = block_scan<WAVES>(t < m_sort ? here : 0, sh.part.u, whole);
+    const u64 goal = (u64)(u * (double)whole);
+    // by_index is above 0 wherever something stays
+    if (mine_is_it(t < m_sort && here > 0, upto_w > goal)) {
+      const int token = kMaxVocab - (int)(by_index >> 16);
+      result(token, log(weight(x.at(token)) / ldexp((double)whole, -c.unit)));
     }
-    double upto_w = block_scan<WAVES>(kept, sh.part.d, whole) - kept;
-    if (t == 0) {
-      sh.first = kCandidates;
+    return true;
+  }
+
+  // The first thread that passes the goal, or, where rounding leaves none, the last with something.
+  __device__ __forceinline__ bool mine_is_it(bool some, bool passes) {
+    if (threadIdx.x == 0) {
+      sh.first = THREADS;
       sh.m = -1;
     }
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      if (!keep[r]) continue;
-      upto_w += w[r];
-      atomicMax(&sh.m, t * ROUNDS + r);               // the last one, where rounding leaves none
-      if (upto_w > u * whole) atomicMin(&sh.first, t * ROUNDS + r);
+    const u64 has = __ballot(some), over = __ballot(some && passes);
+    if ((threadIdx.x & 63) == 0) {
+      const int at = threadIdx.x;
+      if (has) atomicMax(&sh.m, at + 63 - __builtin_clzll(has));
+      if (over) atomicMin(&sh.first, at + __builtin_ctzll(over));
     }
     __syncthreads();
-    const int pick = min(sh.first, sh.m);
-    if (t == 0) result(l.at[1][pick], log(l.w[pick] / whole));
-    return true;
+    return (int)threadIdx.x == min(sh.first, sh.m);
   }
 
   // A border in the order of keys from `lo` to `hi`: the key at which `limit` is passed, going down,
@@ -497,12 +545,18 @@ struct Draw {
       ties = at == key ? min(ties, stay) : stay;
       key = at;
     }
-    // by index: each thread a run of slices
-    const int per = (c.slices + THREADS - 1) / THREADS * c.slice;
+    // by index: each thread a run of tokens
+    const int per = ((c.vocab + THREADS - 1) / THREADS + 7) & ~7;
     const int begin = min(c.vocab, (int)threadIdx.x * per), end = min(c.vocab, begin + per);
-    const double wk = weight(x.of_key(key));
-    double sum = 0;
-    int same = 0;
+    const float vk = x.of_key(key);
+    const double wk = weight(vk);
+    const u64 tie = wk >= m || vk == weight.top ? whole_units(wk, c.unit) : 0;
+    auto stays = [&](float v) {
+      const double w = weight(v);
+      return w >= m || v == weight.top ? whole_units(w, c.unit) : 0;
+    };
+    u64 sum = 0, whole;
+    int same = 0, all_same;
     for (int i = begin; i < end; i += 8) {
       float v[8];
       x.load(i, v);
@@ -511,50 +565,28 @@ struct Draw {
         if (i + j >= end || v[j] == -__builtin_inff()) continue;
         const uint32_t b = x.key(v[j]);
         same += b == key;
-        if (b > key) {
-          const double w = weight(v[j]);
-          if (w >= m || v[j] == weight.top) sum += w;
-        }
+        if (b > key) sum += stays(v[j]);
       }
     }
-    int all_same;
     const int had = block_scan<WAVES>(same, sh.part.i, all_same) - same;
-    if (wk >= m || x.of_key(key) == weight.top) sum += (double)min(max(ties - had, 0), same) * wk;
-    double whole;
-    const double upto = block_scan<WAVES>(sum, sh.part.d, whole);
-    const double goal = u * whole;
+    sum += (u64)min(max(ties - had, 0), same) * tie;
+    const u64 upto = block_scan<WAVES>(sum, sh.part.u, whole);
+    const u64 goal = (u64)(u * (double)whole);
     if (!mine_is_it(sum > 0, upto > goal)) return;
     // within the run that the draw falls into
-    double run = upto - sum, w_last = 0;
+    u64 run = upto - sum;
     int last = -1, seen = had;
-    for (int i = begin; i < end; ++i) {
+    for (int i = begin; i < end && run <= goal; ++i) {
       const float v = x.at(i);
       if (v == -__builtin_inff()) continue;
       const uint32_t b = x.key(v);
       if (b < key || (b == key && seen++ >= ties)) continue;
-      const double w = weight(v);
-      if (!(w >= m || v == weight.top) || !(w > 0)) continue;
+      const u64 w = b == key ? tie : stays(v);
+      if (w == 0) continue;
       run += w;
       last = i;
-      w_last = w;
-      if (run > goal) break;
     }
-    result(last, log(w_last / whole));
-  }
-
-  // The first thread that passes the goal, or, where rounding leaves none, the last with something.
-  __device__ __forceinline__ bool mine_is_it(bool some, bool passes) {
-    if (threadIdx.x == 0) {
-      sh.first = THREADS;
-      sh.m = -1;
-    }
-    __syncthreads();
-    if (some) {
-      atomicMax(&sh.m, (int)threadIdx.x);
-      if (passes) atomicMin(&sh.first, (int)threadIdx.x);
-    }
-    __syncthreads();
-    return (int)threadIdx.x == min(sh.first, sh.m);
+    result(last, log(weight(x.at(last)) / ldexp((double)whole, -c.unit)));
   }
 
   // Draws from a weighed row: top-p alone, or no filter.  False where min-p cuts deeper.
@@ -617,8 +649,8 @@ struct Draw {
         }
       };
       const float far = step == kSteps - 1 ? __builtin_inff()
-                                           : __uint_as_float((uint32_t)(step + 1 + kFirstStep) << 18);
-      const float near = step == 0 ? 0.f : __uint_as_float((uint32_t)(step + kFirstStep) << 18);
+                                           : __uint_as_float((uint32_t)(step + 1 + kFirstStep) << 16);
+      const float near = step == 0 ? 0.f : __uint_as_float((uint32_t)(step + kFirstStep) << 16);
       const uint32_t low = key, high = x.key(weight.top);
       const uint32_t lo = max(x.key(weight.top - far), low + 2) - 2;
       border<true>([&](auto&& f) { in_step([&](int, float v) { f(v); }); }, lo,
@@ -666,7 +698,7 @@ struct Draw {
     }
     __syncthreads();
     // the draw falls into chunk sh.n, a thread 8 tokens of it
-    static_assert(kChunk <= 8 * kThreads, "a thread's tokens");
+    static_assert(kChunk % (8 * kThreads) == 0 && kChunk <= 32 * kThreads, "a thread's tokens");
     constexpr int EACH = kChunk / THREADS;
     const int chunk = sh.n, begin = chunk * kChunk + threadIdx.x * EACH;
     u64 w[EACH], sum = 0;
@@ -788,8 +820,9 @@ __global__ void __launch_bounds__(kChunkThreads) sample_weights_kernel(SampleCal
   for (int i = threadIdx.x; i < kSteps; i += kChunkThreads) to[i] = steps[i];
 }
 
-template <int T, int THREADS>
-__global__ void __launch_bounds__(THREADS) sample_kernel(SampleCall c) {
+template <int T>
+__global__ void __launch_bounds__(kThreads) sample_kernel(SampleCall c) {
+  constexpr int THREADS = kThreads;
   __shared__ Shared sh;
   const int64_t row = blockIdx.x;
   const Settings s(c, row);
@@ -802,8 +835,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleCall c) {
     for (int i = threadIdx.x; i < c.slices; i += THREADS)
       top = fmaxf(top, sh.top[i] = c.tops[row * c.slices + i]);
   }
-  top = block_max<THREADS / 64>(top, sh.part.f);
-  Draw<T, THREADS> d(c, row, sh, top, s, u);
+  top = block_max<kWaves>(top, sh.part.f);
+  Draw<T> d(c, row, sh, top, s, u);
   if (top == -__builtin_inff()) {
     if (threadIdx.x == 0) d.result(-1, -__builtin_inff());
     return;
@@ -811,7 +844,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleCall c) {
   if (s.greedy()) return d.greedy();
   if ((s.k < c.vocab || s.p < 1.f || s.m > 0.f) && d.by_list()) return;
   __syncthreads();
-  if (THREADS == kThreads && d.weighed && d.by_chunks()) return;
+  if (d.weighed && d.by_chunks()) return;
   __syncthreads();
   d.by_passes();
 }
@@ -844,10 +877,7 @@ static void launch_sample(const SampleCall& c, int64_t rows, hipStream_t stream)
   const dim3 grid(c.chunks, (unsigned)rows);
   if (c.chunks) sample_tops_kernel<T><<<grid, kChunkThreads, 0, stream>>>(c);
   if (c.weighed) sample_weights_kernel<T><<<grid, kChunkThreads, 0, stream>>>(c);
-  if (c.vocab <= kSmallVocab)
-    sample_kernel<T, kSmallThreads><<<(unsigned)rows, kSmallThreads, 0, stream>>>(c);
-  else
-    sample_kernel<T, kThreads><<<(unsigned)rows, kThreads, 0, stream>>>(c);
+  sample_kernel<T><<<(unsigned)rows, kThreads, 0, stream>>>(c);
 }
 
 }  // namespace mtl
