@@ -32,6 +32,7 @@ constexpr int kChunkThreads = 256;
 constexpr int kCandidates = kThreads;
 constexpr int kFew = 256, kFewer = 64;  // tokens that a list is made for
 constexpr int kBins = 2048;
+constexpr int kHeld = 1024;
 constexpr int kMaxSlices = 8192;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxChunks = kMaxVocab / kChunk;
@@ -42,7 +43,7 @@ constexpr int kSteps = 1024;
 struct SampleCall {
   const void* x;
   int64_t ld;
-  int vocab, slice, slices, unit;       // unit: weights are counted in 2^-unit
+  int vocab, slice_shift, slices, unit; // slices of 2^slice_shift; weights are counted in 2^-unit
   int chunks;                           // 0: one launch does it all
   int weighed;                          // rows that need the sum of their weights have it
   const float* u;
@@ -50,6 +51,7 @@ struct SampleCall {
   int64_t* token;
   float* logprob;
   float* tops;                          // [rows][slices]
+  float* chunk_tops;                    // [rows][chunks]
   u64* sums;                            // [rows][chunks]
   u64* steps;                           // [rows][chunks][kSteps]; null: no row can need them
 };
@@ -98,13 +100,8 @@ struct Logits {
     return clean(T == MTL_T_BF16 ? bf16_to_f32(e) : f16_to_f32(e));
   }
 
-  // Logits i .. i + 7, -infinity past the end.
-  __device__ __forceinline__ void load(int i, float (&x)[8]) const {
-    if (i + 8 > n) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = i + j < n ? at(i + j) : -__builtin_inff();
-      return;
-    }
+  // Logits i .. i + 7, all there.
+  __device__ __forceinline__ void load_whole(int i, float (&x)[8]) const {
     if (T == MTL_T_F32) {
       float v[8];
       __builtin_memcpy(v, p + (int64_t)i * 4, 32);
@@ -119,6 +116,13 @@ struct Logits {
         x[j] = clean(T == MTL_T_BF16 ? bf16_to_f32(e) : f16_to_f32(e));
       }
     }
+  }
+
+  // Logits i .. i + 7, -infinity past the end.
+  __device__ __forceinline__ void load(int i, float (&x)[8]) const {
+    if (i + 8 <= n) return load_whole(i, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = i + j < n ? at(i + j) : -__builtin_inff();
   }
 
   // Whole numbers in the logits' order; key: without the bits that the type does not have.
@@ -248,6 +252,7 @@ struct Shared {
     int i[kWaves];
     float f[kWaves];
   } part;
+  u64 held[kHeld];                      // tokens of one step: (logit, index)
   u64 chunk[kMaxChunks];                // what stays of each chunk
   int ties[kMaxChunks];
   int n, m, first;
@@ -284,7 +289,7 @@ struct Draw {
     __syncthreads();
     for (int s = threadIdx.x; s < c.slices; s += THREADS) {
       if (sh.top[s] != weight.top) continue;
-      for (int i = s * c.slice; i < min(c.vocab, (s + 1) * c.slice); ++i)
+      for (int i = s << c.slice_shift; i < min(c.vocab, (s + 1) << c.slice_shift); ++i)
         if (x.at(i) == weight.top) {
           atomicMin(&sh.first, i);
           break;
@@ -317,22 +322,56 @@ struct Draw {
     return whole;
   }
 
-  // Sorts the values of threads 0 .. m - 1 (a power of two, at least 64), the largest first.
-  __device__ u64 sorted(u64 v, int m) {
-    for (int size = 2; size <= m; size <<= 1)
-      for (int by = size >> 1; by > 0; by >>= 1) {
-        u64 other;
-        if (by < 64) {
-          other = __shfl_xor(v, by);
-        } else {
-          __syncthreads();
-          sh.list.swap[threadIdx.x] = v;
-          __syncthreads();
-          other = sh.list.swap[threadIdx.x ^ by];
-        }
-        const bool first = !(threadIdx.x & by), down = !(threadIdx.x & size);
-        v = (v > other) == (first == down) ? v : other;
+  // One exchange of a sort between lanes `BY` apart: v and the other's in any order.
+  template <int BY>
+  static __device__ __forceinline__ void lanes_apart(u64 v, u64& a, u64& b) {
+    uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32), lo2 = lo, hi2 = hi;
+    if (BY == 32) {
+      permlane_swap32(lo, lo2);
+      permlane_swap32(hi, hi2);
+    } else if (BY == 16) {
+      permlane_swap16(lo, lo2);
+      permlane_swap16(hi, hi2);
+    } else {
+      constexpr int kCtrl = BY == 8 ? kDppRor8 : BY == 4 ? kDppHalfMirror : BY == 2 ? kDppXor2
+                                                                                    : kDppXor1;
+      lo2 = __builtin_amdgcn_update_dpp(0, lo, kCtrl, 0xf, 0xf, false);
+      hi2 = __builtin_amdgcn_update_dpp(0, hi, kCtrl, 0xf, 0xf, false);
+      if (BY == 4) {                    // the mirror of 8 and that of 4: 4 apart
+        lo2 = __builtin_amdgcn_update_dpp(0, lo2, 0x1b, 0xf, 0xf, false);
+        hi2 = __builtin_amdgcn_update_dpp(0, hi2, 0x1b, 0xf, 0xf, false);
       }
+    }
+    a = (u64)hi << 32 | lo;
+    b = (u64)hi2 << 32 | lo2;
+  }
+
+  template <int BY>
+  static __device__ __forceinline__ u64 exchanged(u64 v, bool down) {
+    u64 a, b;
+    lanes_apart<BY>(v, a, b);
+    const bool larger = !(threadIdx.x & BY) == down;
+    return (a > b) == larger ? a : b;
+  }
+
+  // Sorts the values of threads 0 .. m - 1 (a power of two, at least 64), the largest first.
+  __device__ __forceinline__ u64 sorted(u64 v, int m) {
+    for (int size = 2; size <= m; size <<= 1) {
+      const bool down = !(threadIdx.x & size);
+      for (int by = size >> 1; by > 32; by >>= 1) {
+        __syncthreads();
+        sh.list.swap[threadIdx.x] = v;
+        __syncthreads();
+        const u64 other = sh.list.swap[threadIdx.x ^ by];
+        v = (v > other) == (!(threadIdx.x & by) == down) ? v : other;
+      }
+      if (size > 32) v = exchanged<32>(v, down);
+      if (size > 16) v = exchanged<16>(v, down);
+      if (size > 8) v = exchanged<8>(v, down);
+      if (size > 4) v = exchanged<4>(v, down);
+      if (size > 2) v = exchanged<2>(v, down);
+      v = exchanged<1>(v, down);
+    }
     return v;
   }
 
@@ -379,9 +418,9 @@ struct Draw {
     __syncthreads();
     const int active = sh.m;
     if (active > kCandidates) return false;
-    for (int i = t; i < active * c.slice; i += THREADS) {
-      const int e = l.active[i / c.slice] * c.slice + i % c.slice;
-      const float v = c.slice == 1 ? sh.top[e] : e < c.vocab ? x.at(e) : -__builtin_inff();
+    for (int i = t; i < active << c.slice_shift; i += THREADS) {
+      const int e = (l.active[i >> c.slice_shift] << c.slice_shift) + (i & ((1 << c.slice_shift) - 1));
+      const float v = c.slice_shift == 0 ? sh.top[e] : e < c.vocab ? x.at(e) : -__builtin_inff();
       if (v != -__builtin_inff() && step_of(weight.top, v) <= last) {
         const int at = atomicAdd(&sh.n, 1);
         if (at < kCandidates) l.order[at] = (u64)x.order(v) << 32 | (uint32_t)~e;
@@ -392,36 +431,37 @@ struct Draw {
     if (n > kCandidates) return false;
     int m_sort = 64;
     while (m_sort < n) m_sort <<= 1;
-    const u64 mine_is = sorted(t < n ? l.order[t] : 0, m_sort);
-    const float v = x.of_order((uint32_t)(mine_is >> 32));
-    const double w = t < n ? weight(v) : 0.0;
-    const u64 units = whole_units(w, c.unit);
-    u64 mass, whole;
-    const u64 before = block_scan<WAVES>(units, sh.part.u, whole) - units;
-    // the weight of those that top-k left
-    if (t == 0) sh.above = whole;
-    __syncthreads();
-    if (t == k) sh.above = before;
-    __syncthreads();
-    mass = sh.above;
-    if (last < kSteps - 1 && !(k_set && k <= n)) {    // tokens outside the list may count
-      if (k_set) return false;
-      if (t == 0) sh.m = 0;
+    // sorted by the order, and then what stays by index, each token with its rank
+    u64 by_index = t < n ? l.order[t] : 0, mass, whole;
+    for (int pass = 0; pass < 2; ++pass) {            // one copy of the code
+      by_index = sorted(by_index, m_sort);
+      if (pass) break;
+      const u64 mine_is = by_index;
+      const double w = t < n ? weight(x.of_order((uint32_t)(mine_is >> 32))) : 0.0;
+      const u64 units = whole_units(w, c.unit);
+      const u64 before = block_scan<WAVES>(units, sh.part.u, whole) - units;
+      // the weight of those that top-k left
+      if (t == 0) sh.above = whole;
       __syncthreads();
-      if (t < n && !(w >= m)) sh.m = 1;
+      if (t == k) sh.above = before;
       __syncthreads();
-      const bool low = sh.m;
-      if (!low && p >= 1) return false;
-      mass = p < 1 ? total() : 0;
-      if (!low && !(whole > (u64)(p * (double)mass))) return false;
+      mass = sh.above;
+      if (last < kSteps - 1 && !(k_set && k <= n)) {  // tokens outside the list may count
+        if (k_set) return false;
+        if (t == 0) sh.m = 0;
+        __syncthreads();
+        if (t < n && !(w >= m)) sh.m = 1;
+        __syncthreads();
+        const bool low = sh.m;
+        if (!low && p >= 1) return false;
+        mass = p < 1 ? total() : 0;
+        if (!low && !(whole > (u64)(p * (double)mass))) return false;
+      }
+      const bool keep = t < n && t < k && (p >= 1 || before <= (u64)(p * (double)mass)) &&
+                        (w >= m || t == 0) && units > 0;
+      l.w[t] = units;
+      by_index = keep ? (u64)(kMaxVocab - (int)~(uint32_t)mine_is) << 16 | (uint32_t)t : 0;
     }
-    const bool keep = t < n && t < k && (p >= 1 || before <= (u64)(p * (double)mass)) &&
-                      (w >= m || t == 0) && units > 0;
-    // the draw goes by index: sorted by it, each with its rank
-    __syncthreads();
-    l.w[t] = units;
-    const u64 by_index = sorted(
-        keep ? (u64)(kMaxVocab - (int)~(uint32_t)mine_is) << 16 | (uint32_t)t : 0, m_sort);
     __syncthreads();
     const int rank = (int)(by_index & 0xffff);
     const u64 here = by_index ? l.w[rank] : 0;
@@ -604,6 +644,7 @@ struct Draw {
       const double limit = p * ldexp((double)whole, -c.unit);
       const u64 limit_units = (u64)ldexp(limit, c.unit);
       u64 of[EACH] = {}, sum = 0, total;
+#pragma unroll 8
       for (int i = 0; i < c.chunks; ++i)
 #pragma unroll
         for (int e = 0; e < EACH; ++e) of[e] += steps[i * kSteps + threadIdx.x * EACH + e];
@@ -635,25 +676,52 @@ struct Draw {
       }
       __syncthreads();
       u64 above = sh.above;
-      // its tokens lie in slices that reach it, and between two keys (two off for rounding)
+      // its tokens lie between two keys (two off for rounding)
+      // A few in a hundred tokens are in the step: lanes first note which of theirs are, and then
+      // each takes its next one, so that f runs as often as the fullest lane has tokens, not for
+      // each of the 32.
       auto in_step = [&](auto&& f) {
-        for (int s = threadIdx.x / 4; s < c.slices; s += THREADS / 4) {
-          if (step_of(weight.top, sh.top[s]) > step) continue;
-          for (int i = (threadIdx.x & 3) * 8; i < c.slice; i += 32) {
-            float v[8];
-            x.load(s * c.slice + i, v);
+        constexpr int AHEAD = 4;                      // pieces of 8 tokens on their way at a time
+        for (int i0 = threadIdx.x; i0 * 8 < c.vocab; i0 += AHEAD * THREADS) {
+          float v[AHEAD][8];
+#pragma unroll
+          for (int a = 0; a < AHEAD; ++a)             // the last one begins earlier
+            x.load_whole(min((i0 + a * THREADS) * 8, c.vocab - 8), v[a]);
+          uint32_t hits = 0;
+#pragma unroll
+          for (int a = 0; a < AHEAD; ++a) {
+            const int i = (i0 + a * THREADS) * 8, from = min(i, c.vocab - 8);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              if (step_of(weight.top, v[j]) == step) f(s * c.slice + i + j, v[j]);
+              if (from + j >= i && step_of(weight.top, v[a][j]) == step) hits |= 1u << (8 * a + j);
+          }
+          for (; hits; hits &= hits - 1) {
+            const int bit = __builtin_ctz(hits);
+            const int i = min((i0 + (bit >> 3) * THREADS) * 8, c.vocab - 8) + (bit & 7);
+            f(i, x.at(i));
           }
         }
+      };
+      // they are looked for once, where there are not too many
+      if (threadIdx.x == 0) sh.n = 0;
+      __syncthreads();
+      in_step([&](int i, float v) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < kHeld) sh.held[at] = (u64)__float_as_uint(v) << 32 | (uint32_t)i;
+      });
+      __syncthreads();
+      const int held = sh.n;
+      auto tokens = [&](auto&& f) {
+        if (held > kHeld) return in_step(f);
+        for (int i = threadIdx.x; i < held; i += THREADS)
+          f((int)(uint32_t)sh.held[i], __uint_as_float((uint32_t)(sh.held[i] >> 32)));
       };
       const float far = step == kSteps - 1 ? __builtin_inff()
                                            : __uint_as_float((uint32_t)(step + 1 + kFirstStep) << 16);
       const float near = step == 0 ? 0.f : __uint_as_float((uint32_t)(step + kFirstStep) << 16);
       const uint32_t low = key, high = x.key(weight.top);
       const uint32_t lo = max(x.key(weight.top - far), low + 2) - 2;
-      border<true>([&](auto&& f) { in_step([&](int, float v) { f(v); }); }, lo,
+      border<true>([&](auto&& f) { tokens([&](int, float v) { f(v); }); }, lo,
                    min(x.key(weight.top - near) + 2, high), limit_units, key, above);
       const double wk = weight(x.of_key(key));
       if (!(wk >= m)) return false;
@@ -665,7 +733,7 @@ struct Draw {
         sh.ties[i] = 0;
       }
       __syncthreads();
-      in_step([&](int i, float v) {
+      tokens([&](int i, float v) {
         if (v == -__builtin_inff()) return;
         const uint32_t b = x.key(v);
         if (b > key) atomicAdd(&sh.chunk[i / kChunk], whole_units(weight(v), c.unit));
@@ -748,7 +816,9 @@ template <int T>
 __global__ void __launch_bounds__(kChunkThreads) sample_tops_kernel(SampleCall c) {
   const int64_t row = blockIdx.y;
   const Logits<T> x(c, row);
-  const int lanes = c.slice / 8;                      // of a slice: 4 or 16
+  const int lanes = 1 << (c.slice_shift - 3);         // of a slice: 4 or 16
+  __shared__ float part[kChunkThreads / 64];
+  float top = -__builtin_inff();
   float v[kChunk / kChunkThreads / 8][8];
 #pragma unroll
   for (int i = 0; i < kChunk / kChunkThreads / 8; ++i) {
@@ -761,14 +831,19 @@ __global__ void __launch_bounds__(kChunkThreads) sample_tops_kernel(SampleCall c
     float best = v[i][0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) best = fmaxf(best, v[i][j]);
+    top = fmaxf(top, best);
     best = fmaxf(best, dpp_f32<kDppXor1>(best));
     best = fmaxf(best, dpp_f32<kDppXor2>(best));
     if (lanes == 16) {
       best = fmaxf(best, dpp_f32<kDppHalfMirror>(best));
       best = fmaxf(best, dpp_f32<kDppMirror>(best));
     }
-    if (at < c.vocab && threadIdx.x % lanes == 0) c.tops[row * c.slices + at / c.slice] = best;
+    if (at < c.vocab && (threadIdx.x & (lanes - 1)) == 0)
+      c.tops[row * c.slices + (at >> c.slice_shift)] = best;
   }
+  if (!c.weighed) return;
+  top = block_max<kChunkThreads / 64>(top, part);
+  if (threadIdx.x == 0) c.chunk_tops[row * c.chunks + blockIdx.x] = top;
 }
 
 // Each chunk's weights, and by steps, of rows that need them.
@@ -792,8 +867,7 @@ __global__ void __launch_bounds__(kChunkThreads) sample_weights_kernel(SampleCal
     x.load(min(at, c.vocab), v[i]);
   }
   float top = -__builtin_inff();
-  for (int i = threadIdx.x; i < c.slices; i += kChunkThreads)
-    top = fmaxf(top, c.tops[row * c.slices + i]);
+  if ((int)threadIdx.x < c.chunks) top = c.chunk_tops[row * c.chunks + threadIdx.x];
   top = block_max<WAVES>(top, part.f);
   if (by_steps)
     for (int i = threadIdx.x; i < kSteps; i += kChunkThreads) steps[i] = 0;
@@ -829,11 +903,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleCall c) {
   const float u = c.u[row];
   const Logits<T> x(c, row);
   float top = -__builtin_inff();
-  if (c.slice == 1) {
-    for (int i = threadIdx.x; i < c.vocab; i += THREADS) top = fmaxf(top, sh.top[i] = x.at(i));
-  } else {
-    for (int i = threadIdx.x; i < c.slices; i += THREADS)
-      top = fmaxf(top, sh.top[i] = c.tops[row * c.slices + i]);
+  const float* tops = c.tops + row * c.slices;
+  for (int i0 = threadIdx.x; i0 < c.slices; i0 += 4 * THREADS) {
+    float v[4];                         // four on their way at a time
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = min(i0 + j * THREADS, c.slices - 1);
+      v[j] = c.slice_shift == 0 ? x.at(i) : tops[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      top = fmaxf(top, v[j]);
+      if (i0 + j * THREADS < c.slices) sh.top[i0 + j * THREADS] = v[j];
+    }
   }
   top = block_max<kWaves>(top, sh.part.f);
   Draw<T> d(c, row, sh, top, s, u);
@@ -868,7 +950,7 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab, const mtl_sample_sett
   p.weighed = p.steps || (k_open && draws && (s.min_p || !(s.min_p_all > 0.f)));
   p.steps_bytes = p.steps ? rows * p.chunks * kSteps * 8 : 0;
   p.sums_bytes = p.weighed ? rows * p.chunks * 8 : 0;
-  p.bytes = p.steps_bytes + p.sums_bytes + rows * p.slices * 4;
+  p.bytes = p.steps_bytes + p.sums_bytes + rows * (p.slices + p.chunks) * 4;
   return p;
 }
 
@@ -907,9 +989,9 @@ extern "C" int mtl_sample(const void* logits, int64_t ld, int64_t rows, int64_t 
   int unit = 44;
   while (unit > 0 && (vocab >> (62 - unit)) > 0) --unit;
   char* ws = static_cast<char*>(workspace);
-  const SampleCall c{logits, ld, (int)vocab, p.slice, (int)p.slices, unit, p.chunks, p.weighed, u,
-                     *settings, token, logprob,
-                     reinterpret_cast<float*>(ws + p.steps_bytes + p.sums_bytes),
+  float* tops = reinterpret_cast<float*>(ws + p.steps_bytes + p.sums_bytes);
+  const SampleCall c{logits, ld, (int)vocab, __builtin_ctz(p.slice), (int)p.slices, unit, p.chunks,
+                     p.weighed, u, *settings, token, logprob, tops, tops + rows * p.slices,
                      reinterpret_cast<u64*>(ws + p.steps_bytes),
                      p.steps ? reinterpret_cast<u64*>(ws) : nullptr};
   hipStream_t st = (hipStream_t)stream;
