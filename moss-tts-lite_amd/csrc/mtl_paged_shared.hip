@@ -70,13 +70,24 @@ struct Lists {
   int2 own[kStash];                     // a sequence's own positions [x, y)
 };
 
+__device__ __forceinline__ int blocks_in(int positions) {
+  return (positions + kSharedBlock - 1) / kSharedBlock;
+}
+
+// The cost of `columns` columns over `blocks` blocks, `wide` (a power of two) of them an item.
+__device__ __forceinline__ int cost_of(int columns, int blocks, int wide) {
+  const int rest = columns & (wide - 1);
+  return columns / wide * item_cost(wide, blocks) + (rest ? item_cost(rest, blocks) : 0);
+}
+
 struct Batch {
   const SharedCall& a;
   Lists& l;
+  int wide;                             // columns of an item, at most
   bool near;
 
-  __device__ __forceinline__ Batch(const SharedCall& a, Lists& l)
-      : a(a), l(l), near(a.seqs <= kStash && a.n_groups <= kStash) {
+  __device__ __forceinline__ Batch(const SharedCall& a, Lists& l, int wide)
+      : a(a), l(l), wide(wide), near(a.seqs <= kStash && a.n_groups <= kStash) {
     if (!near) return;
     for (int i = threadIdx.x; i < max(a.seqs, a.n_groups + 1); i += kSharedWaves * 64) {
       if (i < a.seqs) l.lens[i] = clamp_len(a.lens[i], a.cap);
@@ -97,7 +108,11 @@ struct Batch {
     Group g;
     g.begin = min(max(start(i), 0), a.seqs);
     g.end = min(max(start(i + 1), g.begin), a.seqs);
-    g.shared = g.end - g.begin > 1 ? clamp_len(near ? l.shared[i] : a.shared[i], a.cap) & ~15 : 0;
+    g.shared = clamp_len(near ? l.shared[i] : a.shared[i], a.cap) & ~15;
+    // Few sequences with a short prefix read it for themselves, where that costs no more.
+    const int n = g.end - g.begin, blocks = blocks_in(g.shared);
+    if (cost_of(n * a.per_kv, blocks, wide) >= n * blocks * block_cost(min(a.per_kv, wide)))
+      g.shared = 0;
     return g;
   }
 
@@ -128,17 +143,6 @@ struct Batch {
   }
 };
 
-__device__ __forceinline__ int blocks_in(int positions) {
-  return (positions + kSharedBlock - 1) / kSharedBlock;
-}
-
-// The cost of `columns` columns over `blocks` blocks, WIDE columns an item.
-template <int WIDE>
-__device__ __forceinline__ int cost_of(int columns, int blocks) {
-  return columns / WIDE * item_cost(WIDE, blocks) +
-         (columns % WIDE ? item_cost(columns % WIDE, blocks) : 0);
-}
-
 // Where the items lie in the row, as every wave finds it: a lane adds up a run of groups and a run
 // of sequences.
 template <int WIDE>
@@ -155,7 +159,7 @@ struct Row {
       if (at >= a.n_groups) break;
       const Group g = batch.group((int)at);
       const int columns = (g.end - g.begin) * a.per_kv;
-      cost += cost_of<WIDE>(columns, blocks_in(g.shared));
+      cost += cost_of(columns, blocks_in(g.shared), WIDE);
       if (g.shared) widest = max(widest, min(columns, WIDE));
     }
     const int most = block_cost(__builtin_amdgcn_readfirstlane((int)wave_max_valu((float)widest)));
@@ -166,7 +170,7 @@ struct Row {
       const int64_t at = (int64_t)lane * per_seq + i;
       if (at >= a.seqs) break;
       const int2 own = batch.own_of((int)at);
-      cost += cost_of<WIDE>(a.per_kv, blocks_in(own.y - own.x));
+      cost += cost_of(a.per_kv, blocks_in(own.y - own.x), WIDE);
     }
     seqs_upto = wave_scan(cost);
     total = shared_cost + __builtin_amdgcn_readlane(seqs_upto, 63);
@@ -743,7 +747,7 @@ __global__ void __launch_bounds__(kSharedWaves * 64, 2) paged_shared_kernel(Shar
   __shared__ Lists lists;
   const int units = pool.kv_heads;
   const int kvh = blockIdx.x % units, piece = blockIdx.x / units;
-  const Batch batch(a, lists);
+  const Batch batch(a, lists, WIDE);
   const Row<WIDE> row(a, batch);
   if (piece == a.pieces) {
     if (kvh == 0) write_items<WIDE>(batch, row);
@@ -779,7 +783,7 @@ __global__ void __launch_bounds__(kSharedWaves * 64, 2) paged_shared_kernel(Shar
       first = g.begin;
       columns = (g.end - g.begin) * a.per_kv;
       blocks = blocks_in(g.shared);
-      const int cost = cost_of<WIDE>(columns, blocks);
+      const int cost = cost_of(columns, blocks, WIDE);
       if (base + cost <= lo) {
         base += cost;
         continue;
