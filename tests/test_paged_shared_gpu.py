@@ -157,6 +157,57 @@ def test_holes_and_long_lens(dev):
     check(a)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1.5, -2.0])
+def test_scales_of_either_sign(dev, kv, scale):
+    a = shared_case(dev, [3, 20], [500, 300], [520, 500, 640] + [300 + i for i in range(20)], 8, 2,
+                    64, 16, "bf16", kv, 12)
+    a["scale"] = scale
+    if kv == "e4m3":
+        a["k_scale"][1] *= -1
+        a["v_scale"][0] *= -1
+    # scores are up to 12 times larger here: so is what float32 products are off
+    out, lse = paged.paged_attention_shared(**a, return_lse=True)
+    ref, rlse, mag = attention64(**{k: v for k, v in a.items() if k not in ("groups", "shared")})
+    rel = 2 ** -16 + 2 ** -14 * max(1, abs(scale) * 8)
+    assert ((out.cpu().double() - ref).abs() <= 2 ** -8 * ref.abs() + rel * mag + 2.0 ** -24).all()
+    assert ((lse.cpu().double() - rlse).abs() <= 2e-4 * max(1, abs(scale) * 8)).all()
+
+
+@pytest.mark.parametrize("n", [511, 512, 513])
+def test_as_many_sequences_as_fit_a_workgroups_lists(dev, n):
+    sizes = [7] * (n // 7) + ([n % 7] if n % 7 else [])
+    rng = random.Random(n)
+    shared = [rng.choice([0, 48, 400]) for _ in sizes]
+    lens = [s + rng.randint(0, 40) for k, s in zip(sizes, shared) for _ in range(k)]
+    check(shared_case(dev, sizes, shared, lens, 2, 1, 64, 16, seed=n))
+
+
+def test_more_groups_than_sequences(dev):
+    sizes = [0] * 300 + [3] + [0] * 300 + [2]
+    shared = [50] * 300 + [600] + [9] * 300 + [700]
+    check(shared_case(dev, sizes, shared, [610, 600, 777, 700, 730], 8, 2, 128, 16, seed=9))
+
+
+def test_growing_and_falling_scores(dev):
+    # the running maximum moves in every tile, or never after the first
+    for sign in (1, -1):
+        a = shared_case(dev, [20], [2000], [2000 + 5 * i for i in range(20)], 8, 2, 128, 32, seed=3)
+        n, hkv, page, d = a["k_pages"].shape
+        rank = torch.full((n,), 0.0, device=dev)
+        rank[a["table"][0, :62].long()] = torch.arange(62, device=dev).float()
+        a["k_pages"] = (a["k_pages"].nan_to_num() * 0.05).float()
+        a["k_pages"][..., 0] += sign * rank[:, None, None] * 0.5
+        a["k_pages"] = a["k_pages"].bfloat16()
+        a["v_pages"] = a["v_pages"].nan_to_num()
+        a["q"][..., 0] = 8.0                         # a page's scores are some 0.35 above the last's
+        out = paged.paged_attention_shared(**a)
+        ref, _, mag = attention64(**{k: v for k, v in a.items() if k not in ("groups", "shared")})
+        # scores up to 22: 2^-24 of the products' sizes (some 260) a step
+        assert ((out.cpu().double() - ref).abs() <=
+                2 ** -8 * ref.abs() + (2 ** -16 + 2 ** -12) * mag + 2.0 ** -24).all()
+
+
 def test_many_sequences(dev):
     rng = random.Random(1)
     sizes = [rng.randint(1, 30) for _ in range(90)]  # past what a workgroup keeps of lengths

@@ -84,6 +84,57 @@ def test_equal_logits(dev, vocab, kw):
             assert int(tok) == want, (value, r)
 
 
+@pytest.mark.parametrize("vocab", [9000, 70001])
+@pytest.mark.parametrize("spread", [1e-5, 0.02, 30.0, 1000.0])
+@pytest.mark.parametrize("kw", [dict(), dict(top_p=0.3), dict(top_p=0.97), dict(top_k=100),
+                                dict(top_p=0.6, min_p=0.3), dict(min_p=0.7),
+                                dict(top_p=0.9, temperature=0.3)], ids=str)
+def test_spreads(dev, vocab, spread, kw):
+    # nuclei of one token to nearly all, borders among thousands of tokens of one step
+    gen = torch.Generator().manual_seed(int(spread * 1e5) + vocab)
+    x = spread * torch.randn(3, vocab, generator=gen) + 0.3
+    check(dev, x, torch.rand(3, generator=gen), **kw)
+    check(dev, x.half(), torch.rand(3, generator=gen), **kw)
+
+
+@pytest.mark.parametrize("vocab", [8192, 8193, 16384, 16385, 24577])
+def test_draws_in_every_chunk(dev, vocab):
+    gen = torch.Generator().manual_seed(vocab)
+    x = torch.randn(1, vocab, generator=gen).expand(40, vocab)
+    u = (torch.arange(40).float() + 0.5) / 40
+    for kw in (dict(), dict(top_p=0.9), dict(top_p=0.999)):
+        tok = check(dev, x, u, **kw)
+        assert (tok[1:] >= tok[:-1]).all() and int(tok[-1]) > vocab - vocab // 10
+
+
+def test_large_masked_rows(dev):
+    inf = float("inf")
+    gen = torch.Generator().manual_seed(18)
+    x = logits_of(gen, 6, 30000, torch.float32)
+    x[0] = -inf
+    x[1, :29999] = -inf
+    x[2, 100:29000] = float("nan")
+    x[3, [5, 8191, 8192, 29999]] = inf
+    x[4] = torch.finfo(torch.float32).min
+    x[5, 10:] = -inf
+    u = torch.rand(6, generator=gen)
+    for kw in (dict(), dict(top_p=0.71), dict(top_k=3), dict(min_p=0.1), dict(temperature=0.0),
+               dict(top_k=20000)):
+        tok = check(dev, x, u, **kw)
+        assert tok[:2].tolist() == [-1, 29999] and int(tok[3]) in (5, 8191, 8192, 29999)
+
+
+def test_equal_logits_of_a_large_row(dev):
+    # the border lies among equals, over all chunks
+    vocab = 50000
+    x = torch.zeros(5, vocab, dtype=torch.bfloat16)
+    x[:, 7::1000] = 1.0
+    u = torch.tensor([0.0, 0.23, 0.47, 0.77, 0.9999])
+    for kw in (dict(top_p=0.001), dict(top_p=0.2), dict(top_p=0.83), dict(top_k=1000),
+               dict(top_k=30000, top_p=0.4), dict(min_p=0.5), dict(min_p=0.3)):
+        check(dev, x, u, **kw)
+
+
 def test_two_levels_of_many_ties(dev):
     gen = torch.Generator().manual_seed(5)
     x = torch.randint(0, 3, (6, 5000), generator=gen).float() * 2
