@@ -32,8 +32,8 @@ constexpr int kChunkThreads = 256;
 constexpr int kCandidates = kThreads;
 constexpr int kFew = 256, kFewer = 64;  // tokens that a list is made for
 constexpr int kBins = 2048;
-constexpr int kHeld = 1024;
 constexpr int kMaxSlices = 8192;
+constexpr int kHeld = kMaxSlices / 2;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxChunks = kMaxVocab / kChunk;
 constexpr int kMaxRows = 65535;
@@ -236,7 +236,10 @@ __device__ __forceinline__ float block_max(float v, float* part) {
 }
 
 struct Shared {
-  float top[kMaxSlices];                // each slice's largest logit
+  union {
+    float top[kMaxSlices];              // each slice's largest logit
+    u64 held[kHeld];                    // tokens of one step: (logit, index)
+  };
   union {
     u64 sums[kBins];
     struct {
@@ -252,7 +255,6 @@ struct Shared {
     int i[kWaves];
     float f[kWaves];
   } part;
-  u64 held[kHeld];                      // tokens of one step: (logit, index)
   u64 chunk[kMaxChunks];                // what stays of each chunk
   int ties[kMaxChunks];
   int n, m, first;
@@ -322,6 +324,22 @@ struct Draw {
     return whole;
   }
 
+  // Calls f(slice, its largest logit) for all slices with a number.
+  template <class F>
+  __device__ __forceinline__ void tops(F&& f) const {
+    constexpr int AHEAD = 4;
+    for (int s0 = threadIdx.x; s0 < c.slices; s0 += AHEAD * THREADS) {
+      float v[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a)
+        v[a] = s0 + a * THREADS < c.slices ? sh.top[min(s0 + a * THREADS, kMaxSlices - 1)]
+                                           : -__builtin_inff();
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a)
+        if (v[a] != -__builtin_inff()) f(s0 + a * THREADS, v[a]);
+    }
+  }
+
   // One exchange of a sort between lanes `BY` apart: v and the other's in any order.
   template <int BY>
   static __device__ __forceinline__ void lanes_apart(u64 v, u64& a, u64& b) {
@@ -365,6 +383,7 @@ struct Draw {
         const u64 other = sh.list.swap[threadIdx.x ^ by];
         v = (v > other) == (!(threadIdx.x & by) == down) ? v : other;
       }
+      if ((int)threadIdx.x >= m) continue;            // whole waves
       if (size > 32) v = exchanged<32>(v, down);
       if (size > 16) v = exchanged<16>(v, down);
       if (size > 8) v = exchanged<8>(v, down);
@@ -388,9 +407,7 @@ struct Draw {
       sh.first = kSteps - 1;
     }
     __syncthreads();
-    for (int s = t; s < c.slices; s += THREADS)
-      if (sh.top[s] != -__builtin_inff())
-        atomicAdd(&l.steps[step_of(weight.top, sh.top[s])], 1u);
+    tops([&](int, float v) { atomicAdd(&l.steps[step_of(weight.top, v)], 1u); });
     __syncthreads();
     // the first step that `want` slices reach, or the last
     constexpr int EACH = kSteps / THREADS;
@@ -410,11 +427,11 @@ struct Draw {
     }
     __syncthreads();
     const int last = sh.first;
-    for (int s = t; s < c.slices; s += THREADS)
-      if (sh.top[s] != -__builtin_inff() && step_of(weight.top, sh.top[s]) <= last) {
-        const int at = atomicAdd(&sh.m, 1);
-        if (at < kCandidates) l.active[at] = s;
-      }
+    tops([&](int s, float v) {
+      if (step_of(weight.top, v) > last) return;
+      const int at = atomicAdd(&sh.m, 1);
+      if (at < kCandidates) l.active[at] = s;
+    });
     __syncthreads();
     const int active = sh.m;
     if (active > kCandidates) return false;
@@ -678,41 +695,35 @@ struct Draw {
       u64 above = sh.above;
       // its tokens lie between two keys (two off for rounding)
       // A few in a hundred tokens are in the step: lanes first note which of theirs are, and then
-      // each takes its next one, so that f runs as often as the fullest lane has tokens, not for
-      // each of the 32.
-      auto in_step = [&](auto&& f) {
-        constexpr int AHEAD = 4;                      // pieces of 8 tokens on their way at a time
-        for (int i0 = threadIdx.x; i0 * 8 < c.vocab; i0 += AHEAD * THREADS) {
-          float v[AHEAD][8];
-#pragma unroll
-          for (int a = 0; a < AHEAD; ++a)             // the last one begins earlier
-            x.load_whole(min((i0 + a * THREADS) * 8, c.vocab - 8), v[a]);
-          uint32_t hits = 0;
-#pragma unroll
-          for (int a = 0; a < AHEAD; ++a) {
-            const int i = (i0 + a * THREADS) * 8, from = min(i, c.vocab - 8);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (from + j >= i && step_of(weight.top, v[a][j]) == step) hits |= 1u << (8 * a + j);
-          }
-          for (; hits; hits &= hits - 1) {
-            const int bit = __builtin_ctz(hits);
-            const int i = min((i0 + (bit >> 3) * THREADS) * 8, c.vocab - 8) + (bit & 7);
-            f(i, x.at(i));
-          }
-        }
-      };
-      // they are looked for once, where there are not too many
+      // each keeps its next one, as often as the fullest lane has some.  They are kept where the
+      // slices' largest logits were.
       if (threadIdx.x == 0) sh.n = 0;
       __syncthreads();
-      in_step([&](int i, float v) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kHeld) sh.held[at] = (u64)__float_as_uint(v) << 32 | (uint32_t)i;
-      });
+      constexpr int AHEAD = 4;                        // pieces of 8 tokens on their way at a time
+      for (int i0 = threadIdx.x; i0 * 8 < c.vocab; i0 += AHEAD * THREADS) {
+        float v[AHEAD][8];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)               // the last one begins earlier
+          x.load_whole(min((i0 + a * THREADS) * 8, c.vocab - 8), v[a]);
+        uint32_t hits = 0;
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+          const int i = (i0 + a * THREADS) * 8, from = min(i, c.vocab - 8);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (from + j >= i && step_of(weight.top, v[a][j]) == step) hits |= 1u << (8 * a + j);
+        }
+        for (; hits; hits &= hits - 1) {
+          const int bit = __builtin_ctz(hits);
+          const int i = min((i0 + (bit >> 3) * THREADS) * 8, c.vocab - 8) + (bit & 7);
+          const int to = atomicAdd(&sh.n, 1);
+          if (to < kHeld) sh.held[to] = (u64)__float_as_uint(x.at(i)) << 32 | (uint32_t)i;
+        }
+      }
       __syncthreads();
       const int held = sh.n;
+      if (held > kHeld) return false;
       auto tokens = [&](auto&& f) {
-        if (held > kHeld) return in_step(f);
         for (int i = threadIdx.x; i < held; i += THREADS)
           f((int)(uint32_t)sh.held[i], __uint_as_float((uint32_t)(sh.held[i] >> 32)));
       };
@@ -903,16 +914,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleCall c) {
   const float u = c.u[row];
   const Logits<T> x(c, row);
   float top = -__builtin_inff();
+  constexpr int kAhead = 5;
   const float* tops = c.tops + row * c.slices;
-  for (int i0 = threadIdx.x; i0 < c.slices; i0 += 4 * THREADS) {
-    float v[4];                         // four on their way at a time
+  for (int i0 = threadIdx.x; i0 < c.slices; i0 += kAhead * THREADS) {
+    float v[kAhead];                    // several on their way at a time
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kAhead; ++j) {
       const int i = min(i0 + j * THREADS, c.slices - 1);
       v[j] = c.slice_shift == 0 ? x.at(i) : tops[i];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kAhead; ++j) {
       top = fmaxf(top, v[j]);
       if (i0 + j * THREADS < c.slices) sh.top[i0 + j * THREADS] = v[j];
     }
