@@ -25,6 +25,13 @@ constexpr int kSharedWaves = 4;
 constexpr int kSharedBlock = kTile * kSharedWaves;
 constexpr int kStage = 64;              // positions of a tile in LDS
 constexpr int kSharedWorkgroups = 512;  // 2 on each of 256 CUs: all their registers' room
+// Tables up to which, and sequences times kv heads (and 16 query heads) up to which a sequence by
+// itself is faster: one launch instead of two, and what is read again comes from the L2s.  Both
+// sides measured in us, head_dim 128, bf16, 300 shared of 400 positions in one group: 2 sequences of
+// 80 positions 9.9 (12.5 shared), 16 of 32 heads over 8 10.0 (15.3), 64 13.4 (19.5); 400 of 450
+// positions in groups of 4, 64 sequences 17.1 (20.1), 128 32.8 (28.5), 256 63.4 (55.6).
+constexpr int kShortTable = 512;
+constexpr int kShortUnits = 512;
 constexpr int kStash = 512;             // sequences and groups that a workgroup keeps in LDS
 constexpr int kNarrow = 32;             // columns up to which waves take positions, not columns
 constexpr int kWide = 64;               // columns of an item, at most
@@ -932,6 +939,14 @@ static bool shared_sizes_ok(int64_t seqs, int64_t groups, int32_t n_heads, int32
          seqs * n_heads <= (int64_t)UINT32_MAX / 64 && (int64_t)(p.pieces + 1) * kv_heads <= 1 << 23;
 }
 
+// Few sequences with short tables: one launch that takes each by itself (mtl_paged_attention without
+// a workspace) instead of two.
+static bool alone_is_faster(int64_t seqs, int32_t n_heads, int32_t kv_heads, int64_t width,
+                            int32_t page_size) {
+  const int64_t units = (int64_t)kv_heads * ((n_heads / kv_heads + 15) / 16);
+  return width * page_size <= kShortTable && seqs * units <= kShortUnits;
+}
+
 extern "C" int64_t mtl_paged_attention_shared_workspace_bytes(int64_t seqs, int64_t groups,
                                                               int32_t n_heads, int32_t kv_heads,
                                                               int32_t head_dim, int64_t width,
@@ -939,6 +954,7 @@ extern "C" int64_t mtl_paged_attention_shared_workspace_bytes(int64_t seqs, int6
   if (seqs < 1 || head_dim < 1 ||
       !shared_sizes_ok(seqs, groups, n_heads, kv_heads, width, page_size))
     return 0;
+  if (alone_is_faster(seqs, n_heads, kv_heads, width, page_size)) return 16;   // not used
   const SharedPlan p = shared_plan(seqs, groups, n_heads, kv_heads);
   return p.rows * (head_dim + 2) * 4 + 8 * (p.tiles + seqs * (p.own_tiles + 1));
 }
@@ -966,6 +982,9 @@ extern "C" int mtl_paged_attention_shared(const void* q, int64_t ldq, int64_t ld
                                    p.page_size))
     return MTL_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MTL_ERR_ALIGN;
+  if (alone_is_faster(seqs, n_heads, pool->kv_heads, table->width, p.page_size))
+    return mtl_paged_attention(q, ldq, ldh, pool, table, lens, n_heads, q_type, scale, out, lse,
+                               nullptr, 0, stream);
   const SharedPlan s = shared_plan(seqs, n_groups, n_heads, pool->kv_heads);
   float* parts = static_cast<float*>(workspace);
   float* ml = parts + s.rows * d;

@@ -13,9 +13,10 @@ from tests._sampling import reference as sample_reference
 pytestmark = pytest.mark.gpu
 
 
-def shared_case(dev, sizes, shared, lens, H, Hkv, D, page, typ="bf16", kv="bf16", seed=0, room=1):
+def shared_case(dev, sizes, shared, lens, H, Hkv, D, page, typ="bf16", kv="bf16", seed=0, room=33):
     """Groups whose whole shared pages are held by all, and whose partly shared page is copied; pages
-    and rows that nobody holds are NaN."""
+    and rows that nobody holds are NaN.  ``room``: entries of the table past the longest sequence;
+    tables of more than 512 positions are the ones whose prefixes are read once."""
     gen = torch.Generator().manual_seed(seed)
     width = max([1] + [-(-n // page) for n in lens]) + room
     need = sum(-(-n // page) for n in lens) + sum(s // page for s in shared) + 3
@@ -90,6 +91,24 @@ def test_edges(dev, page, kv):
 def test_heads_and_types(dev, H, Hkv, typ, kv, D):
     check(shared_case(dev, [3, 1, 4], [200, 30, 77], [210, 200, 333, 90, 77, 78, 0, 150], H, Hkv, D,
                       16, typ, kv, H))
+
+
+# tables of up to 512 positions: 512 sequences times kv heads and sets of 16 query heads, and more
+@pytest.mark.parametrize("n,H,Hkv", [(3, 8, 2), (63, 28, 4), (64, 32, 8), (65, 32, 8), (255, 34, 2),
+                                     (300, 17, 1)])
+@pytest.mark.parametrize("typ,kv,D,page", [("bf16", "bf16", 128, 16), ("f16", "e4m3", 64, 32),
+                                           ("f16", "f16", 128, 256)])
+def test_short_tables(dev, n, H, Hkv, typ, kv, D, page):
+    rng = random.Random(n)
+    shared = [rng.choice([0, 17, 64, 300]) for _ in range(n // 3)]
+    lens = [min(s + rng.choice(OWN), 512) if rng.random() < .9 else 0
+            for s in shared for _ in range(3)]
+    check(shared_case(dev, [3] * (n // 3), shared, lens, H, Hkv, D, page, typ, kv, n, 0))
+
+
+@pytest.mark.parametrize("room", [0, 1])
+def test_tables_of_512_and_more(dev, room):
+    check(shared_case(dev, [3, 1], [300, 0], [300, 512, 0, 470], 8, 2, 128, 16, room=room))
 
 
 # 1 to 5 sets of 16 columns, and columns that end inside one
