@@ -27,10 +27,10 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;          // of a row
 constexpr int kWaves = kThreads / 64;
-constexpr int kChunk = 8192;            // tokens of a workgroup of the first two launches
-constexpr int kChunkThreads = 256;
+constexpr int kChunk = 4096;            // tokens of a workgroup of the first two launches
+constexpr int kChunkThreads = 512;
 constexpr int kCandidates = kThreads;
-constexpr int kFew = 256, kFewer = 64;  // tokens that a list is made for
+constexpr int kFew = 384, kFewer = 64;  // tokens that a list is made for
 constexpr int kBins = 2048;
 constexpr int kMaxSlices = 8192;
 constexpr int kHeld = kMaxSlices / 2;
@@ -178,11 +178,11 @@ __device__ __forceinline__ u64 whole_units(double w, int unit) {
 // Steps of the distance to the largest logit, 128 to an octave from 1/4 to 64: the same or a later
 // one for a smaller logit.
 constexpr int kFirstStep = 125 * 128 - 1;
-__device__ __forceinline__ int step_of(float top, float x) {
-  if (x == top) return 0;
-  const int s = (int)(__float_as_uint(top - x) >> 16) - kFirstStep;
+__device__ __forceinline__ int step_at(float distance) {
+  const int s = (int)(__float_as_uint(distance) >> 16) - kFirstStep;
   return min(max(s, 0), kSteps - 1);
 }
+__device__ __forceinline__ int step_of(float top, float x) { return x == top ? 0 : step_at(top - x); }
 
 // ------------------------------------------------------------------------------ workgroup steps
 template <int CTRL, int ROWS>
@@ -399,12 +399,18 @@ struct Draw {
     auto& l = sh.list;
     const int t = threadIdx.x;
     const bool k_set = k < c.vocab;
+    // The step that min-p's border lies in (a little further, for rounding): no token past it stays,
+    // nor is one looked at unless the mass that top-k leaves is asked for.
+    int cut = kSteps;
+    if (m > 0 && (p >= 1 || !k_set))
+      cut = step_at((float)((double)(0.f - log2f((float)m)) / weight.by) * 1.0001f);
+    if (k_set && k > kCandidates && cut == kSteps) return false;
     // a weighed row has another way where its list is too short
-    const int want = k_set ? min(k, kFew) : weighed ? kFewer : kFew;
+    const int want = k_set ? min(k, kFew) : weighed ? kFewer : c.vocab + 1;
     for (int i = t; i < kSteps; i += THREADS) l.steps[i] = 0;
     if (t == 0) {
       sh.n = sh.m = 0;
-      sh.first = kSteps - 1;
+      sh.first = min(kSteps - 1, cut);
     }
     __syncthreads();
     tops([&](int, float v) { atomicAdd(&l.steps[step_of(weight.top, v)], 1u); });
@@ -420,7 +426,7 @@ struct Draw {
       for (int i = 0; i < EACH; ++i) {
         upto += (int)l.steps[t * EACH + i];
         if (upto >= want) {
-          sh.first = t * EACH + i;
+          sh.first = min(t * EACH + i, cut);
           break;
         }
       }
@@ -464,15 +470,10 @@ struct Draw {
       __syncthreads();
       mass = sh.above;
       if (last < kSteps - 1 && !(k_set && k <= n)) {  // tokens outside the list may count
-        if (k_set) return false;
-        if (t == 0) sh.m = 0;
-        __syncthreads();
-        if (t < n && !(w >= m)) sh.m = 1;
-        __syncthreads();
-        const bool low = sh.m;
-        if (!low && p >= 1) return false;
-        mass = p < 1 ? total() : 0;
-        if (!low && !(whole > (u64)(p * (double)mass))) return false;
+        const bool enough = last >= cut;              // ... or not, by min-p
+        if (!enough && (k_set || p >= 1)) return false;
+        if (p < 1) mass = total();
+        if (!enough && !(whole > (u64)(p * (double)mass))) return false;
       }
       const bool keep = t < n && t < k && (p >= 1 || before <= (u64)(p * (double)mass)) &&
                         (w >= m || t == 0) && units > 0;

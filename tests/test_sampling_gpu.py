@@ -63,6 +63,22 @@ def test_large_vocabularies(dev, vocab, kw):
     check(dev, logits_of(gen, 2, vocab, typ), torch.rand(2, generator=gen), **kw)
 
 
+# around the sizes of a list, and min-p's border without a sum
+@pytest.mark.parametrize("vocab", [700, 8192, 50000, 300001])
+@pytest.mark.parametrize("kw", [dict(top_k=383), dict(top_k=385, top_p=0.97), dict(top_k=511),
+                                dict(top_k=513, top_p=0.99), dict(top_k=1500),
+                                dict(top_k=2500, top_p=0.9, temperature=3.0),
+                                dict(top_k=4097, top_p=0.98), dict(top_k=900, min_p=0.05),
+                                dict(top_k=900, top_p=0.8, min_p=0.05), dict(min_p=0.3),
+                                dict(min_p=1e-6, temperature=0.2), dict(min_p=0.7, temperature=60.0),
+                                dict(min_p=0.999999), dict(min_p=0.2, top_p=0.6, temperature=4.0),
+                                dict(min_p=1e-40), dict(top_k=30, min_p=1e-7)], ids=str)
+def test_long_lists(dev, vocab, kw):
+    gen = torch.Generator().manual_seed(vocab + 3)
+    for typ in TYPES:
+        check(dev, logits_of(gen, 3, vocab, typ, peaks=200), torch.rand(3, generator=gen), **kw)
+
+
 @pytest.mark.parametrize("vocab", [600, 33000])
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=7), dict(top_k=400), dict(top_p=0.5),
                                 dict(top_p=0.25, top_k=600), dict(min_p=0.5)], ids=str)
