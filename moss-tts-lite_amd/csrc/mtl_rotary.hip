@@ -8,6 +8,10 @@
 // The angle: the frequency in turns as two doubles, times the position, less its whole turns; the
 // product's rounding comes back from an fma.  What is left is exact to 2^-50 of a turn for any
 // position below 2^53, and float32 from there on.
+//
+// Measured (a copy moves 4.9 TB/s): 16 000 rows of 32 + 8 heads of 128 in bf16, 328 MB in and out,
+// 72 us, 4.5 TB/s; 3300 rows, 68 MB, which stays in the last cache, 13 us, 5.1 TB/s; 18 rows 4 us,
+// where a launch and two trips to the memory (position and frequencies, heads) are all there is.
 #include "mtl_common.h"
 #include "mtl_paged.h"
 #include "mtl_rotary.h"
@@ -18,6 +22,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRotaryWaves = 4;
 constexpr int kMaxHeadDim = 512;
+// Up to so many rows every wave's worth of heads gets a wave of its own, which makes the angles anew.
+// Both sides measured in us, 32 + 8 heads of 128 (of 256): 1 row 3.3 (8.0 by one wave a row), 256
+// 4.6 (9.5), 1024 8.7 (10.7), 2048 14.0 (13.9); of 256 15.8 (21.4) at 1024, 26.9 (24.6) at 2048.
+constexpr int kFewRows = 1024;
 
 struct RotaryHeads {
   const uint16_t* x;
@@ -172,7 +180,7 @@ static void launch_rotary(const RotaryHeads& q, const RotaryHeads& k, int64_t ro
                           bool interleaved, float amplitude, float eps, hipStream_t stream) {
   const int heads = q.heads + k.heads;
   const dim3 grid((unsigned)((rows + kRotaryWaves - 1) / kRotaryWaves),
-                  rows <= 512 ? min(1024, (heads + 64 / G - 1) / (64 / G)) : 1);
+                  rows <= kFewRows ? min(1024, (heads + 64 / G - 1) / (64 / G)) : 1);
   const size_t lds = (size_t)kRotaryWaves * half * sizeof(float2);
 #define MTL_RUN(MODE)                                                                          \
   qk_rotary_kernel<T, G, MODE><<<grid, kRotaryWaves * 64, lds, stream>>>(                      \

@@ -30,7 +30,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kChunk = 4096;            // tokens of a workgroup of the first two launches
 constexpr int kChunkThreads = 512;
 constexpr int kCandidates = kThreads;
-constexpr int kFew = 384, kFewer = 64;  // tokens that a list is made for
+constexpr int kFewer = 64;             // tokens that a weighed row's list is made for
 constexpr int kBins = 2048;
 constexpr int kMaxSlices = 8192;
 constexpr int kHeld = kMaxSlices / 2;
@@ -242,6 +242,7 @@ struct Shared {
   };
   union {
     u64 sums[kBins];
+    int active[kHeld];
     struct {
       uint32_t steps[kSteps];
       int active[kCandidates];
@@ -273,20 +274,26 @@ struct Draw {
   int k;
   double p, m, u;
   bool weighed;
+  // What is left to draw from once the borders are known: tokens down to `key`, the first `ties` of
+  // its own; `mine` of their weight lies in chunk threadIdx.x, and sh.ties[chunk] tokens of the key
+  // in earlier chunks.
+  u64 mine;
+  uint32_t key;
+  int ties, held_step = -1;             // of a long list
 
-  __device__ Draw(const SampleCall& c, int64_t row, Shared& sh, float top, const Settings& s,
+  __device__ __forceinline__ Draw(const SampleCall& c, int64_t row, Shared& sh, float top, const Settings& s,
                   float u)
       : c(c), row(row), sh(sh), x(c, row), weight(top, s.temperature), k(s.k), p(s.p), m(s.m),
         u(u >= 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0),
         weighed(c.weighed && s.weighed(c.vocab)) {}
 
-  __device__ void result(int token, double logprob) {
+  __device__ __forceinline__ void result(int token, double logprob) {
     c.token[row] = token;
     if (c.logprob) c.logprob[row] = (float)logprob;
   }
 
   // The lowest index of the largest logit.
-  __device__ void greedy() {
+  __device__ __forceinline__ void greedy() {
     if (threadIdx.x == 0) sh.first = c.vocab;
     __syncthreads();
     for (int s = threadIdx.x; s < c.slices; s += THREADS) {
@@ -313,7 +320,7 @@ struct Draw {
   }
 
   // The sum of all weights.
-  __device__ u64 total() {
+  __device__ __forceinline__ u64 total() {
     u64 sum = 0, whole;
     if (weighed) {
       for (int i = threadIdx.x; i < c.chunks; i += THREADS) sum += c.sums[row * c.chunks + i];
@@ -395,7 +402,7 @@ struct Draw {
   }
 
   // Draws from a list of candidates; false where a list cannot settle the row.
-  __device__ bool by_list() {
+  __device__ __forceinline__ bool by_list() {
     auto& l = sh.list;
     const int t = threadIdx.x;
     const bool k_set = k < c.vocab;
@@ -404,9 +411,8 @@ struct Draw {
     int cut = kSteps;
     if (m > 0 && (p >= 1 || !k_set))
       cut = step_at((float)((double)(0.f - log2f((float)m)) / weight.by) * 1.0001f);
-    if (k_set && k > kCandidates && cut == kSteps) return false;
     // a weighed row has another way where its list is too short
-    const int want = k_set ? min(k, kFew) : weighed ? kFewer : c.vocab + 1;
+    const int want = k_set ? k : weighed ? kFewer : c.vocab + 1;
     for (int i = t; i < kSteps; i += THREADS) l.steps[i] = 0;
     if (t == 0) {
       sh.n = sh.m = 0;
@@ -433,6 +439,8 @@ struct Draw {
     }
     __syncthreads();
     const int last = sh.first;
+    if (k_set) held_step = last;                      // where the list has no room
+    if (k_set && k > kCandidates && cut == kSteps) return false;
     tops([&](int s, float v) {
       if (step_of(weight.top, v) > last) return;
       const int at = atomicAdd(&sh.m, 1);
@@ -514,7 +522,7 @@ struct Draw {
   // and what lies above it (`above` at first lies above hi).  each(f) calls f(logit) for all tokens
   // in question.  WEIGH: weights in units of 2^-unit, else tokens.
   template <bool WEIGH, class Each>
-  __device__ void border(Each&& each, uint32_t lo, uint32_t hi, u64 limit, uint32_t& key,
+  __device__ __forceinline__ void border(Each&& each, uint32_t lo, uint32_t hi, u64 limit, uint32_t& key,
                          u64& above) {
     constexpr int EACH = kBins / THREADS;
     while (true) {
@@ -574,7 +582,7 @@ struct Draw {
   }
 
   // Draws by passes over the row.
-  __device__ void by_passes() {
+  __device__ __forceinline__ void by_passes() {
     auto row_of = [&](auto&& f) { all([&](int, float v) { f(v); }); };
     const uint32_t low = x.key(-__builtin_inff()) + 1, high = x.key(weight.top);
     uint32_t key = low, at;
@@ -606,13 +614,7 @@ struct Draw {
     // by index: each thread a run of tokens
     const int per = ((c.vocab + THREADS - 1) / THREADS + 7) & ~7;
     const int begin = min(c.vocab, (int)threadIdx.x * per), end = min(c.vocab, begin + per);
-    const float vk = x.of_key(key);
-    const double wk = weight(vk);
-    const u64 tie = wk >= m || vk == weight.top ? whole_units(wk, c.unit) : 0;
-    auto stays = [&](float v) {
-      const double w = weight(v);
-      return w >= m || v == weight.top ? whole_units(w, c.unit) : 0;
-    };
+    const u64 tie = stays(x.of_key(key));
     u64 sum = 0, whole;
     int same = 0, all_same;
     for (int i = begin; i < end; i += 8) {
@@ -647,12 +649,172 @@ struct Draw {
     result(last, log(weight(x.at(last)) / ldexp((double)whole, -c.unit)));
   }
 
-  // Draws from a weighed row: top-p alone, or no filter.  False where min-p cuts deeper.
-  __device__ bool by_chunks() {
-    uint32_t key = x.key(-__builtin_inff()) + 1;
-    int ties = c.vocab;
+  // A token's weight in whole units, 0 where min-p drops it.
+  __device__ __forceinline__ u64 stays(float v) const {
+    const double w = weight(v);
+    return w >= m || v == weight.top ? whole_units(w, c.unit) : 0;
+  }
+
+  // The draw among what is left.
+  __device__ __forceinline__ void in_chunk() {
+    u64 whole, upto = block_scan<WAVES>(mine, sh.part.u, whole);
+    const u64 goal = (u64)(u * (double)whole);
+    if (mine_is_it(mine > 0, upto > goal)) {
+      sh.n = threadIdx.x;
+      sh.above = upto - mine;
+    }
+    __syncthreads();
+    // the draw falls into chunk sh.n, a thread 8 tokens of it
+    static_assert(kChunk % (8 * kThreads) == 0 && kChunk <= 32 * kThreads, "a thread's tokens");
+    constexpr int EACH = kChunk / THREADS;
+    const int chunk = sh.n, begin = chunk * kChunk + threadIdx.x * EACH;
+    u64 w[EACH], sum = 0;
+    int tied = 0, same = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i += 8) {
+      float v[8];
+      x.load(min(begin + i, c.vocab), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool there = begin + i + j < c.vocab && v[j] != -__builtin_inff();
+        const uint32_t b = x.key(v[j]);
+        w[i + j] = there && b >= key ? stays(v[j]) : 0;
+        if (there && b == key) {
+          tied |= 1 << (i + j);
+          ++same;
+        }
+      }
+    }
+    int all_same;
+    int left = ties - sh.ties[chunk] - (block_scan<WAVES>(same, sh.part.i, all_same) - same);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (tied >> i & 1 && left-- <= 0) w[i] = 0;
+      sum += w[i];
+    }
+    const u64 before = sh.above;
+    u64 chunk_whole;
+    upto = before + block_scan<WAVES>(sum, sh.part.u, chunk_whole);
+    if (!mine_is_it(sum > 0, upto > goal)) return;
+    u64 run = upto - sum;
+    int last = -1;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (w[i] && run <= goal) {
+        run += w[i];
+        last = begin + i;
+      }
+    // the weight itself, not in whole units: it may be small
+    result(last, log(weight(x.at(last)) / ldexp((double)whole, -c.unit)));
+  }
+
+  // Tokens kept where the slices' largest logits were, each with its index.
+  struct Held {
+    const u64* of;
+    int n;
+    template <class F>
+    __device__ __forceinline__ void operator()(F&& f) const {
+      for (int i = threadIdx.x; i < n; i += THREADS)
+        f((int)(uint32_t)of[i], __uint_as_float((uint32_t)(of[i] >> 32)));
+    }
+  };
+
+  // `mine` of these tokens; `earlier(chunk)` is what the chunk has besides, a wave at a time.
+  template <class Earlier>
+  __device__ __forceinline__ void of_chunks(const Held& tokens, Earlier&& earlier) {
+    const int chunks = (c.vocab + kChunk - 1) / kChunk;
+    __syncthreads();
+    for (int i = threadIdx.x; i < chunks; i += THREADS) {
+      sh.chunk[i] = 0;
+      sh.ties[i] = 0;
+    }
+    __syncthreads();
+    tokens([&](int i, float v) {
+      if (v == -__builtin_inff()) return;
+      const uint32_t b = x.key(v);
+      if (b > key) atomicAdd(&sh.chunk[i / kChunk], stays(v));
+      if (b == key) atomicAdd(&sh.ties[i / kChunk], 1);
+    });
+    for (int i = wave_id(); i < chunks; i += WAVES) {
+      const u64 v = earlier(i);
+      if (v && (threadIdx.x & 63) == 0) atomicAdd(&sh.chunk[i], v);
+    }
+    __syncthreads();
+    int has = (int)threadIdx.x < chunks ? sh.ties[threadIdx.x] : 0, all_has;
+    const int had = block_scan<WAVES>(has, sh.part.i, all_has) - has;
+    mine = 0;
+    if ((int)threadIdx.x < chunks) {
+      sh.ties[threadIdx.x] = had;
+      mine = sh.chunk[threadIdx.x] + (u64)min(max(ties - had, 0), has) * stays(x.of_key(key));
+    }
+  }
+
+  // The borders where top-k keeps more tokens than a list has room for, all of them in steps up to `last`:
+  // these are kept, and borders looked for among them.
+  __device__ __forceinline__ bool by_held(int last) {
+    if (last == kSteps - 1) return false;
+    if (threadIdx.x == 0) sh.n = sh.m = 0;
+    __syncthreads();
+    tops([&](int s, float v) {
+      if (step_of(weight.top, v) > last) return;
+      const int at = atomicAdd(&sh.m, 1);
+      if (at < kHeld) sh.active[at] = s;
+    });
+    __syncthreads();
+    const int active = sh.m;
+    if (active > kHeld) return false;
+    // 8 tokens at a time, or one
+    const int parts = c.slice_shift == 0 ? 0 : c.slice_shift - 3;
+    for (int i = threadIdx.x; i < active << parts; i += THREADS) {
+      const int from = (sh.active[i >> parts] << c.slice_shift) + (i & ((1 << parts) - 1)) * 8;
+      float v[8];
+      x.load(min(from, c.vocab), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (c.slice_shift == 0 && j > 0) break;
+        if (v[j] == -__builtin_inff() || step_of(weight.top, v[j]) > last) continue;
+        const int to = atomicAdd(&sh.n, 1);
+        if (to < kHeld) sh.held[to] = (u64)__float_as_uint(v[j]) << 32 | (uint32_t)(from + j);
+      }
+    }
+    __syncthreads();
+    const Held tokens{sh.held, sh.n};
+    if (tokens.n > kHeld) return false;
+    auto logits = [&](auto&& f) { tokens([&](int, float v) { f(v); }); };
+    const uint32_t low = x.key(-__builtin_inff()) + 1, high = x.key(weight.top);
+    uint32_t at;
+    u64 above = 0;
+    border<false>(logits, low, high, (u64)k, at, above);
+    key = at;
+    ties = k - (int)above;
+    if (p < 1) {
+      u64 sum = 0, whole;
+      int same = 0, all_same;
+      above = 0;
+      tokens([&](int, float v) {
+        if (x.key(v) > key) sum += whole_units(weight(v), c.unit);
+        same += x.key(v) == key;
+      });
+      block_scan<WAVES>(sum, sh.part.u, whole);
+      block_scan<WAVES>(same, sh.part.i, all_same);
+      const double limit = p * (ldexp((double)whole, -c.unit) +
+                                (double)min(ties, all_same) * weight(x.of_key(key)));
+      border<true>(logits, low, high, (u64)ldexp(limit, c.unit), at, above);
+      const int stay = that_stay(limit, above, weight(x.of_key(at)));
+      ties = at == key ? min(ties, stay) : stay;
+      key = at;
+    }
+    of_chunks(tokens, [](int) { return (u64)0; });
+    return true;
+  }
+
+  // The border of a weighed row: top-p alone, or no filter.  False where min-p cuts deeper.
+  __device__ __forceinline__ bool by_chunks() {
+    key = x.key(-__builtin_inff()) + 1;
+    ties = c.vocab;
     const u64* sums = c.sums + row * c.chunks;
-    u64 mine = (int)threadIdx.x < c.chunks ? sums[threadIdx.x] : 0, whole;
+    u64 whole;
+    mine = (int)threadIdx.x < c.chunks ? sums[threadIdx.x] : 0;
     block_scan<WAVES>(mine, sh.part.u, whole);
     if (p < 1) {
       // the step of the border, of all chunks together
@@ -724,10 +886,7 @@ struct Draw {
       __syncthreads();
       const int held = sh.n;
       if (held > kHeld) return false;
-      auto tokens = [&](auto&& f) {
-        for (int i = threadIdx.x; i < held; i += THREADS)
-          f((int)(uint32_t)sh.held[i], __uint_as_float((uint32_t)(sh.held[i] >> 32)));
-      };
+      const Held tokens{sh.held, held};
       const float far = step == kSteps - 1 ? __builtin_inff()
                                            : __uint_as_float((uint32_t)(step + 1 + kFirstStep) << 16);
       const float near = step == 0 ? 0.f : __uint_as_float((uint32_t)(step + kFirstStep) << 16);
@@ -738,87 +897,16 @@ struct Draw {
       const double wk = weight(x.of_key(key));
       if (!(wk >= m)) return false;
       ties = that_stay(limit, above, wk);
-      // what stays of each chunk
-      __syncthreads();
-      for (int i = threadIdx.x; i < c.chunks; i += THREADS) {
-        sh.chunk[i] = 0;
-        sh.ties[i] = 0;
-      }
-      __syncthreads();
-      tokens([&](int i, float v) {
-        if (v == -__builtin_inff()) return;
-        const uint32_t b = x.key(v);
-        if (b > key) atomicAdd(&sh.chunk[i / kChunk], whole_units(weight(v), c.unit));
-        if (b == key) atomicAdd(&sh.ties[i / kChunk], 1);
-      });
-      for (int i = wave_id(); i < c.chunks; i += WAVES) {       // its earlier steps
+      of_chunks(tokens, [&](int i) {                            // its earlier steps
         u64 v = 0;
         for (int e = threadIdx.x & 63; e < step; e += 64) v += steps[i * kSteps + e];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.chunk[i], v);
-      }
-      __syncthreads();
-      int has = (int)threadIdx.x < c.chunks ? sh.ties[threadIdx.x] : 0, all_has;
-      const int had = block_scan<WAVES>(has, sh.part.i, all_has) - has;
-      mine = 0;
-      if ((int)threadIdx.x < c.chunks) {
-        mine = sh.chunk[threadIdx.x] +
-               (u64)min(max(ties - had, 0), has) * whole_units(wk, c.unit);
-        sh.ties[threadIdx.x] = had;
-      }
+        return v;
+      });
     } else if ((int)threadIdx.x < c.chunks) {
       sh.ties[threadIdx.x] = 0;
     }
-    u64 upto = block_scan<WAVES>(mine, sh.part.u, whole);
-    const u64 goal = (u64)(u * (double)whole);
-    if (mine_is_it(mine > 0, upto > goal)) {
-      sh.n = threadIdx.x;
-      sh.above = upto - mine;
-    }
-    __syncthreads();
-    // the draw falls into chunk sh.n, a thread 8 tokens of it
-    static_assert(kChunk % (8 * kThreads) == 0 && kChunk <= 32 * kThreads, "a thread's tokens");
-    constexpr int EACH = kChunk / THREADS;
-    const int chunk = sh.n, begin = chunk * kChunk + threadIdx.x * EACH;
-    u64 w[EACH], sum = 0;
-    int tied = 0, same = 0;
-#pragma unroll
-    for (int i = 0; i < EACH; i += 8) {
-      float v[8];
-      x.load(min(begin + i, c.vocab), v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool there = begin + i + j < c.vocab && v[j] != -__builtin_inff();
-        const uint32_t b = x.key(v[j]);
-        w[i + j] = there && b >= key ? whole_units(weight(v[j]), c.unit) : 0;
-        if (there && b == key) {
-          tied |= 1 << (i + j);
-          ++same;
-        }
-      }
-    }
-    int all_same;
-    int left = ties - sh.ties[chunk] - (block_scan<WAVES>(same, sh.part.i, all_same) - same);
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      if (tied >> i & 1 && left-- <= 0) w[i] = 0;
-      sum += w[i];
-    }
-    const u64 before = sh.above;
-    u64 chunk_whole;
-    upto = before + block_scan<WAVES>(sum, sh.part.u, chunk_whole);
-    if (!mine_is_it(sum > 0, upto > goal)) return true;
-    u64 run = upto - sum;
-    int last = -1;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i)
-      if (w[i] && run <= goal) {
-        run += w[i];
-        last = begin + i;
-      }
-    // the weight itself, not in whole units: it may be small
-    result(last, log(weight(x.at(last)) / ldexp((double)whole, -c.unit)));
     return true;
   }
 };
@@ -939,7 +1027,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleCall c) {
   if (s.greedy()) return d.greedy();
   if ((s.k < c.vocab || s.p < 1.f || s.m > 0.f) && d.by_list()) return;
   __syncthreads();
-  if (d.weighed && d.by_chunks()) return;
+  if (d.held_step >= 0 ? d.by_held(d.held_step) : d.weighed && d.by_chunks()) return d.in_chunk();
   __syncthreads();
   d.by_passes();
 }
