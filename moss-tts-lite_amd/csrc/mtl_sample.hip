@@ -856,7 +856,6 @@ struct Draw {
       }
       __syncthreads();
       u64 above = sh.above;
-      // its tokens lie between two keys (two off for rounding)
       // A few in a hundred tokens are in the step: lanes first note which of theirs are, and then
       // each keeps its next one, as often as the fullest lane has some.  They are kept where the
       // slices' largest logits were.
@@ -887,13 +886,15 @@ struct Draw {
       const int held = sh.n;
       if (held > kHeld) return false;
       const Held tokens{sh.held, held};
+      // The step's tokens lie between two keys: distances are off by 2^-24 of themselves, which are many
+      // keys where the logit is near 0, and the bounds' own rounding is within two.
       const float far = step == kSteps - 1 ? __builtin_inff()
                                            : __uint_as_float((uint32_t)(step + 1 + kFirstStep) << 16);
       const float near = step == 0 ? 0.f : __uint_as_float((uint32_t)(step + kFirstStep) << 16);
       const uint32_t low = key, high = x.key(weight.top);
-      const uint32_t lo = max(x.key(weight.top - far), low + 2) - 2;
+      const uint32_t lo = max(x.key(weight.top - far * 1.000001f), low + 2) - 2;
       border<true>([&](auto&& f) { tokens([&](int, float v) { f(v); }); }, lo,
-                   min(x.key(weight.top - near) + 2, high), limit_units, key, above);
+                   min(x.key(weight.top - near * 0.999999f) + 2, high), limit_units, key, above);
       const double wk = weight(x.of_key(key));
       if (!(wk >= m)) return false;
       ties = that_stay(limit, above, wk);

@@ -72,6 +72,10 @@ def test_large_vocabularies(dev, vocab, kw):
                                 dict(top_k=900, top_p=0.8, min_p=0.05), dict(min_p=0.3),
                                 dict(min_p=1e-6, temperature=0.2), dict(min_p=0.7, temperature=60.0),
                                 dict(min_p=0.999999), dict(min_p=0.2, top_p=0.6, temperature=4.0),
+                                dict(min_p=0.02, temperature=2.5),
+                                dict(min_p=0.02, top_p=0.8, temperature=2.5),
+                                dict(min_p=0.002, top_p=0.3, temperature=2.5),
+                                dict(min_p=0.0001, top_p=0.8, temperature=2.5),
                                 dict(min_p=1e-40), dict(top_k=30, min_p=1e-7)], ids=str)
 def test_long_lists(dev, vocab, kw):
     gen = torch.Generator().manual_seed(vocab + 3)
@@ -121,6 +125,20 @@ def test_draws_in_every_chunk(dev, vocab):
     for kw in (dict(), dict(top_p=0.9), dict(top_p=0.999)):
         tok = check(dev, x, u, **kw)
         assert (tok[1:] >= tok[:-1]).all() and int(tok[-1]) > vocab - vocab // 10
+
+
+def test_borders_near_zero(dev):
+    """Logits near 0 lie closer than their distances to the largest can tell apart: the border's step
+    holds tokens above the logit that it begins at."""
+    gen = torch.Generator().manual_seed(21)
+    vocab = 40000
+    x = -3 + 0.03 * torch.randn(4, vocab, generator=gen)
+    for r in range(4):
+        at = torch.randperm(vocab, generator=gen)[:2001]
+        x[r, at] = 1e-8 * torch.randn(2001, generator=gen)
+        x[r, at[0]] = 12.5 + 0.0625 * r              # distances of 12.5 .. are where steps begin
+    for p in (0.05, 0.085, 0.12):
+        check(dev, x, torch.rand(4, generator=gen), temperature=2.5, top_p=p)
 
 
 def test_large_masked_rows(dev):
