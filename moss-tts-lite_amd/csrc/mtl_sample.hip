@@ -439,7 +439,8 @@ struct Draw {
     }
     __syncthreads();
     const int last = sh.first;
-    if (k_set) held_step = last;                      // where the list has no room
+    // where the list has no room
+    if (k_set || cut < kSteps - 1) held_step = k_set ? last : cut;
     if (k_set && k > kCandidates && cut == kSteps) return false;
     tops([&](int s, float v) {
       if (step_of(weight.top, v) > last) return;
@@ -749,8 +750,8 @@ struct Draw {
     }
   }
 
-  // The borders where top-k keeps more tokens than a list has room for, all of them in steps up to `last`:
-  // these are kept, and borders looked for among them.
+  // The borders where top-k or min-p keeps more tokens than a list has room for, all of them in steps
+  // up to `last`: these are kept, and borders looked for among them.
   __device__ __forceinline__ bool by_held(int last) {
     if (last == kSteps - 1) return false;
     if (threadIdx.x == 0) sh.n = sh.m = 0;
@@ -782,21 +783,30 @@ struct Draw {
     if (tokens.n > kHeld) return false;
     auto logits = [&](auto&& f) { tokens([&](int, float v) { f(v); }); };
     const uint32_t low = x.key(-__builtin_inff()) + 1, high = x.key(weight.top);
+    const bool k_set = k < c.vocab;
     uint32_t at;
     u64 above = 0;
-    border<false>(logits, low, high, (u64)k, at, above);
-    key = at;
-    ties = k - (int)above;
+    key = low;
+    ties = c.vocab;
+    if (k_set) {
+      border<false>(logits, low, high, (u64)k, at, above);
+      key = at;
+      ties = k - (int)above;
+    }
     if (p < 1) {
       u64 sum = 0, whole;
-      int same = 0, all_same;
+      int same = 0, all_same = 0;
       above = 0;
-      tokens([&](int, float v) {
-        if (x.key(v) > key) sum += whole_units(weight(v), c.unit);
-        same += x.key(v) == key;
-      });
-      block_scan<WAVES>(sum, sh.part.u, whole);
-      block_scan<WAVES>(same, sh.part.i, all_same);
+      if (k_set) {
+        tokens([&](int, float v) {
+          if (x.key(v) > key) sum += whole_units(weight(v), c.unit);
+          same += x.key(v) == key;
+        });
+        block_scan<WAVES>(sum, sh.part.u, whole);
+        block_scan<WAVES>(same, sh.part.i, all_same);
+      } else {
+        whole = total();
+      }
       const double limit = p * (ldexp((double)whole, -c.unit) +
                                 (double)min(ties, all_same) * weight(x.of_key(key)));
       border<true>(logits, low, high, (u64)ldexp(limit, c.unit), at, above);
@@ -1028,7 +1038,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleCall c) {
   if (s.greedy()) return d.greedy();
   if ((s.k < c.vocab || s.p < 1.f || s.m > 0.f) && d.by_list()) return;
   __syncthreads();
-  if (d.held_step >= 0 ? d.by_held(d.held_step) : d.weighed && d.by_chunks()) return d.in_chunk();
+  bool found = d.held_step >= 0 && d.by_held(d.held_step);
+  __syncthreads();
+  if (!found) found = d.weighed && d.by_chunks();
+  if (found) return d.in_chunk();
   __syncthreads();
   d.by_passes();
 }
