@@ -889,12 +889,28 @@ struct Draw {
           const int bit = __builtin_ctz(hits);
           const int i = min((i0 + (bit >> 3) * THREADS) * 8, c.vocab - 8) + (bit & 7);
           const int to = atomicAdd(&sh.n, 1);
-          if (to < kHeld) sh.held[to] = (u64)__float_as_uint(x.at(i)) << 32 | (uint32_t)i;
+          if (to < kHeld) sh.held[to] = (uint32_t)i;
         }
       }
       __syncthreads();
       const int held = sh.n;
       if (held > kHeld) return false;
+      // their logits, all on their way at once (read again where they were noted, they would wait for
+      // one another)
+      constexpr int ALL = kHeld / THREADS;
+      uint32_t at[ALL];
+      float logit[ALL];
+#pragma unroll
+      for (int i = 0; i < ALL; ++i) {
+        const int to = (int)threadIdx.x + i * THREADS;
+        at[i] = to < held ? (uint32_t)sh.held[to] : 0;
+        logit[i] = x.at((int)at[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < ALL; ++i)
+        if ((int)threadIdx.x + i * THREADS < held)
+          sh.held[threadIdx.x + i * THREADS] = (u64)__float_as_uint(logit[i]) << 32 | at[i];
+      __syncthreads();
       const Held tokens{sh.held, held};
       // The step's tokens lie between two keys: distances are off by 2^-24 of themselves, which are many
       // keys where the logit is near 0, and the bounds' own rounding is within two.
@@ -910,7 +926,14 @@ struct Draw {
       ties = that_stay(limit, above, wk);
       of_chunks(tokens, [&](int i) {                            // its earlier steps
         u64 v = 0;
-        for (int e = threadIdx.x & 63; e < step; e += 64) v += steps[i * kSteps + e];
+        const int e0 = 2 * (threadIdx.x & 63);
+        u64 two[kSteps / 128][2];                     // all on their way at once
+#pragma unroll
+        for (int j = 0; j < kSteps / 128; ++j)
+          __builtin_memcpy(two[j], steps + i * kSteps + e0 + 128 * j, 16);
+#pragma unroll
+        for (int j = 0; j < kSteps / 128; ++j)
+          v += (e0 + 128 * j < step ? two[j][0] : 0) + (e0 + 1 + 128 * j < step ? two[j][1] : 0);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
         return v;
