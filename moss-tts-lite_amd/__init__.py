@@ -9,6 +9,8 @@ Modules
 ``ops``      torch-facing int4 GEMM / pack / dequant ops
 ``gptq``     the GPTQ linear module and the reference's format helpers
 ``paged``    paged key-value cache of several sequences: attention, writes, page bookkeeping
+``rotary``   q and k heads' RMSNorm and rotation from integer positions
+``sampling`` token draws: temperature, top-k, top-p, min-p
 ``build``    the hipcc recipe of ``libmtl_hip.so``
 """
 __version__ = "0.1.0"

@@ -2,21 +2,41 @@
 // sequences form groups that hold their first positions in the same pages (gfx950).
 //
 // A group's shared positions are attended once for all of its queries: the query heads of one kv
-// head, of all its sequences, are the columns of the matrix products, kWide of them at a time, and
-// K and V of a tile of 32 positions stay in a wave's registers for all of these columns.  What a
+// head, of all its sequences, are the columns of the matrix products, up to kWide at a time.  What a
 // sequence holds by itself follows in the same launch, and a second launch joins the parts of each
-// query head.
+// query head.  Products, softmax and the two-term weights are those of mtl_paged_attention.
 //
 // * Items: (group, up to kWide columns, its shared positions) and (sequence, up to kWide query
 //   heads of a kv head, its own positions), cut into blocks of 128 positions, each with a cost by
 //   its columns.  They stand in one row, which the workgroups of a kv head share evenly; each
-//   finds its piece on the device from lengths and groups.
-// * A wave takes every fourth tile of a piece, with running maxima and sums of its own, joined
-//   through LDS at a piece's end.  As soon as a product has used up K (or V) in the registers, the
-//   next tile's is on its way there.
+//   finds its piece on the device from lengths and groups, which it keeps in LDS where there is
+//   room.
+// * Up to kNarrow columns: a wave takes every fourth tile of 32 positions, K and V in registers, with
+//   running maxima and sums of its own, joined through LDS at a piece's end.  As soon as a product
+//   has used up K (or V) in the registers, the next tile's is on its way there.  More columns would
+//   spill, or read every tile for each 32 of them.
+// * Up to kWide columns: tiles of kStage positions pass through LDS; two waves take half of the
+//   columns each, two the other half of the positions.
 // * Groups that overlap or leave the batch give undefined results, but every index is bounded.
 // * Shared positions count in multiples of 16, so that tiles begin at whole halves; the rest of a
 //   shared prefix is read as the sequences' own.
+// * A short prefix of few sequences stays with the sequences (Batch::group): an item of its own
+//   costs more than what is read again from the L2 (13 us by themselves, 20 shared).
+//
+// Measured, head_dim 128, bf16, 32 heads over 8 kv heads: 192 sequences on a prefix of 6001
+// positions and up to 700 of their own (121 MB of K and V once; 19 GFLOP) 70 + 6 us in the two
+// launches, 77 for a call, where the matrix rate would take 16 and memory 17.  A tile of 64
+// positions by 64 columns takes some 3600 cycles, of which vector instructions are issued in 85 of
+// 100 and the matrix units work in 25 to 40: the softmax of 4096 scores and their two terms are the
+// bound, 4 instructions or so a score each.  About 18 000 cycles of a piece do not grow with it
+// (lists, queries, first tile; joining its waves).  16 sentences with up to 6 candidates (67 MB) 20 +
+// 4 us; a prefix in e4m3 (51 MB) 22 + 4; head_dim 64 in f16, 8 groups, 17 + 5; two sequences of 700
+// positions 8.4 + 3.5.
+//
+// Tried and slower: 64 columns a wave with K and V straight from the caches (222 us for the 192
+// sequences), 128-column tiles of 4 waves (ahead past some 20 000 positions
+// only, 154 against 160 us, and behind below), page ids by scalar loads, 384, 768 and 1024
+// workgroups (768 takes many small groups at head_dim 64 from 89 to 70 us and others from 23 to 30).
 #include "mtl_paged_tiles.h"
 
 namespace mtl {

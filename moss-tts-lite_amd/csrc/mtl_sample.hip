@@ -5,18 +5,28 @@
 // Weights are of 64 bits and their sums whole numbers of 2^-44, whose order changes nothing.
 //
 // The work is one read of the logits; no row is ever sorted:
-// * A first launch cuts rows into slices of 32 tokens and keeps the largest logit of each (rows of
-//   up to kMaxSlices tokens need none: they fit LDS).
-// * Rows that need the sum of all weights (top-p without a small top-k; no filter) are weighed in a
-//   second launch: a sum for each 8192 tokens, and for top-p by the logits' distance to the
-//   largest, in steps of 1/128 octave.
-// * In the last launch a workgroup takes a row.  The slices' largest logits give a bound that at
-//   least n tokens reach (n slices' largest do); the slices that reach it are read again and give a
-//   short list, in which every token counts those ahead of it and their weight.  Where a list cannot
-//   settle a top-p row, its border lies in one step, whose tokens are weighed by digits of their
-//   ordered keys; then the draw falls into one chunk of 8192, which is read again.
-// * What neither settles (a large top-k, a wide min-p, thousands of equal logits) takes passes over
-//   the whole row.
+// * A first launch cuts rows into slices of 32 tokens (128 past 262 144) and keeps the largest logit
+//   of each (rows of up to kMaxSlices tokens need none: they fit LDS).
+// * Rows that need the sum of all weights (top-p without top-k; no filter) are weighed in a second
+//   launch: a sum for each kChunk tokens, and for top-p by the logits' distance to the largest, in
+//   steps of 1/128 octave.
+// * In the last launch a workgroup takes a row.  The slices' largest logits, counted by steps, give a
+//   step that top-k's tokens lie within (as many slices' largest do); min-p's border is a step known
+//   beforehand.  The slices that reach it are read again: up to kCandidates tokens are sorted in
+//   registers, by the order for the borders and by index for the draw.  More of them are kept in LDS,
+//   and borders found among them by digits of their ordered keys.
+// * Where a list of kFewer cannot settle a row that top-p alone cuts, its border lies in one step,
+//   whose tokens are gathered; the draw then falls into one chunk, which is read again.
+// * What none of these settles (over kHeld tokens within the step; thousands of equal logits) takes
+//   passes over the whole row: 290 us for 151 000 tokens, where kept tokens take 46.
+//
+// What bounds it: a chain of dependent steps in one workgroup (barriers, 3 to 5 trips to memory), not
+// the bytes.  Measured: one row of 151 936 bf16 logits, top-k 50, 2.5 + 12 us; 31
+// rows of 1025, top-k 25 and top-p, 10 us in one launch; 24 rows of 151 936 by top-p 4 + 10 + 16 us;
+// 96 float32 rows with a setting each (58 MB) 10 + 11 + 16 us, and 60 in the last where a row's
+// top-p border is past its list: that row's workgroup reads its 600 KB alone.  The first
+// launch reads 5.6 TB/s there.  Tried and slower: 1024 threads a row, ranks by comparing all pairs of
+// a list, more kept tokens (96 KB of LDS: even, and 287 -> 354 us for 500 rows).
 #include "mtl_common.h"
 #include "mtl_paged.h"
 #include "mtl_sample.h"
@@ -27,13 +37,17 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;          // of a row
 constexpr int kWaves = kThreads / 64;
-constexpr int kChunk = 4096;            // tokens of a workgroup of the first two launches
+// Tokens of a workgroup of the first two launches (8192 tokens and 256 threads: one row by top-p 26 us
+// for 22, no filter 24 for 20, 24 rows by top-p 29.6 for 28.6).
+constexpr int kChunk = 4096;
 constexpr int kChunkThreads = 512;
 constexpr int kCandidates = kThreads;
-constexpr int kFewer = 64;             // tokens that a weighed row's list is made for
+// Tokens that a weighed row's list is made for: 24 rows of top-p 0.95 28.6 us, with 32 51 (rows whose
+// border is past their list), with 128 32.6 (a longer sort for all).
+constexpr int kFewer = 64;
 constexpr int kBins = 2048;
 constexpr int kMaxSlices = 8192;
-constexpr int kHeld = kMaxSlices / 2;
+constexpr int kHeld = kMaxSlices / 2;   // tokens kept, in the room of the slices' largest logits
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxChunks = kMaxVocab / kChunk;
 constexpr int kMaxRows = 65535;
