@@ -34,9 +34,9 @@
 // positions 8.4 + 3.5.
 //
 // Tried and slower: 64 columns a wave with K and V straight from the caches (222 us for the 192
-// sequences), 128-column tiles of 4 waves (ahead past some 20 000 positions
-// only, 154 against 160 us, and behind below), page ids by scalar loads, 384, 768 and 1024
-// workgroups (768 takes many small groups at head_dim 64 from 89 to 70 us and others from 23 to 30).
+// sequences), 128-column tiles of 4 waves (ahead past some 20 000 positions only, 154 against 160 us,
+// and behind below), page ids by scalar loads, 384, 768 and 1024 workgroups (768 takes many
+// small groups at head_dim 64 from 89 to 70 us and others from 23 to 30).
 #include "mtl_paged_tiles.h"
 
 namespace mtl {

@@ -89,7 +89,8 @@ def paged_attention_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     number of sequences) are a group, and its first ``shared[g]`` positions (int32 ``[n]``) lie in
     the same pages for all of them, or in copies of these: a page that :func:`pages_extend` copied
     holds the same K and V up to where the fork was made.  They are read through the table row of
-    the group's first sequence that reaches them all.  Shorter and empty sequences of a group
+    the group's first sequence that reaches them all, or, where that is faster, through each
+    sequence's own.  Shorter and empty sequences of a group
     attend to what their length holds.  Results are those of :func:`paged_attention`, with sums in
     another order, and the same call gives the same bits.  K and V that any sequence of a group
     attends to are finite (an infinity or NaN there may give NaN in all of the group)."""
