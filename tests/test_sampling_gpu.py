@@ -216,6 +216,21 @@ def test_a_setting_for_each_row(dev):
         assert int(one) == int(a[r])
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_mixed_settings(dev, seed):
+    # every way through a row beside every other
+    gen = torch.Generator().manual_seed(100 + seed)
+    rows = 12
+    vocab = [5300, 8192, 8193, 30000, 65537, 151936][seed % 6]
+    x = logits_of(gen, rows, vocab, TYPES[seed % 3], spread=[0.3, 1.0, 2.0, 4.0][seed % 4],
+                  peaks=[1, 20, 600][seed // 4])
+    pick = lambda *z: torch.tensor([z[int(i)] for i in torch.randint(0, len(z), (rows,),
+                                                                    generator=gen)])
+    kw = dict(temperature=pick(0.3, 0.9, 1.3, 2.0, 3.0), top_k=pick(0, 0, 30, 480, 1100, 3000).int(),
+              top_p=pick(1.0, 0.95, 0.8, 0.4), min_p=pick(0.0, 0.0, 1e-4, 0.004, 0.05))
+    check(dev, x, torch.rand(rows, generator=gen), **kw)
+
+
 def test_random_numbers_at_the_ends(dev):
     gen = torch.Generator().manual_seed(4)
     x = logits_of(gen, 1, 2000, torch.float32).expand(6, 2000)
@@ -278,7 +293,8 @@ def test_repeats_captures_and_streams(dev):
     x = logits_of(gen, 20, 50000, torch.bfloat16).to(dev)
     u = torch.rand(20, generator=gen).to(dev)
     t = torch.linspace(0.2, 2, 20).to(dev)
-    for kw in (dict(top_k=50), dict(top_p=0.97), dict()):
+    for kw in (dict(top_k=50), dict(top_p=0.97), dict(), dict(top_k=1500, top_p=0.9),
+               dict(top_p=0.8, min_p=0.02)):
         want = sampling.sample(x, u, t, return_logprob=True, **kw)
         graphs = []
         torch.cuda.synchronize()
