@@ -37,12 +37,13 @@
 // sequences), 128-column tiles of 4 waves (ahead past some 20 000 positions only, 154 against 160 us,
 // and behind below), page ids by scalar loads, 384, 768 and 1024 workgroups (768 takes many
 // small groups at head_dim 64 from 89 to 70 us and others from 23 to 30).
+#include "mtl_paged_items.h"
 #include "mtl_paged_tiles.h"
 
 namespace mtl {
 
 constexpr int kSharedWaves = 4;
-constexpr int kSharedBlock = kTile * kSharedWaves;
+static_assert(kSharedBlock == kTile * kSharedWaves, "a tile of each wave");
 constexpr int kStage = 64;              // positions of a tile in LDS
 constexpr int kSharedWorkgroups = 512;  // 2 on each of 256 CUs: all their registers' room
 // Tables up to which, and sequences times kv heads (and 16 query heads) up to which a sequence by
@@ -53,17 +54,6 @@ constexpr int kSharedWorkgroups = 512;  // 2 on each of 256 CUs: all their regis
 constexpr int kShortTable = 512;
 constexpr int kShortUnits = 512;
 constexpr int kStash = 512;             // sequences and groups that a workgroup keeps in LDS
-constexpr int kNarrow = 32;             // columns up to which waves take positions, not columns
-constexpr int kWide = 64;               // columns of an item, at most
-
-// What a block of an item costs by its columns, and an item by itself.
-__host__ __device__ constexpr int block_cost(int columns) {
-  return columns <= 16 ? 3 : columns <= kNarrow ? 4 : 8;
-}
-constexpr int kItemCost = 12;
-__host__ __device__ constexpr int item_cost(int columns, int blocks) {
-  return blocks ? kItemCost + blocks * block_cost(columns) : 0;
-}
 
 struct SharedCall {
   const uint16_t* q;
@@ -96,16 +86,6 @@ struct Lists {
   int lens[kStash], groups[kStash + 1], shared[kStash];
   int2 own[kStash];                     // a sequence's own positions [x, y)
 };
-
-__device__ __forceinline__ int blocks_in(int positions) {
-  return (positions + kSharedBlock - 1) / kSharedBlock;
-}
-
-// The cost of `columns` columns over `blocks` blocks, `wide` (a power of two) of them an item.
-__device__ __forceinline__ int cost_of(int columns, int blocks, int wide) {
-  const int rest = columns & (wide - 1);
-  return columns / wide * item_cost(wide, blocks) + (rest ? item_cost(rest, blocks) : 0);
-}
 
 struct Batch {
   const SharedCall& a;
@@ -174,7 +154,8 @@ struct Batch {
 // of sequences.
 template <int WIDE>
 struct Row {
-  int per_group, per_seq, groups_upto, seqs_upto, shared_cost, total, pieces, each, longer;
+  int per_group, per_seq, groups_upto, seqs_upto, shared_cost, total, pieces;
+  Pieces cut;
 
   __device__ __forceinline__ Row(const SharedCall& a, const Batch& batch) {
     const int lane = threadIdx.x & 63;
@@ -203,24 +184,13 @@ struct Row {
     total = shared_cost + __builtin_amdgcn_readlane(seqs_upto, 63);
     // no piece is shorter than a block
     pieces = max(1, min(a.pieces, total / most));
-    each = total / pieces;
-    longer = total - each * pieces;
+    cut.each = total / pieces;
+    cut.longer = total - cut.each * pieces;
   }
 
-  // Pieces differ by one in length at most.
-  __device__ __forceinline__ int start(int piece) const {
-    return piece * each + min(piece, longer);
-  }
-  __device__ __forceinline__ int piece_of(int at) const {
-    const int head = longer * (each + 1);
-    return at < head ? at / (each + 1) : longer + (at - head) / max(each, 1);
-  }
-  // The pieces that an item of `columns` columns and `blocks` blocks from `base` on lies in.
   __device__ __forceinline__ int2 pieces_of(int base, int blocks, int columns) const {
-    base += kItemCost;
-    return blocks ? make_int2(piece_of(base),
-                              piece_of(base + (blocks - 1) * block_cost(columns)))
-                  : make_int2(0, -1);
+    const Span x = cut.pieces_of(base, blocks, columns);
+    return make_int2(x.x, x.y);
   }
 };
 
@@ -714,15 +684,6 @@ struct Piece {
   }
 };
 
-// The blocks [x, y) of an item that fall into a piece: blocks that begin within [lo, hi).
-__device__ __forceinline__ int2 blocks_within(int base, int blocks, int columns, int lo, int hi) {
-  const int each = block_cost(columns);
-  base += kItemCost;
-  const int x = lo <= base ? 0 : (lo - base + each - 1) / each;
-  const int y = hi <= base ? 0 : (hi - base + each - 1) / each;
-  return make_int2(min(max(x, 0), blocks), min(max(y, 0), blocks));
-}
-
 // What the second launch goes by.
 template <int WIDE>
 __device__ __forceinline__ void write_items(const Batch& batch, const Row<WIDE>& row) {
@@ -781,7 +742,7 @@ __global__ void __launch_bounds__(kSharedWaves * 64, 2) paged_shared_kernel(Shar
     return;
   }
   if (piece >= row.pieces || row.total <= 0) return;
-  const int lo = row.start(piece), hi = row.start(piece + 1);
+  const int lo = row.cut.start(piece), hi = row.cut.start(piece + 1);
   if (lo >= hi) return;
   Piece<QT, KT, D, N> p(batch, pool, kvh, lds);
   const int64_t slot = (int64_t)blockIdx.x * 2 * WIDE;
@@ -828,19 +789,12 @@ __global__ void __launch_bounds__(kSharedWaves * 64, 2) paged_shared_kernel(Shar
       end = __builtin_amdgcn_readfirstlane(at.y);
       blocks = blocks_in(end - begin);
     }
-    const int full = max(item_cost(WIDE, blocks), 1);
-    const int skip = lo > base ? max(min((lo - base) / full, columns / WIDE), 0) : 0;
-    base += skip * full;
-    for (int c = skip * WIDE; c < columns; c += WIDE) {
-      const int n = min(WIDE, columns - c);
-      const int2 b = blocks_within(base, blocks, n, lo, hi);
-      if (b.x < b.y)
-        p.attend(first, c, n, leader, begin + b.x * kSharedBlock,
-                 min(begin + b.y * kSharedBlock, end), a.whole + (own ? heads * D : 0),
-                 a.whole_ml + (own ? 2 * heads : 0),
-                 b.x == 0 && b.y == blocks ? -1 : slot + (b.x == 0) * WIDE);
-      base += item_cost(n, blocks);
-    }
+    items_within<WIDE>(base, columns, blocks, lo, hi, [&](int c, int n, Span b) {
+      p.attend(first, c, n, leader, begin + b.x * kSharedBlock,
+               min(begin + b.y * kSharedBlock, end), a.whole + (own ? heads * D : 0),
+               a.whole_ml + (own ? 2 * heads : 0),
+               b.x == 0 && b.y == blocks ? -1 : slot + (b.x == 0) * WIDE);
+    });
   }
 }
 

@@ -208,6 +208,26 @@ def test_more_groups_than_sequences(dev):
     check(shared_case(dev, sizes, shared, [610, 600, 777, 700, 730], 8, 2, 128, 16, seed=9))
 
 
+# 64 query heads to a kv head and more: a sequence is whole items of 64 columns, several of a lane's
+# run of sequences, and some have nothing of their own
+@pytest.mark.parametrize("n", [65, 96, 192])
+@pytest.mark.parametrize("H,Hkv", [(64, 1), (71, 1), (128, 1), (128, 2), (512, 8)])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_many_sequences_of_wide_heads(dev, n, H, Hkv, grouped):
+    rng = random.Random(n + H)
+    sizes, shared, lens = [], [], []
+    while len(lens) < n:
+        m = min(rng.randint(1, 12) if grouped else 1, n - len(lens))
+        s = rng.choice([0, 40, 128, 260, 300]) if grouped else 0
+        sizes.append(m)
+        shared.append(s)
+        for _ in range(m):
+            r = rng.random()
+            lens.append(0 if r < .15 else rng.randint(0, s) if r < .3 else
+                        s + rng.choice([1, 100, 128, 129, 300, 640]))
+    check(shared_case(dev, sizes, shared, lens, H, Hkv, 64, 16, seed=n))
+
+
 def test_growing_and_falling_scores(dev):
     # the running maximum moves in every tile, or never after the first
     for sign in (1, -1):
