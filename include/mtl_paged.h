@@ -91,7 +91,7 @@ int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh, const mtl_page_
  * prefixes, and tables of up to 512 positions of few sequences, through each sequence's own row.
  * The result is that of mtl_paged_attention, with sums in another order.
  *   groups   int32 [n_groups + 1] (device), ascending from 0 to seqs; a sequence outside of them
- *            is attended by itself
+ *            is attended by itself, and so are all where the numbers do not ascend
  *   shared   int32 [n_groups] (device), counted in whole multiples of 16; past a sequence's own
  *            length nothing counts for it, negative ones count as 0.  A group of one sequence
  *            shares nothing

@@ -17,7 +17,8 @@
 //   spill, or read every tile for each 32 of them.
 // * Up to kWide columns: tiles of kStage positions pass through LDS; two waves take half of the
 //   columns each, two the other half of the positions.
-// * Groups that overlap or leave the batch give undefined results, but every index is bounded.
+// * Groups whose numbers do not ascend are not there, and numbers past the batch count as its end: so
+//   groups never overlap, which the sum of all costs needs to stay within 32 bits.
 // * Shared positions count in multiples of 16, so that tiles begin at whole halves; the rest of a
 //   shared prefix is read as the sequences' own.
 // * A short prefix of few sequences stays with the sequences (Batch::group): an item of its own
@@ -85,6 +86,7 @@ struct Group {
 struct Lists {
   int lens[kStash], groups[kStash + 1], shared[kStash];
   int2 own[kStash];                     // a sequence's own positions [x, y)
+  int falls[kSharedWaves];              // of each wave: whether a group begins behind its end
 };
 
 struct Batch {
@@ -92,16 +94,27 @@ struct Batch {
   Lists& l;
   int wide;                             // columns of an item, at most
   bool near;
+  int n_groups;                         // 0 where they do not ascend
 
   __device__ __forceinline__ Batch(const SharedCall& a, Lists& l, int wide)
       : a(a), l(l), wide(wide), near(a.seqs <= kStash && a.n_groups <= kStash) {
-    if (!near) return;
-    for (int i = threadIdx.x; i < max(a.seqs, a.n_groups + 1); i += kSharedWaves * 64) {
+    bool falls = false;
+    const int entries = near ? max(a.seqs, a.n_groups + 1) : a.n_groups;
+    for (int i = threadIdx.x; i < entries; i += kSharedWaves * 64) {
+      if (i < a.n_groups) falls |= a.groups[i] > a.groups[i + 1];
+      if (!near) continue;
       if (i < a.seqs) l.lens[i] = clamp_len(a.lens[i], a.cap);
       if (i <= a.n_groups) l.groups[i] = a.groups[i];
       if (i < a.n_groups) l.shared[i] = a.shared[i];
     }
+    const bool any = __any(falls);
+    if ((threadIdx.x & 63) == 0) l.falls[wave_id()] = any;
     __syncthreads();
+    int found = 0;
+#pragma unroll
+    for (int i = 0; i < kSharedWaves; ++i) found |= l.falls[i];
+    n_groups = __builtin_amdgcn_readfirstlane(found) ? 0 : a.n_groups;
+    if (!near) return;
     for (int i = threadIdx.x; i < a.seqs; i += kSharedWaves * 64) l.own[i] = find_own(i);
     __syncthreads();
   }
@@ -125,7 +138,7 @@ struct Batch {
 
   // The group of a sequence: -1 for none.
   __device__ __forceinline__ int group_of(int seq, Group& g) const {
-    int lo = 0, hi = a.n_groups;        // groups below lo begin at or before seq
+    int lo = 0, hi = n_groups;          // groups below lo begin at or before seq
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (start(mid) <= seq) lo = mid + 1;
@@ -159,12 +172,12 @@ struct Row {
 
   __device__ __forceinline__ Row(const SharedCall& a, const Batch& batch) {
     const int lane = threadIdx.x & 63;
-    per_group = (a.n_groups + 63) / 64;
+    per_group = (batch.n_groups + 63) / 64;
     per_seq = (a.seqs + 63) / 64;
     int cost = 0, widest = min(a.per_kv, WIDE);
     for (int i = 0; i < per_group; ++i) {
       const int64_t at = (int64_t)lane * per_group + i;
-      if (at >= a.n_groups) break;
+      if (at >= batch.n_groups) break;
       const Group g = batch.group((int)at);
       const int columns = (g.end - g.begin) * a.per_kv;
       cost += cost_of(columns, blocks_in(g.shared), WIDE);
@@ -695,7 +708,7 @@ __device__ __forceinline__ void write_items(const Batch& batch, const Row<WIDE>&
     int base = before_groups;
     for (int i = 0; i < row.per_group; ++i) {
       const int64_t at = (int64_t)lane * row.per_group + i;
-      if (at >= a.n_groups) break;
+      if (at >= batch.n_groups) break;
       const Group g = batch.group((int)at);
       const int blocks = blocks_in(g.shared), columns = (g.end - g.begin) * a.per_kv;
       if (!blocks) continue;
@@ -758,7 +771,7 @@ __global__ void __launch_bounds__(kSharedWaves * 64, 2) paged_shared_kernel(Shar
   while (base < hi) {
     int first, columns, leader, begin, end, blocks;
     if (!own) {
-      if (i >= a.n_groups) {
+      if (i >= batch.n_groups) {
         own = true;
         i = 0;
         base = row.shared_cost;

@@ -86,7 +86,7 @@ def paged_attention_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     (``mtl_paged_attention_shared``): forks of one sequence, requests on one prompt.
 
     Sequences ``groups[g]`` to ``groups[g + 1] - 1`` (int32 ``[n + 1]``, ascending from 0 to the
-    number of sequences) are a group, and its first ``shared[g]`` positions (int32 ``[n]``) lie in
+    number of sequences; where it does not ascend, each sequence is by itself) are a group, and its first ``shared[g]`` positions (int32 ``[n]``) lie in
     the same pages for all of them, or in copies of these: a page that :func:`pages_extend` copied
     holds the same K and V up to where the fork was made.  They are read through the table row of
     the group's first sequence that reaches them all, or, where that is faster, through each

@@ -162,6 +162,29 @@ def test_sequences_outside_the_groups(dev):
     check(a)
 
 
+@pytest.mark.parametrize("n", [6, 300, 600])     # sequences in LDS or not
+@pytest.mark.parametrize("repeats", [1, 250, 600])
+def test_groups_that_do_not_ascend(dev, n, repeats):
+    """Overlapping groups are not there: each sequence is attended by itself."""
+    rng = random.Random(n)
+    a = shared_case(dev, [n], [64], [rng.choice([0, 64, 65, 200]) for _ in range(n)], 8, 2, 64, 16,
+                    room=40)
+    want = None
+    for starts in ([0, n] * repeats, [n, 0] * repeats, [0, 2, 1] + [n] * repeats,
+                   [0, 2 ** 31 - 1, -(2 ** 31)] * repeats, [0] * repeats + [n, n - 1]):
+        a["groups"] = torch.tensor(starts, dtype=torch.int32, device=dev)
+        if (a["groups"][1:] >= a["groups"][:-1]).all():
+            continue
+        a["shared"] = torch.full((len(starts) - 1,), 64, dtype=torch.int32, device=dev)
+        if want is None:
+            want = check(a)
+        assert torch.equal(paged.paged_attention_shared(**a), want)
+    # numbers past the batch are its ends
+    a["groups"] = torch.tensor([-5, n + 3, 2 ** 31 - 1], dtype=torch.int32, device=dev)
+    a["shared"] = torch.full((2,), 64, dtype=torch.int32, device=dev)
+    check(a)
+
+
 def test_holes_and_long_lens(dev):
     a = shared_case(dev, [3], [128], [140, 200, 170], 8, 2, 128, 16, seed=4)
     a["table"][:, 2] = -1                            # a hole in the shared pages
