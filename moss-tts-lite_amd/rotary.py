@@ -26,19 +26,30 @@ from . import ops
 
 def rotary_freqs(turned: int, base: float = 10000.0, factor: float = 1.0,
                  original: int | None = None, slow: float = 1.0, fast: float = 32.0,
-                 device="cuda") -> torch.Tensor:
+                 device="cuda", ramp: str = "dims") -> torch.Tensor:
     """float64 ``[turned / 2]`` frequencies in radians a position: f_t = base^(-2t / turned).
 
     ``factor`` > 1 stretches them for contexts ``factor`` times as long.  Without ``original``
     every frequency is divided by it (positions are interpolated).  With ``original``, the context
-    a model was trained on, a dim that makes n = original f_t / (2 pi) turns within it keeps its
-    frequency from ``fast`` turns on, is divided by ``factor`` up to ``slow`` turns, and in between
-    gets (1 - g) f_t / factor + g f_t with g = (n - slow) / (fast - slow).  Raising the base
-    instead, by factor^(turned / (turned - 2)), is a matter of ``base``."""
+    a model was trained on, a dim that makes ``fast`` turns or more within it keeps its frequency,
+    one that makes ``slow`` turns or fewer is divided by ``factor``, and in between it gets
+    (1 - g) f_t / factor + g f_t.  g falls from 1 to 0
+
+    * with ``ramp="dims"`` evenly from dim to dim, where dim t makes original f_t / (2 pi) turns:
+      g = (b - t) / (b - a), a (rounded down, at least 0) the dim of ``fast`` turns, b (rounded up,
+      below ``turned``) that of ``slow``.  Checkpoints whose configuration has ``rope_type`` "yarn"
+      (``beta_slow``, ``beta_fast``) are made for this, with :func:`rotary_amplitude`;
+    * with ``ramp="turns"`` with the number n of turns: g = (n - slow) / (fast - slow).  This is for
+      configurations that give ``low_freq_factor`` and ``high_freq_factor`` (here ``slow`` and
+      ``fast``), with amplitude 1.
+
+    Raising the base instead, by factor^(turned / (turned - 2)), is a matter of ``base``."""
     if turned < 0 or turned % 2:
         raise RuntimeError(f"turned must be even, got {turned}")
     if not (base > 0 and factor > 0):
         raise RuntimeError("base and factor must be positive")
+    if ramp not in ("dims", "turns"):
+        raise RuntimeError(f'ramp must be "dims" or "turns", got {ramp!r}')
     t = torch.arange(0, turned, 2, dtype=torch.float64)
     f = base ** (-t / max(turned, 1))
     if factor != 1.0:
@@ -47,14 +58,31 @@ def rotary_freqs(turned: int, base: float = 10000.0, factor: float = 1.0,
         else:
             if not (original > 0 and fast > slow):
                 raise RuntimeError("original must be positive and fast above slow")
-            keep = ((original * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+            if ramp == "turns":
+                keep = ((original * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+            else:
+                keep = _kept_by_dims(t / 2, turned, base, original, slow, fast)
             f = f / factor * (1 - keep) + f * keep
     return f.to(device)
 
 
+def _kept_by_dims(t: torch.Tensor, turned: int, base: float, original: int, slow: float,
+                  fast: float) -> torch.Tensor:
+    """How much of dim t's own frequency stays where it falls evenly over the dims."""
+    if not (base > 1 and slow > 0):
+        raise RuntimeError('base must be above 1 and slow above 0 for ramp="dims"')
+    a, b = (turned * math.log(original / (2 * math.pi * n)) / (2 * math.log(base))
+            for n in (fast, slow))
+    a, b = max(math.floor(a), 0), min(math.ceil(b), turned - 1)
+    if b <= 0:                                       # no dim makes more than `slow` turns
+        return torch.zeros_like(t)
+    return 1 - ((t - a) / max(b - a, 1)).clamp(0, 1)  # a = b: dims up to a stay
+
+
 def rotary_amplitude(factor: float) -> float:
     """0.1 ln(factor) + 1 (1 up to factor 1): what cosines and sines are multiplied with where
-    :func:`rotary_freqs` stretches by turns, so that the softmax over more keys stays as sharp."""
+    :func:`rotary_freqs` stretches with ``original`` and ``ramp="dims"``, so that the softmax over
+    more keys stays as sharp."""
     return 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
 
 

@@ -119,3 +119,46 @@ def test_frequencies():
                dict(turned=8, factor=2.0, original=64, slow=4.0, fast=4.0)):
         with pytest.raises(RuntimeError):
             rotary.rotary_freqs(**kw, device="cpu")
+
+
+@pytest.mark.parametrize("turned,base,factor,original,slow,fast,a,b", [
+    (128, 1e6, 4.0, 32768, 1.0, 32.0, 23, 40), (64, 1e4, 8.0, 4096, 1.0, 32.0, 10, 23),
+    (128, 5e5, 2.0, 8192, 2.0, 16.0, 21, 32), (96, 1e7, 40.0, 2048, 1.0, 64.0, 4, 18)])
+def test_frequencies_that_fall_from_dim_to_dim(turned, base, factor, original, slow, fast, a, b):
+    """What rope type "yarn" means: from the dim of `fast` turns, rounded down, to that of `slow`
+    turns, rounded up, in equal steps."""
+    turns = [original * base ** (-2 * t / turned) / (2 * math.pi) for t in (a, a + 1, b - 1, b)]
+    assert turns[0] >= fast > turns[1] and turns[2] > slow >= turns[3]
+    f = rotary.rotary_freqs(turned, base, factor, original, slow, fast, "cpu")
+    for t in range(turned // 2):
+        g = 1.0 if t <= a else 0.0 if t >= b else (b - t) / (b - a)
+        want = base ** (-2 * t / turned) * (g + (1 - g) / factor)
+        assert abs(float(f[t]) - want) <= 1e-12 * want, t
+
+
+def test_frequencies_that_fall_with_the_turns():
+    # wavelengths of original / 4 and shorter keep theirs, of original and longer are divided
+    f = rotary.rotary_freqs(128, 5e5, device="cpu")
+    g = rotary.rotary_freqs(128, 5e5, 8.0, 8192, slow=1.0, fast=4.0, device="cpu", ramp="turns")
+    for t in range(64):
+        n = 8192 * float(f[t]) / (2 * math.pi)
+        keep = min(max((n - 1) / 3, 0), 1)
+        want = float(f[t]) * (keep + (1 - keep) / 8)
+        assert abs(float(g[t]) - want) <= 1e-12 * want, t
+    # some of the values that such a checkpoint's program has, in float32
+    for t, part in ((28, 1.0), (29, 0.8281684), (32, 0.3711222), (34, 0.1902107), (35, 0.125)):
+        assert abs(float(g[t] / f[t]) - part) <= 3e-7
+
+
+def test_frequencies_of_short_contexts():
+    f = rotary.rotary_freqs(64, 1e4, device="cpu")
+    # no dim makes a turn; none makes 32 (dim 0 begins the fall); all make 32
+    assert torch.equal(rotary.rotary_freqs(64, 1e4, 4.0, 6, device="cpu"), f / 4)
+    g = rotary.rotary_freqs(64, 1e4, 4.0, 100, device="cpu")
+    assert g[0] == f[0] and (g[1:] < f[1:]).all() and torch.equal(g[10:], f[10:] / 4)
+    assert torch.equal(rotary.rotary_freqs(64, 1e4, 4.0, 1 << 30, device="cpu"), f)
+    assert torch.equal(rotary.rotary_freqs(64, 1e4, 4.0, 6, device="cpu", ramp="turns"), f / 4)
+    assert rotary.rotary_freqs(0, 1e4, 4.0, 100, device="cpu").numel() == 0
+    for kw in (dict(ramp="dim"), dict(base=1.0), dict(base=0.5), dict(slow=0.0)):
+        with pytest.raises(RuntimeError):
+            rotary.rotary_freqs(**{**dict(turned=64, factor=4.0, original=100, device="cpu"), **kw})
