@@ -42,8 +42,11 @@ typedef struct mtl_sample_settings {
  * which the weights of those that stay, summed by index, exceed u[r] times their whole sum; logprob
  * the logarithm of w_i over that sum.  A temperature that is not above 0 gives the first of the
  * order, logprob 0.  A NaN counts as -infinity, which has weight 0; beside +infinity everything
- * finite has weight 0.  A row of -infinity only: -1, logprob -infinity.  The sums are of 64 bits,
- * in an order that goes by the call's shape and settings: the same call gives the same bits.
+ * finite has weight 0.  A row of -infinity only: -1, logprob -infinity.
+ * Sums are whole numbers of 64 bits, so that their order changes nothing: a weight counts as a
+ * multiple of 2^-n, with the largest n up to 51 for which vocab 2^n is at most 2^63 (51 up to 4096
+ * tokens, 45 up to 2^18, 43 at 2^20).  So borders are right to half of 2^-n a token, and a token of
+ * less weight than that is not drawn, unless it is the first of the order.
  *   logits   [rows, vocab] of type, ld elements apart (0: every row draws from the same ones)
  *   u        fp32 [rows] in [0, 1) (others count as the nearest of these, NaN as 0)
  *   token    int64 [rows];  logprob  NULL, or fp32 [rows]

@@ -2,7 +2,9 @@
 //
 // Everything is decided by sums of weights, and a row has as many borders as tokens: with float32
 // sums (2^-24 of the whole) one row in some thousands would draw another token than the definition.
-// Weights are of 64 bits and their sums whole numbers of 2^-44, whose order changes nothing.
+// Weights are of 64 bits and their sums whole numbers of 2^-51 up to 4096 tokens, of twice that for
+// each doubling (2^-45 up to 2^18 tokens, 2^-43 at 2^20: a row of the largest weights is 2^63 then),
+// whose order changes nothing.  A border may be off by half a unit for each token before it.
 //
 // The work is one read of the logits; no row is ever sorted:
 // * A first launch cuts rows into slices of 32 tokens (128 past 262 144) and keeps the largest logit
@@ -51,6 +53,7 @@ constexpr int kHeld = kMaxSlices / 2;   // tokens kept, in the room of the slice
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxChunks = kMaxVocab / kChunk;
 constexpr int kMaxRows = 65535;
+constexpr int kMostUnit = 51;           // a weight beside 2^52, which rounds it, stays below 2^53
 
 constexpr int kSteps = 1024;
 
@@ -183,7 +186,7 @@ struct Weight {
   }
 };
 
-// A weight (at most 1) in whole units of 2^-unit, unit <= 44: the sum with 2^52 rounds to them.
+// A weight (at most 1) in whole units of 2^-unit, unit <= kMostUnit: the sum with 2^52 rounds to them.
 __device__ __forceinline__ u64 whole_units(double w, int unit) {
   const double one = __longlong_as_double((u64)(1023 + unit) << 52);
   return (u64)__double_as_longlong(fma(w, one, 0x1p52)) - (u64)__double_as_longlong(0x1p52);
@@ -1138,8 +1141,8 @@ extern "C" int mtl_sample(const void* logits, int64_t ld, int64_t rows, int64_t 
   const SamplePlan p = sample_plan(rows, vocab, *settings);
   if (p.bytes > 0 && (!workspace || ws_bytes < p.bytes)) return MTL_ERR_WORKSPACE;
   if (p.bytes > 0 && !aligned16(workspace)) return MTL_ERR_ALIGN;
-  int unit = 44;
-  while (unit > 0 && (vocab >> (62 - unit)) > 0) --unit;
+  int unit = kMostUnit;
+  while (vocab > (int64_t)1 << (63 - unit)) --unit;
   char* ws = static_cast<char*>(workspace);
   float* tops = reinterpret_cast<float*>(ws + p.steps_bytes + p.sums_bytes);
   const SampleCall c{logits, ld, (int)vocab, __builtin_ctz(p.slice), (int)p.slices, unit, p.chunks,

@@ -34,9 +34,11 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Ten
 
     Each setting is a number or a tensor ``[rows]`` (fp32, ``top_k`` int32).  A temperature that is
     not above 0 takes the first of the order.  NaN logits count as -infinity and are never drawn; a
-    row of nothing else gives -1.  Weights and sums are of 64 bits.  With ``return_logprob`` also
-    the fp32 logarithm of the token's probability among those that stayed (0 without temperature,
-    -infinity for -1).  An expanded row of logits draws several tokens from it."""
+    row of nothing else gives -1.  Weights are of 64 bits and summed as the nearest multiples of
+    2^-n, n = 51 up to 4096 tokens and one less for each doubling (45 for 151 936): a token of less
+    than half of that is not drawn.  With ``return_logprob`` also the fp32 logarithm of the token's
+    probability among those that stayed (0 without temperature, -infinity for -1).  An expanded row
+    of logits draws several tokens from it."""
     t, k, p, m = (x if isinstance(x, torch.Tensor) else None
                   for x in (temperature, top_k, top_p, min_p))
     op = ops.overload("sample_logprob" if return_logprob else "sample")

@@ -141,6 +141,22 @@ def test_borders_near_zero(dev):
         check(dev, x, torch.rand(4, generator=gen), temperature=2.5, top_p=p)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=(1 << 20) - 1), dict(top_p=1 - 2.0 ** -24)],
+                         ids=str)
+def test_a_tail_of_tiny_weights(dev, kw):
+    """2^20 - 1 tokens of 2^-42.1 beside one of weight 1: together 2^-22.1, which u can tell apart."""
+    n = 1 << 20
+    x = torch.full((1, n), -29.2)
+    x[0, -1] = 0.0
+    w = math.exp(float(x[0, 0]))
+    u = torch.tensor([2.0 ** -23])
+    assert 2.0 ** -23 < (n - 1) * w - 2.0 ** -24        # also behind top-p's border
+    token, logprob = sampling.sample(x.to(dev), u.to(dev), return_logprob=True, **kw)
+    # each weight counts to half of 2^-43: sums up to a token, and the whole, are off by 2^-24
+    assert abs((int(token) + 1) * w - 2.0 ** -23) <= 2.0 ** -24 + 2.0 ** -40
+    assert abs(float(logprob) - math.log(w)) <= 2 ** -23 * 29.2 + 2.0 ** -21
+
+
 def test_large_masked_rows(dev):
     inf = float("inf")
     gen = torch.Generator().manual_seed(18)
