@@ -388,6 +388,16 @@ def test_repeats_bitwise_captures_and_streams(dev):
     assert torch.equal(graphs[0][1][0], check(a))
 
 
+@pytest.mark.parametrize("typ,kv", [("bf16", "e4m3"), ("f16", "f16"), ("f16", "e4m3")])
+def test_the_same_call_gives_the_same_bits(dev, typ, kv):
+    a = shared_case(dev, [20, 2, 40], [3000, 300, 777], [3000 + 40 * i for i in range(20)] +
+                    [300, 0] + [777 + 9 * i for i in range(40)], 32, 8, 128, 32, typ, kv, seed=13)
+    want = paged.paged_attention_shared(**a, return_lse=True)
+    for _ in range(30):
+        got = paged.paged_attention_shared(**a, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_schemas(dev):
     from moss_tts_lite_amd import ops
 

@@ -232,6 +232,30 @@ def test_a_setting_for_each_row(dev):
         assert int(one) == int(a[r])
 
 
+@pytest.mark.parametrize("vocab", [3000, 9000, 70001])
+def test_a_row_draws_the_same_in_any_batch(dev, vocab):
+    """Token and probability to the last bit, whether settings are numbers or tensors and whatever the
+    other rows' are; borders among ties of weights that are no whole units."""
+    gen = torch.Generator().manual_seed(vocab)
+    rows = 40
+    x = torch.randint(0, 60, (rows, vocab), generator=gen).float() / 7
+    x[::4] = x[::4].round()
+    x, u = x.to(dev), torch.rand(rows, generator=gen).to(dev)
+    pick = lambda *z: torch.tensor([z[int(i)] for i in torch.randint(0, len(z), (rows,),
+                                                                    generator=gen)]).to(dev)
+    kw = dict(temperature=pick(0.3, 0.9, 1.7), top_k=pick(0, 0, 30, 480, 700, 2500).int(),
+              top_p=pick(1.0, 0.9, 0.5), min_p=pick(0.0, 0.0, 0.01))
+    token, logprob = sampling.sample(x, u, return_logprob=True, **kw)
+    for r in range(rows):
+        one = sampling.sample(x[r:r + 1], u[r:r + 1], return_logprob=True,
+                              **{k: v[r].item() for k, v in kw.items()})
+        assert int(one[0]) == int(token[r]) and torch.equal(one[1], logprob[r:r + 1]), r
+        mixed = {k: v[r].item() if i % 2 == r % 2 else v[r:r + 1] for i, (k, v) in
+                 enumerate(kw.items())}
+        two = sampling.sample(x[r:r + 1], u[r:r + 1], return_logprob=True, **mixed)
+        assert torch.equal(two[0], one[0]) and torch.equal(two[1], one[1]), r
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_mixed_settings(dev, seed):
     # every way through a row beside every other
