@@ -86,8 +86,8 @@ int mtl_paged_attention(const void* q, int64_t ldq, int64_t ldh, const mtl_page_
 /*
  * mtl_paged_attention for sequences that share a prefix: sequences groups[g] .. groups[g + 1] - 1
  * are a group, whose first shared[g] positions lie in the same pages or hold the same K and V
- * (copies of a partly filled page), and are read once for all of its queries, through the table
- * row of its first sequence that reaches them all (or, where none does, of its longest); short
+ * (copies of a partly filled page), and are read once for each 64 of its query heads of a kv head,
+ * through the table row of its first sequence that reaches them all (or, where none does, of its longest); short
  * prefixes, and tables of up to 512 positions of few sequences, through each sequence's own row.
  * The result is that of mtl_paged_attention, with sums in another order.
  *   groups   int32 [n_groups + 1] (device), ascending from 0 to seqs; a sequence outside of them

@@ -51,7 +51,8 @@ typedef struct mtl_sample_settings {
  *   u        fp32 [rows] in [0, 1) (others count as the nearest of these, NaN as 0)
  *   token    int64 [rows];  logprob  NULL, or fp32 [rows]
  *   workspace  mtl_sample_workspace_bytes(...) bytes, 16-byte aligned, any content, one launch at a
- *              time
+ *              time.  Past 8192 tokens a row takes 2 bytes or so for each token where top_p may cut
+ *              it without top_k (a pointer may hold any setting), an eighth of one otherwise
  * vocab at most 2^20, rows at most 65535.
  */
 int64_t mtl_sample_workspace_bytes(int64_t rows, int64_t vocab, int32_t type,

@@ -1,10 +1,12 @@
 // Attention of one new token of each sequence over a paged key-value cache, where consecutive
 // sequences form groups that hold their first positions in the same pages (gfx950).
 //
-// A group's shared positions are attended once for all of its queries: the query heads of one kv
-// head, of all its sequences, are the columns of the matrix products, up to kWide at a time.  What a
-// sequence holds by itself follows in the same launch, and a second launch joins the parts of each
-// query head.  Products, softmax and the two-term weights are those of mtl_paged_attention.
+// A group's shared positions are attended for all of its queries together: the query heads of one
+// kv head, of all its sequences, are the columns of the matrix products, up to kWide at a time, and
+// each kWide columns read the K and V once (with kWide query heads to a kv head a sequence fills
+// them, and nothing is read together).  What a sequence holds by itself follows in the same launch,
+// and a second launch joins the parts of each query head.  Products, softmax and the two-term
+// weights are those of mtl_paged_attention.
 //
 // * Items: (group, up to kWide columns, its shared positions) and (sequence, up to kWide query
 //   heads of a kv head, its own positions), cut into blocks of 128 positions, each with a cost by
@@ -24,15 +26,27 @@
 // * A short prefix of few sequences stays with the sequences (Batch::group): an item of its own
 //   costs more than what is read again from the L2 (13 us by themselves, 20 shared).
 //
-// Measured, head_dim 128, bf16, 32 heads over 8 kv heads: 192 sequences on a prefix of 6001
-// positions and up to 700 of their own (121 MB of K and V once; 19 GFLOP) 70 + 6 us in the two
-// launches, 77 for a call, where the matrix rate would take 16 and memory 17.  A tile of 64
-// positions by 64 columns takes some 3600 cycles, of which vector instructions are issued in 85 of
-// 100 and the matrix units work in 25 to 40: the softmax of 4096 scores and their two terms are the
-// bound, 4 instructions or so a score each.  About 18 000 cycles of a piece do not grow with it
-// (lists, queries, first tile; joining its waves).  16 sentences with up to 6 candidates (67 MB) 20 +
-// 4 us; a prefix in e4m3 (51 MB) 22 + 4; head_dim 64 in f16, 8 groups, 17 + 5; two sequences of 700
-// positions 8.4 + 3.5.
+// Measured, head_dim 128, bf16, 32 heads over 8 kv heads, the two launches in a kernel trace: 192
+// sequences on a prefix of 6001 positions and up to 700 of their own (121 MB of K and V once; 19
+// GFLOP) 83 + 6 us (77 for a whole call outside of the trace), where the matrix rate would take 16
+// and memory 17; 16 sentences with up to 6 candidates (67 MB) 24 + 5; prefixes in e4m3 (51 MB)
+// 25 + 4; head_dim 64 in f16, 3 groups, 19 + 5; two sequences of 700 positions 9 + 4.
+// * A tile of 64 positions by 64 columns takes some 3600 cycles, of which vector instructions are
+//   issued in 85 of 100 and the matrix units work in 25 to 40.  A wave has 48 matrix and some 250
+//   vector instructions for it, with 16 scores a lane: 95 for maxima, exponentials and sums, 48 for
+//   the weights' two terms, 32 for V's bytes, 75 for pages, addresses and staging; and 41 more for
+//   each 16 columns whose sums are brought to a new maximum.
+// * By the items' costs the sequences' own parts are 41 of 100 of all work of the 192 sequences, 74
+//   of the candidates, 53 of the e4m3 case and 50 of the two sequences, and some 70 of 100 of that
+//   is what an item costs by itself: a workgroup takes 1 or 2 blocks by 4 columns, clears four waves'
+//   sums and joins them twice through LDS.
+// * About 18 000 cycles of a piece do not grow with it (lists, queries, first tile; joining).
+// * Past 512 sequences or groups the lists do not fit LDS and every workgroup looks for each
+//   sequence's group in memory.  By groups of 16 on 600 positions and up to 200 of their own, 1024
+//   sequences take 218 us; of 16 on 300 and up to 100, 4096 sequences 797.
+// mtl_paged_attention on the same inputs, a call: 500 us for the 192 sequences (77 here), 32 for
+// the candidates (27), 55 in e4m3 (27), 19.5 for head_dim 64 (23.2), 7.9 for the two sequences
+// (12.1), 418 and 965 for the 1024 and 4096 (218, 797).
 //
 // Tried and slower: 64 columns a wave with K and V straight from the caches (222 us for the 192
 // sequences), 128-column tiles of 4 waves (ahead past some 20 000 positions only, 154 against 160 us,

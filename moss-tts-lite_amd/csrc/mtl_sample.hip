@@ -19,13 +19,16 @@
 //   and borders found among them by digits of their ordered keys.
 // * Where a list of kFewer cannot settle a row that top-p alone cuts, its border lies in one step,
 //   whose tokens are gathered; the draw then falls into one chunk, which is read again.
-// * What none of these settles (over kHeld tokens within the step; thousands of equal logits) takes
-//   passes over the whole row: 290 us for 151 000 tokens, where kept tokens take 46.
+// * What none of these settles (over kHeld tokens within the step; thousands of equal logits; top-p
+//   without top-k past a list in rows that need no slices) takes passes over the whole row: 290 us
+//   for 151 000 tokens, where kept tokens take 46; 22 for 31 rows of 1025 by top-p 0.8 alone, 37 for
+//   rows of 8192, though they lie in LDS.
 //
 // What bounds it: a chain of dependent steps in one workgroup (barriers, 3 to 5 trips to memory), not
-// the bytes.  Measured: one row of 151 936 bf16 logits, top-k 50, 2.5 + 12 us; 31
-// rows of 1025, top-k 25 and top-p, 10 us in one launch; 24 rows of 151 936 by top-p 4 + 10 + 16 us;
-// 96 float32 rows with a setting each (58 MB) 10 + 11 + 16 us, and 60 in the last where a row's
+// the bytes.  Measured: one row of 151 936 bf16 logits, top-k 50, 2.5 + 12 us; 31 rows of 1025,
+// top-k 25 and top-p, 10 us in one launch (min-p alone 10, no filter 9); 24 rows of 151 936 by top-p
+// 4 + 12 + 16 us, whose steps (8 KB a chunk, written once and read twice) are as many bytes as bf16
+// logits; 96 float32 rows with a setting each (58 MB) 10 + 11 + 16 us, and 60 in the last where a row's
 // top-p border is past its list: that row's workgroup reads its 600 KB alone.  The first
 // launch reads 5.6 TB/s there.  Tried and slower: 1024 threads a row, ranks by comparing all pairs of
 // a list, more kept tokens (96 KB of LDS: even, and 287 -> 354 us for 500 rows).

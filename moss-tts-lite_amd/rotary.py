@@ -1,9 +1,11 @@
 """Rotation of queries and keys by their positions, with the RMSNorm of each head in the same pass.
 
 The decoder's own step rotates whole heads, half against half, out of a bf16 table of its cache's
-length (``model.rope_tables``, ``fast.py``; ``paged.paged_write`` takes such tables too).  This is
-for what tables do not give: other layouts, part of a head, frequencies scaled for long contexts,
-positions of which no table is held.
+length (``model.rope_tables``, ``fast.py``).  ``paged.paged_write`` takes such tables too, and where
+they do (whole heads, half against half, any frequencies, a row for each position) it norms, rotates
+and writes in one launch, which is the faster way: 16 rows 2.9 us against 6.1 for the two launches
+below.  This is for what tables do not give: other layouts, part of a head, positions of which no
+table is held.
 
 Rows that go into a paged cache are rotated where they lie, in the q | k | v matrix, and then
 written as they are::
