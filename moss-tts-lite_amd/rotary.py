@@ -71,8 +71,8 @@ def rotary_freqs(turned: int, base: float = 10000.0, factor: float = 1.0,
 def _kept_by_dims(t: torch.Tensor, turned: int, base: float, original: int, slow: float,
                   fast: float) -> torch.Tensor:
     """How much of dim t's own frequency stays where it falls evenly over the dims."""
-    if not (base > 1 and slow > 0):
-        raise RuntimeError('base must be above 1 and slow above 0 for ramp="dims"')
+    if not (base > 1 and slow > 0 and all(math.isfinite(x) for x in (base, original, fast))):
+        raise RuntimeError('base must be above 1, slow above 0 and all finite for ramp="dims"')
     a, b = (turned * math.log(original / (2 * math.pi * n)) / (2 * math.log(base))
             for n in (fast, slow))
     a, b = max(math.floor(a), 0), min(math.ceil(b), turned - 1)

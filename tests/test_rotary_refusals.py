@@ -162,3 +162,10 @@ def test_frequencies_of_short_contexts():
     for kw in (dict(ramp="dim"), dict(base=1.0), dict(base=0.5), dict(slow=0.0)):
         with pytest.raises(RuntimeError):
             rotary.rotary_freqs(**{**dict(turned=64, factor=4.0, original=100, device="cpu"), **kw})
+
+
+def test_infinite_settings_of_frequencies():
+    inf = float("inf")
+    for kw in (dict(original=inf), dict(fast=inf), dict(base=inf), dict(slow=float("nan"))):
+        with pytest.raises(RuntimeError):
+            rotary.rotary_freqs(**{**dict(turned=64, factor=4.0, original=100, device="cpu"), **kw})
